@@ -129,21 +129,27 @@ def prepare(case, seed):
 # ---- the plain form: elementary operations in 32 bits, in 64 where a sum or a sign asks for them -------------------------
 
 
+def _threshold(rate):
+    """A rate counts in steps of 2^-16."""
+    return math.floor(rate * 65536 + 0.5)
+
+
 def _keep(rng, rate, count, device):
-    """Truth values, one for each element by its number: Philox4x32-10 (Salmon, Moraes, Dror and Shaw, 2011) with the counter
-    (number / 4, offset) and the seed as key gives four 32-bit words, the element of number i takes word i % 4, and is kept
-    where that word is at least rate * 2^32."""
+    """Truth values, one for each element by its number: Philox4x32-7 (Salmon, Moraes, Dror and Shaw, 2011) with the counter
+    (number / 8, offset) and the seed as key gives eight pieces of 16 bits, the element of number i takes piece i % 8, counted
+    from the lowest bits of the first word, and is kept where that piece is at least rate * 2^16."""
     low = 0xFFFFFFFF
-    block = torch.arange((count + 3) // 4, dtype=torch.int64, device=device)
+    block = torch.arange((count + 7) // 8, dtype=torch.int64, device=device)
     a, b = block & low, block >> 32
     c = (rng[1] & low).expand_as(block)
     d = ((rng[1] >> 32) & low).expand_as(block)
     k0, k1 = rng[0] & low, (rng[0] >> 32) & low
-    for _ in range(10):
+    for _ in range(7):
         p, q = a * 0xD2511F53, c * 0xCD9E8D57           # modulo 2^64: the shifts below take its words apart
         a, b, c, d = ((q >> 32) & low) ^ b ^ k0, q & low, ((p >> 32) & low) ^ d ^ k1, p & low
         k0, k1 = (k0 + 0x9E3779B9) & low, (k1 + 0xBB67AE85) & low
-    return torch.stack([a, b, c, d], dim=1).reshape(-1)[:count] >= math.floor(rate * 2.0 ** 32 + 0.5)
+    pieces = [t for word in (a, b, c, d) for t in (word & 0xFFFF, word >> 16)]
+    return torch.stack(pieces, dim=1).reshape(-1)[:count] >= _threshold(rate)
 
 
 def _last(t):
@@ -156,7 +162,7 @@ def _first(t, like):
 
 
 def _drop(t, keep, rate):
-    return torch.where(keep, t * (1.0 / (1.0 - rate)), torch.zeros((), device=t.device))
+    return torch.where(keep, t * (65536 / (65536 - _threshold(rate))), torch.zeros((), device=t.device))
 
 
 def _act(u, act):
@@ -295,7 +301,7 @@ def work(case):
 
 
 def _words(seed, offset, count, device):
-    """The generator's words, products taken apart into pieces of 16 bits."""
+    """The generator's pieces of 16 bits, products taken apart into pieces of 16 bits."""
     half, low = 0xFFFF, 0xFFFFFFFF
 
     def product(x, k):
@@ -304,14 +310,14 @@ def _words(seed, offset, count, device):
         side = x0 * k1 + (mid & half)
         return x1 * k1 + (mid >> 16) + (side >> 16), ((side & half) << 16) | ((x0 * k0) & half)
 
-    i = torch.arange((count + 3) // 4, dtype=torch.int64, device=device)
+    i = torch.arange((count + 7) // 8, dtype=torch.int64, device=device)
     v = [i % 2 ** 32, i // 2 ** 32, torch.full_like(i, offset & low), torch.full_like(i, (offset >> 32) & low)]
     key = [seed & low, (seed >> 32) & low]
-    for turn in range(10):
+    for turn in range(7):
         h0, l0 = product(v[0], 0xD2511F53)
         h1, l1 = product(v[2], 0xCD9E8D57)
         v = [h1 ^ v[1] ^ ((key[0] + turn * 0x9E3779B9) & low), l1, h0 ^ v[3] ^ ((key[1] + turn * 0xBB67AE85) & low), l0]
-    return torch.stack(v, dim=1).view(-1)[:count]
+    return torch.stack([t for word in v for t in (word % 65536, word // 65536)], dim=1).view(-1)[:count]
 
 
 def exact(case, seed):
@@ -323,7 +329,8 @@ def exact(case, seed):
     if case.get("rate", 0) > 0:
         key, offset = s["rng"].tolist()
         words = _words(key, offset, ins[0].numel(), ins[0].device).view(N, -1, C).movedim(2, 1).reshape(shape)
-        factor = (words.double() / 2 ** 32 >= math.floor(case["rate"] * 2.0 ** 32 + 0.5) / 2 ** 32).double() / (1 - case["rate"])
+        rate = round(case["rate"] * 65536) / 65536
+        factor = (words.double() / 65536 >= rate).double() / (1 - rate)
         del words
     leaves = list(ins)
     if kind == "dropout":
