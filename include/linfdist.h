@@ -46,6 +46,21 @@ extern "C" {
 #define LINF_ERR_LAUNCH     5   /* the CUDA runtime reported an error at launch         */
 #define LINF_ERR_WORKSPACE  6   /* workspace missing, misaligned or too small           */
 #define LINF_ERR_TOO_LARGE  7   /* size beyond a documented fixed maximum               */
+#define LINF_ERR_TYPE       8   /* unknown element type, or parameters of another one   */
+#define LINF_ERR_RATE       9   /* dropout rate outside [0, 1], or > 0 without a state  */
+#define LINF_ERR_EPS       10   /* eps is NaN, infinite or <= 0                         */
+#define LINF_ERR_ACT       11   /* unknown activation                                   */
+
+/* Element types of the operators between two layers. */
+#define LINF_F32   0
+#define LINF_F16   1
+#define LINF_BF16  2
+
+/* Activations behind a group norm. */
+#define LINF_ACT_IDENTITY  0
+#define LINF_ACT_RELU      1
+#define LINF_ACT_TANH      2
+#define LINF_ACT_SILU      3   /* u / (1 + e^-u) */
 
 /* Library version as major*10000 + minor*100 + patch. */
 int linf_version(void);
@@ -347,6 +362,58 @@ int linf_flag_publish(int* flag, int value, void* stream);
 int linf_flags_wait(const int* const* flags, int n, int value, int timeout_ms, int* err, void* stream);
 int linf_grad_rows_merge(float* grad, int rows, int cols, int cap, const int* const* cnts, const void* const* ents,
                          int world, float scale, const int* err, void* stream);
+
+/* ---------------------------------------------------------------------------------
+ * operators between two layers (no counterpart in the reference)
+ * --------------------------------------------------------------------------------- */
+
+/*
+ * Dropout of one to three tensors of n elements under one mask (a value with its lower and upper bounds); a tensor that is
+ * not given is NULL, with its output.  Element i is kept iff piece i % 8 (16 bits, lowest first) of the words that Philox4x32
+ * with 7 rounds gives for the counter (i / 8, offset) under the key `seed` is at least t = round(rate * 2^16); a kept element is
+ * multiplied by 2^16 / (2^16 - t), a dropped one is 0 whatever it was.  So rates count in steps of 2^-16, and at t = 0 every
+ * element stays as it is.  rng points at {seed, offset} on the device.  No mask is stored: the backward pass is the same
+ * call on the gradients.  An output may be its own input.
+ */
+int linf_dropout(const void* x, const void* lower, const void* upper, long long n, int type, double rate, const long long* rng,
+                 void* y, void* y_lower, void* y_upper, void* stream);
+
+/* used = {seed, offset} of `state`, whose offset then rises by 1 (atomically): the pair to draw one mask with. */
+int linf_dropout_next(long long* state, long long* used, void* stream);
+
+/*
+ * Group norm of x [N, L, C], channels last: C/G neighbouring channels over all L positions of a sample form a group,
+ *   h = (x - mean) / sqrt(var + eps),   u = gamma[c] h + beta[c],   y = dropout(activation(u))
+ * gamma, beta: [C] of param_type (fp32 or the type of x), each may be NULL (1 and 0).  rate > 0 drops elements of y under rng as
+ * linf_dropout does, numbered as they lie in memory.  mean, rstd [N, G] (fp32) are kept for the backward pass, or both NULL.
+ * fp32 inside whatever the type; one rounding at the end.  The workspace (16-byte aligned) has
+ * linf_group_norm_workspace_bytes(...) bytes.  N * L * C may exceed 2^31.
+ */
+size_t linf_group_norm_workspace_bytes(int N, int C, int G, int L, int type, int backward);
+int linf_group_norm_forward(const void* x, const void* gamma, const void* beta, int N, int C, int G, int L, int type, int param_type,
+                            double eps, int activation, double rate, const long long* rng, void* y, float* mean, float* rstd,
+                            void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients; grad_x, grad_gamma, grad_beta: each may be NULL, not all.  rate and rng as in the forward call.  Sums have a fixed order. */
+int linf_group_norm_backward(const void* grad_output, const void* x, const void* gamma, const void* beta, const float* mean,
+                             const float* rstd, int N, int C, int G, int L, int type, int param_type, int activation, double rate,
+                             const long long* rng, void* grad_x, void* grad_gamma, void* grad_beta, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/*
+ * Bounds of a group norm with its activation over the box lower <= x <= upper, fp32, same layout: for every x in the box
+ * output_lower <= activation(u) <= output_upper up to the rounding of the results.  The exact range of x_i - mean(x) is divided by
+ * the range of the deviation, [max(0, std(c) - rho), std(c) + rho] with c the box's centre and rho the root mean square of
+ * its radii.  sums [N, G, 4] (64 bits) is kept for the backward pass, or NULL.  Computed in 64 bits, rounded once.
+ */
+size_t linf_group_norm_bound_workspace_bytes(int N, int C, int G, int L, int backward);
+int linf_group_norm_bound_forward(const float* lower, const float* upper, const float* gamma, const float* beta, int N, int C, int G,
+                                  int L, double eps, int activation, float* output_lower, float* output_upper, double* sums,
+                                  void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients of both bounds.  grad_in_lower and grad_in_upper are NULL together; grad_gamma, grad_beta may be NULL. */
+int linf_group_norm_bound_backward(const float* grad_lower, const float* grad_upper, const float* lower, const float* upper,
+                                   const float* gamma, const float* beta, const double* sums, int N, int C, int G, int L, double eps,
+                                   int activation, float* grad_in_lower, float* grad_in_upper, float* grad_gamma, float* grad_beta,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------
  * tuning hook (benchmarks and tests only; no counterpart in the reference)

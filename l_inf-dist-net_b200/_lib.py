@@ -6,7 +6,7 @@ import subprocess
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "liblinfdist.so")
 CSRC = os.path.join(_HERE, "csrc")
-SOURCES = ["adamw.cu", "api.cu", "epilogue.cu", "sparse_exchange.cu", "inf_forward.cu", "inf_prune.cu", "inf_bound.cu", "inf_backward.cu", "inf_backward_accum.cu", "inf_backward_direct.cu", "lp.cu", "lp_tiled.cu", "lp_forward.cu", "lp_backward.cu", "no_alloc.cu", "skinny.cu", "few_rows.cu", "patches.cu"]
+SOURCES = ["adamw.cu", "api.cu", "epilogue.cu", "sparse_exchange.cu", "inf_forward.cu", "inf_prune.cu", "inf_bound.cu", "inf_backward.cu", "inf_backward_accum.cu", "inf_backward_direct.cu", "lp.cu", "lp_tiled.cu", "lp_forward.cu", "lp_backward.cu", "no_alloc.cu", "skinny.cu", "few_rows.cu", "patches.cu", "dropout.cu", "group_norm.cu", "group_norm_bound.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
               "--shared", "-Xcompiler", "-fPIC"]
 
@@ -50,6 +50,17 @@ _PROTOS = {
     "linf_norm_dist_forward_ws": [_F, _F, _INT, _INT, _INT, _INT, _INT, _F, ctypes.c_float, _F, ctypes.c_size_t, _F],
     "linf_norm_dist_backward_workspace_bytes": [_INT, _INT, _INT, _INT, _INT, ctypes.c_float, _INT, _INT],
     "linf_norm_dist_backward": [_F, _F, _F, _F, _INT, _INT, _INT, _INT, _INT, _F, _F, ctypes.c_float, _F, ctypes.c_size_t, _F],
+    "linf_dropout": [_F, _F, _F, ctypes.c_longlong, _INT, ctypes.c_double, _F, _F, _F, _F, _F],
+    "linf_dropout_next": [_F, _F, _F],
+    "linf_group_norm_workspace_bytes": [_INT, _INT, _INT, _INT, _INT, _INT],
+    "linf_group_norm_forward": [_F, _F, _F, _INT, _INT, _INT, _INT, _INT, _INT, ctypes.c_double, _INT, ctypes.c_double, _F, _F, _F, _F, _F,
+                                ctypes.c_size_t, _F],
+    "linf_group_norm_backward": [_F, _F, _F, _F, _F, _F, _INT, _INT, _INT, _INT, _INT, _INT, _INT, ctypes.c_double, _F, _F, _F, _F, _F,
+                                 ctypes.c_size_t, _F],
+    "linf_group_norm_bound_workspace_bytes": [_INT, _INT, _INT, _INT, _INT],
+    "linf_group_norm_bound_forward": [_F, _F, _F, _F, _INT, _INT, _INT, _INT, ctypes.c_double, _INT, _F, _F, _F, _F, ctypes.c_size_t, _F],
+    "linf_group_norm_bound_backward": [_F, _F, _F, _F, _F, _F, _F, _INT, _INT, _INT, _INT, ctypes.c_double, _INT, _F, _F, _F, _F, _F,
+                                       ctypes.c_size_t, _F],
 }
 _RESTYPE = {
     "linf_error_string": ctypes.c_char_p,
@@ -57,6 +68,8 @@ _RESTYPE = {
     "linf_inf_dist_forward_workspace_bytes": ctypes.c_size_t,
     "linf_norm_dist_forward_workspace_bytes": ctypes.c_size_t,
     "linf_norm_dist_backward_workspace_bytes": ctypes.c_size_t,
+    "linf_group_norm_workspace_bytes": ctypes.c_size_t,
+    "linf_group_norm_bound_workspace_bytes": ctypes.c_size_t,
     "linf_inf_dist_forward_pruned_workspace_bytes": ctypes.c_size_t,
     "linf_inf_dist_bound_pruned_workspace_bytes": ctypes.c_size_t,
 }
@@ -69,7 +82,7 @@ _lib = None
 def build(force=False, verbose=False):
     """Compiles csrc/*.cu for sm_100a into liblinfdist.so next to this file."""
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    deps = srcs + [os.path.join(CSRC, "common.cuh"),
+    deps = srcs + [os.path.join(CSRC, "common.cuh"), os.path.join(CSRC, "vec.cuh"), os.path.join(CSRC, "group_norm.cuh"),
                    os.path.join(_HERE, "..", "include", "linfdist.h")]
     if not force and os.path.exists(LIB_PATH):
         t = os.path.getmtime(LIB_PATH)

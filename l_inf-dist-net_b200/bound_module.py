@@ -4,13 +4,16 @@
 API mirror of model/bound_module.py of zbh2047/L_inf-dist-net (BoundReLU :5-12, BoundTanh
 :14-21, BoundLinear :28-46, BoundFinalLinear :48-68, BoundMeanNorm :70-93, BoundFinalIdentity
 :95-103, Predictor :105-116).  These are small dense GEMMs and elementwise maps; they run on
-stock torch ops (cuBLAS), not on custom kernels.
+stock torch ops (cuBLAS), not on custom kernels; the group norm and the dropout that a Predictor may
+have between its layers run on kernels of their own (group_norm.py, dropout.py).
 """
 import math
 
 import torch
 import torch.nn as nn
 
+from .dropout import BoundDropout
+from .group_norm import BoundGroupNorm
 from .norm_dist import MeanNorm
 
 
@@ -115,14 +118,26 @@ class BoundFinalIdentity(nn.Module):
 
 
 class Predictor(nn.Module):
-    """BoundLinear -> tanh -> BoundFinalLinear head used by the '++' nets."""
+    """BoundLinear -> tanh -> BoundFinalLinear head used by the '++' nets.  groups: the hidden units go through a group norm of
+    that many groups before the tanh (one kernel for both); dropout: rate at which hidden units are dropped while training."""
 
-    def __init__(self, in_features, hidden, out_dim):
+    def __init__(self, in_features, hidden, out_dim, groups=None, dropout=0.0):
         super().__init__()
         self.fc1 = BoundLinear(in_features, hidden, bias=True)
-        self.tanh = BoundTanh()
+        if groups is None:
+            self.tanh = BoundTanh()
+            self.drop = BoundDropout(dropout) if dropout > 0 else None
+        else:
+            self.norm = BoundGroupNorm(groups, hidden, activation="tanh", dropout=dropout)
+        self.groups = groups
         self.fc2 = BoundFinalLinear(hidden, out_dim)
 
     def forward(self, x, lower=None, upper=None, targets=None):
-        triple = self.tanh(*self.fc1(x, lower, upper))
+        triple = self.fc1(x, lower, upper)
+        if self.groups is not None:
+            triple = self.norm(*triple)
+        else:
+            triple = self.tanh(*triple)
+            if self.drop is not None:
+                triple = self.drop(*triple)
         return self.fc2(*triple, targets=targets)

@@ -97,6 +97,10 @@ using namespace linf;
 
 namespace {
 inline bool bad_p(float p) { return !(p > 1.f) || isinf(p); }
+inline bool bad_type(int t) { return t != LINF_F32 && t != LINF_F16 && t != LINF_BF16; }
+inline bool bad_act(int a) { return a < LINF_ACT_IDENTITY || a > LINF_ACT_SILU; }
+inline bool bad_eps(double e) { return !(e > 0.f) || isinf(e); }
+inline bool bad_rate(double r, const long long* rng) { return !(r >= 0.0 && r <= 1.0) || (r > 0.0 && rng == nullptr); }
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 }  // namespace
 
@@ -116,6 +120,10 @@ const char* linf_error_string(int code) {
         case LINF_ERR_LAUNCH: return "CUDA reported an error at kernel launch";
         case LINF_ERR_WORKSPACE: return "workspace is missing, misaligned or too small";
         case LINF_ERR_TOO_LARGE: return "size exceeds a fixed maximum of this entry point";
+        case LINF_ERR_TYPE: return "element type is none of LINF_F32, LINF_F16, LINF_BF16, or parameters are neither fp32 nor of that type";
+        case LINF_ERR_RATE: return "dropout rate must lie in [0, 1], and a rate above 0 needs a generator state";
+        case LINF_ERR_EPS: return "eps must be finite and greater than 0";
+        case LINF_ERR_ACT: return "unknown activation";
         default: return "unknown error code";
     }
 }
@@ -374,6 +382,84 @@ int linf_fold_rows(const float* rows, int B, int C, int H, int W, int kernel_siz
                    float* grad_input, void* stream) {
     if (!rows || !grad_input) return LINF_ERR_NULL;
     return fold_rows(rows, B, C, H, W, kernel_size, dilation, padding, stride, grad_input, as_stream(stream));
+}
+
+int linf_dropout_next(long long* state, long long* used, void* stream) {
+    if (!state || !used) return LINF_ERR_NULL;
+    return dropout_next(state, used, as_stream(stream));
+}
+
+int linf_dropout(const void* x, const void* lower, const void* upper, long long n, int type, double rate, const long long* rng,
+                 void* y, void* y_lower, void* y_upper, void* stream) {
+    const void* all[3] = {x, lower, upper};
+    void* outs[3] = {y, y_lower, y_upper};
+    const void* in[3];
+    void* out[3];
+    int tensors = 0;
+    for (int k = 0; k < 3; ++k) {
+        if ((all[k] == nullptr) != (outs[k] == nullptr)) return LINF_ERR_NULL;
+        if (all[k] != nullptr) { in[tensors] = all[k]; out[tensors++] = outs[k]; }
+    }
+    if (tensors == 0) return LINF_ERR_NULL;
+    if (n <= 0) return LINF_ERR_DIMS;
+    if (bad_type(type)) return LINF_ERR_TYPE;
+    if (bad_rate(rate, rng)) return LINF_ERR_RATE;
+    return dropout(in, out, tensors, n, type, rate, rng, as_stream(stream));
+}
+
+size_t linf_group_norm_workspace_bytes(int N, int C, int G, int L, int type, int backward) {
+    if (bad_type(type)) return 0;
+    return group_norm_workspace(N, C, G, L, type, backward != 0);
+}
+
+int linf_group_norm_forward(const void* x, const void* gamma, const void* beta, int N, int C, int G, int L, int type, int param_type,
+                            double eps, int activation, double rate, const long long* rng, void* y, float* mean, float* rstd,
+                            void* workspace, size_t workspace_bytes, void* stream) {
+    if (!x || !y || (mean == nullptr) != (rstd == nullptr)) return LINF_ERR_NULL;
+    if (bad_type(type) || (param_type != LINF_F32 && param_type != type)) return LINF_ERR_TYPE;
+    if (bad_eps(eps)) return LINF_ERR_EPS;
+    if (bad_act(activation)) return LINF_ERR_ACT;
+    if (bad_rate(rate, rng)) return LINF_ERR_RATE;
+    return group_norm_forward(x, gamma, beta, N, C, G, L, type, param_type, eps, activation, rate, rng, y, mean, rstd, workspace,
+                              workspace_bytes, as_stream(stream));
+}
+
+int linf_group_norm_backward(const void* grad_output, const void* x, const void* gamma, const void* beta, const float* mean,
+                             const float* rstd, int N, int C, int G, int L, int type, int param_type, int activation, double rate,
+                             const long long* rng, void* grad_x, void* grad_gamma, void* grad_beta, void* workspace,
+                             size_t workspace_bytes, void* stream) {
+    if (!grad_output || !x || !mean || !rstd || (!grad_x && !grad_gamma && !grad_beta)) return LINF_ERR_NULL;
+    if (bad_type(type) || (param_type != LINF_F32 && param_type != type)) return LINF_ERR_TYPE;
+    if (bad_act(activation)) return LINF_ERR_ACT;
+    if (bad_rate(rate, rng)) return LINF_ERR_RATE;
+    return group_norm_backward(grad_output, x, gamma, beta, mean, rstd, N, C, G, L, type, param_type, activation, rate, rng, grad_x,
+                               grad_gamma, grad_beta, workspace, workspace_bytes, as_stream(stream));
+}
+
+size_t linf_group_norm_bound_workspace_bytes(int N, int C, int G, int L, int backward) {
+    return group_norm_bound_workspace(N, C, G, L, backward != 0);
+}
+
+int linf_group_norm_bound_forward(const float* lower, const float* upper, const float* gamma, const float* beta, int N, int C, int G,
+                                  int L, double eps, int activation, float* output_lower, float* output_upper, double* sums,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+    if (!lower || !upper || !output_lower || !output_upper) return LINF_ERR_NULL;
+    if (bad_eps(eps)) return LINF_ERR_EPS;
+    if (bad_act(activation)) return LINF_ERR_ACT;
+    return group_norm_bound_forward(lower, upper, gamma, beta, N, C, G, L, eps, activation, output_lower, output_upper, sums, workspace,
+                                    workspace_bytes, as_stream(stream));
+}
+
+int linf_group_norm_bound_backward(const float* grad_lower, const float* grad_upper, const float* lower, const float* upper,
+                                   const float* gamma, const float* beta, const double* sums, int N, int C, int G, int L, double eps,
+                                   int activation, float* grad_in_lower, float* grad_in_upper, float* grad_gamma, float* grad_beta,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+    if (!grad_lower || !grad_upper || !lower || !upper || !sums) return LINF_ERR_NULL;
+    if ((grad_in_lower == nullptr) != (grad_in_upper == nullptr) || (!grad_in_lower && !grad_gamma && !grad_beta)) return LINF_ERR_NULL;
+    if (bad_eps(eps)) return LINF_ERR_EPS;
+    if (bad_act(activation)) return LINF_ERR_ACT;
+    return group_norm_bound_backward(grad_lower, grad_upper, lower, upper, gamma, beta, sums, N, C, G, L, eps, activation, grad_in_lower,
+                                     grad_in_upper, grad_gamma, grad_beta, workspace, workspace_bytes, as_stream(stream));
 }
 
 }  // extern "C"

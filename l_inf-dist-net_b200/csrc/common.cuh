@@ -188,6 +188,22 @@ int inf_backward_ordered_both(const float* g, const int* pos, const Dims& d, flo
 // patches of a convolution-shaped layer as rows, and back (patches.cu)
 int unfold_rows(const float* x, int B, int C, int H, int W, int k, int dil, int pad, int stride, float* rows, cudaStream_t st);
 int fold_rows(const float* rows, int B, int C, int H, int W, int k, int dil, int pad, int stride, float* gx, cudaStream_t st);
+// dropout with a mask computed from (seed, offset, element number) (dropout.cu)
+int dropout(const void* const* in, void* const* out, int tensors, long long n, int type, double rate, const long long* rng, cudaStream_t st);
+int dropout_next(long long* state, long long* used, cudaStream_t st);
+// group norm, channels last, with activation and dropout (group_norm.cu), and over a box (group_norm_bound.cu)
+size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back);
+int group_norm_forward(const void* x, const void* gamma, const void* beta, int N, int C, int G, int L, int type, int ptype, double eps, int act,
+                       double rate, const long long* rng, void* y, float* mean, float* rstd, void* ws, size_t ws_bytes, cudaStream_t st);
+int group_norm_backward(const void* dy, const void* x, const void* gamma, const void* beta, const float* mean, const float* rstd, int N, int C,
+                        int G, int L, int type, int ptype, int act, double rate, const long long* rng, void* dx, void* dgamma, void* dbeta,
+                        void* ws, size_t ws_bytes, cudaStream_t st);
+size_t group_norm_bound_workspace(int N, int C, int G, int L, bool back);
+int group_norm_bound_forward(const float* lower, const float* upper, const float* gamma, const float* beta, int N, int C, int G, int L, double eps,
+                             int act, float* out_l, float* out_u, double* sums, void* ws, size_t ws_bytes, cudaStream_t st);
+int group_norm_bound_backward(const float* g_l, const float* g_u, const float* lower, const float* upper, const float* gamma, const float* beta,
+                              const double* sums, int N, int C, int G, int L, double eps, int act, float* d_l, float* d_u, float* dgamma,
+                              float* dbeta, void* ws, size_t ws_bytes, cudaStream_t st);
 // a handful of input rows (few_rows.cu)
 bool inf_few_rows_ok(const Dims& d, bool tiled);
 int inf_forward_few_rows(const float* x, const float* w, const Dims& d, float* y, int* pos, cudaStream_t st, const Post& post);

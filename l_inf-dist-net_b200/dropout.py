@@ -1,0 +1,148 @@
+"""Dropout whose mask is a function of (seed, offset, element number) and is never stored: forward and backward compute it
+again (csrc/dropout.cu; the generator is Philox4x32 with 7 rounds, 16 bits for each element).
+
+Beside the elementwise maps of the heads (BoundReLU, BoundTanh): `BoundDropout` maps a triple (value, lower, upper) under ONE
+mask, so that lower <= value <= upper still holds behind it.  zbh2047/L_inf-dist-net has no counterpart.
+"""
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .norm_dist import _on, _stream
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # LINF_F32, LINF_F16, LINF_BF16
+
+
+def _floating(t, name):
+    if t.dtype not in _TYPES:
+        raise RuntimeError(f"{name} must have dtype torch.float32, torch.float16 or torch.bfloat16")
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} must be a CUDA tensor")
+
+
+def _generator_state(rng, device):
+    if not (torch.is_tensor(rng) and rng.dtype == torch.int64 and rng.shape == (2,) and rng.is_contiguous()):
+        raise RuntimeError("rng must be a contiguous int64 tensor of two elements: seed and offset")
+    if rng.device != device:
+        raise RuntimeError("rng must be on the device of the tensors it drops elements of")
+
+
+def _rate(rate):
+    rate = float(rate)
+    if not 0.0 <= rate <= 1.0:
+        raise ValueError("the dropout rate must lie in [0, 1]")
+    return rate
+
+
+def _is_last(t):
+    """Whether the channels (dimension 1) lie last in memory, without gaps."""
+    return t.dim() > 2 and t.movedim(1, -1).is_contiguous()
+
+
+def _as_stored(t, last):
+    """t with its elements in memory order: as it is, or a copy."""
+    if t.is_contiguous() if not last else _is_last(t):
+        return t
+    return t.contiguous() if not last else t.movedim(1, -1).contiguous().movedim(-1, 1)
+
+
+def _launch(tensors, rate, rng):
+    outs = [None if t is None else torch.empty_like(t) for t in tensors]
+    some = next(t for t in tensors if t is not None)
+    if some.numel() == 0:
+        return outs
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    with _on(some.device):
+        rc = _lib.load().linf_dropout(*map(ptr, tensors), some.numel(), _TYPES[some.dtype], rate, rng.data_ptr(), *map(ptr, outs), _stream())
+    _lib.check(rc, "dropout")
+    return outs
+
+
+class DropoutF(torch.autograd.Function):
+    """The same mask on each of up to three tensors; the backward pass drops the gradients under it."""
+
+    @staticmethod
+    def forward(ctx, rate, rng, *tensors):
+        ctx.set_materialize_grads(False)
+        last = not tensors[0].is_contiguous() and _is_last(tensors[0])
+        ctx.last, ctx.rate = last, rate
+        ctx.save_for_backward(rng)
+        return tuple(_launch([_as_stored(t, last) for t in tensors] + [None] * (3 - len(tensors)), rate, rng)[:len(tensors)])
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        rng, = ctx.saved_tensors
+        asked = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[2:])]
+        given = [None if g is None else _as_stored(g, ctx.last) for g in asked]
+        if all(g is None for g in given):
+            return (None, None, *given)
+        return (None, None, *_launch(given + [None] * (3 - len(given)), ctx.rate, rng)[:len(given)])
+
+
+def dropout_next(state):
+    """{seed, offset} to draw one mask with, as a tensor of its own; the offset of `state` rises by 1.  Runs on the device, so a
+    captured graph draws another mask each time it is replayed, and calls on several streams never get the same offset."""
+    _generator_state(state, state.device)
+    if not state.is_cuda:
+        raise RuntimeError("rng must be a CUDA tensor")
+    used = torch.empty_like(state)
+    with _on(state.device):
+        rc = _lib.load().linf_dropout_next(state.data_ptr(), used.data_ptr(), _stream())
+    _lib.check(rc, "dropout_next")
+    torch.autograd.graph.increment_version(state)       # a backward pass that was to read `state` itself is refused by autograd
+    return used
+
+
+def dropout(x, rate, rng, lower=None, upper=None):
+    """x with each element dropped (0) with probability `rate`, the others multiplied by 1 / (1 - rate); with lower / upper the
+    triple under one mask.  fp32, fp16 or bf16.
+
+    rng: int64 CUDA tensor {seed, offset}; the same pair gives the same mask (see `dropout_next`), and it has to hold its values
+    until the backward pass.  Rates count in steps of 2^-16, the scale makes up for that.  Elements are numbered as they lie
+    in memory where x is contiguous or has its channels last; another layout is copied to a contiguous one first, and
+    lower / upper to the layout of x."""
+    rate = _rate(rate)
+    tensors = [x] + [t for t in (lower, upper) if t is not None]
+    if (lower is None) != (upper is None):
+        raise RuntimeError("lower and upper are given together")
+    for t, name in zip(tensors[1:], ("lower", "upper")):
+        if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+            raise RuntimeError(f"{name} must have the shape, dtype and device of x")
+    _generator_state(rng, x.device)
+    _floating(x, "x")
+    outs = DropoutF.apply(rate, rng, *tensors)
+    return outs[0] if lower is None else outs
+
+
+class _Masks(nn.Module):
+    """Keeps the generator state of a module that drops elements: a buffer `rng` of {seed, offset}."""
+
+    def _make_masks(self, rate, seed):
+        self.rate = _rate(rate)
+        if self.rate > 0:
+            seed = int(torch.randint(0, 2 ** 62, ())) if seed is None else int(seed)
+            self.register_buffer("rng", torch.tensor([seed, 0], dtype=torch.int64))
+
+
+class BoundDropout(_Masks):
+    """Dropout of a triple (value, lower, upper) while training; nothing in eval mode.  Every forward pass draws a mask of its own.
+    seed: by default a number from torch's CPU generator.  Replicas of a data-parallel job need seeds of their own."""
+
+    def __init__(self, rate, seed=None):
+        super().__init__()
+        self._make_masks(rate, seed)
+
+    def forward(self, x, lower=None, upper=None):
+        if lower is None or upper is None:
+            lower = upper = None
+        if not self.training or self.rate == 0:
+            return x, lower, upper
+        used = dropout_next(self.rng)
+        if lower is None:
+            return dropout(x, self.rate, used), None, None
+        return dropout(x, self.rate, used, lower, upper)
+
+    def extra_repr(self):
+        return f"rate={self.rate}"

@@ -368,6 +368,11 @@ class bounds_only:
         _bounds_only = self.saved
 
 
+def skips_values():
+    """Whether a `bounds_only` block is open."""
+    return _bounds_only
+
+
 def set_fused_epilogue(flag):
     """True (default): on CUDA, dense layers run the training-mode mean shift as one launch and fold the
     eval-mode mean shift / bias / sign flip into the forward and bound kernels.  False: the same steps as
@@ -410,18 +415,19 @@ class MeanNorm(nn.Module):
 
 class NormDistConv(nn.Module):
     """Convolution-shaped distance layer: every output is the L_p distance between an input
-    patch and a weight row.  state_dict keys match the reference: weight [CO, CI/group, k, k],
+    patch and a weight row.  channels_last=True leaves the output of a call without bounds as the rows have it, channels last
+    in memory (what `group_norm` takes without a copy), where it is made of patch rows.  state_dict keys match the reference: weight [CO, CI/group, k, k],
     optional bias [CO], optional normalize.running_mean [CO]."""
 
     tag_counter = 0
 
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1, group=1, p=0,
-                 bias=True, mean_normalize=False, identity_init=True):
+                 bias=True, mean_normalize=False, identity_init=True, channels_last=False):
         super().__init__()
         assert in_channels % group == 0 and out_channels % group == 0
         self.in_channels, self.out_channels = in_channels, out_channels
         self.kernel_size, self.stride, self.padding, self.dilation = kernel_size, stride, padding, dilation
-        self.group, self.p = group, p
+        self.group, self.p, self.channels_last = group, p, channels_last
         per_group = in_channels // group
         w = torch.randn(out_channels, per_group, kernel_size, kernel_size)
         if identity_init and in_channels <= out_channels:
@@ -474,7 +480,8 @@ class NormDistConv(nn.Module):
             # the patches go straight into the rows of a dense layer (DistF would copy them there)
             rows = PatchRowsF.apply(x, self.kernel_size, self.dilation, self.padding, self.stride, ho * wo)
             y = norm_dist(rows, weight, self.group, p=self.p, tag=self.tag)
-            y = self._post(y.view(x.size(0), ho, wo, -1).permute(0, 3, 1, 2).contiguous())
+            y = y.view(x.size(0), ho, wo, -1).permute(0, 3, 1, 2)
+            y = self._post(y if self.channels_last else y.contiguous())
             return (-y if negate else y), None, None
         cols = self._patches(x)
         post = self._fused_post(negate)

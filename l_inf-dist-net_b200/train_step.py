@@ -67,13 +67,14 @@ def build_cifar_net(device, depth=5, width=5, p=float("inf"), eps=8.0 / 255.0, s
     return net
 
 
-def build_tiny_net(device, depth=5, width=5, hidden=512, p=float("inf"), eps=1.0 / 255.0, seed=2020):
+def build_tiny_net(device, depth=5, width=5, hidden=512, p=float("inf"), eps=1.0 / 255.0, seed=2020,
+                   groups=None, dropout=0.0):
     """The '++' variant on TinyImageNet-shaped inputs (3x64x64 = 12288 features, 200 classes): `depth`
     distance layers as feature extractor, then the reference's BoundLinear -> tanh -> BoundFinalLinear
-    head (model/bound_module.py:105-116; the reference head uses tanh, not ReLU)."""
+    head (model/bound_module.py:105-116; the reference head uses tanh, not ReLU).  groups, dropout: of the Predictor."""
     torch.manual_seed(seed)
     feat = MLPFeature(depth, width, (3, 64, 64))
-    net = Model(feat, Predictor(feat.out_features, hidden, 200), eps).to(device)
+    net = Model(feat, Predictor(feat.out_features, hidden, 200, groups=groups, dropout=dropout), eps).to(device)
     set_p_norm(net, p)
     return net
 
