@@ -33,34 +33,41 @@ template <typename T> struct Eight {
     }
 };
 
-template <typename T, bool WIDE>
+template <typename T, bool WIDE, int TENSORS>
 __global__ void __launch_bounds__(256)
-dropout_kernel(Tensors t, int tensors, long long n, Drop d) {
+dropout_kernel(Tensors t, long long n, Drop d) {
     const DropKey key = drop_key(d);
     const long long step = (long long)gridDim.x * blockDim.x;
     for (long long b = (long long)blockIdx.x * blockDim.x + threadIdx.x; b * 8 < n; b += step) {
         const bool whole = WIDE && b * 8 + 8 <= n;
-        float keep[8];
+        float f[TENSORS][8];
+        if (whole) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) keep[j] = 1.f;
-        drop_apply<8>(d, key, (unsigned long long)b * 8, keep);
-        for (int k = 0; k < tensors; ++k) {
-            const T* in = static_cast<const T*>(t.in[k]) + b * 8;
-            T* out = static_cast<T*>(t.out[k]) + b * 8;
-            float f[8];
-            if (whole) {
-                Eight<T>::load(in, f);
+            for (int k = 0; k < TENSORS; ++k) Eight<T>::load(static_cast<const T*>(t.in[k]) + b * 8, f[k]);
+        } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) f[j] = keep[j] != 0.f ? f[j] * keep[j] : 0.f;
-                Eight<T>::store(out, f);
-            } else {
+            for (int k = 0; k < TENSORS; ++k)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    if (b * 8 + j < n) {
-                        const float v = to_float<T>(in[j]);
-                        out[j] = from_float<T>(keep[j] != 0.f ? v * keep[j] : 0.f);
-                    }
-            }
+                    if (b * 8 + j < n) f[k][j] = to_float<T>(static_cast<const T*>(t.in[k])[b * 8 + j]);
+        }
+        const uint4 w = drop_words(key, (unsigned long long)b);
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const unsigned piece = (j & 1) ? u[j >> 1] >> 16 : u[j >> 1] & 0xffffu;
+#pragma unroll
+            for (int k = 0; k < TENSORS; ++k) f[k][j] = drop_one(d, piece, f[k][j]);
+        }
+        if (whole) {
+#pragma unroll
+            for (int k = 0; k < TENSORS; ++k) Eight<T>::store(static_cast<T*>(t.out[k]) + b * 8, f[k]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < TENSORS; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (b * 8 + j < n) static_cast<T*>(t.out[k])[b * 8 + j] = from_float<T>(f[k][j]);
         }
     }
 }
@@ -70,15 +77,19 @@ __global__ void dropout_next_kernel(long long* state, long long* used) {
     used[1] = (long long)atomicAdd(reinterpret_cast<unsigned long long*>(state + 1), 1ull);
 }
 
-template <typename T>
-int launch(const Tensors& t, int tensors, long long n, const Drop& d, cudaStream_t st) {
+template <typename T, int TENSORS>
+int launch(const Tensors& t, long long n, const Drop& d, cudaStream_t st) {
     bool wide = true;
-    for (int k = 0; k < tensors; ++k) wide = wide && aligned16(t.in[k]) && aligned16(t.out[k]);
+    for (int k = 0; k < TENSORS; ++k) wide = wide && aligned16(t.in[k]) && aligned16(t.out[k]);
     const long long blocks = (n + 8 * 256 - 1) / (8 * 256), most = (long long)sm_count() * 64;
     const int grid = (int)(blocks < most ? blocks : most);
-    if (wide) dropout_kernel<T, true><<<grid, 256, 0, st>>>(t, tensors, n, d);
-    else dropout_kernel<T, false><<<grid, 256, 0, st>>>(t, tensors, n, d);
+    if (wide) dropout_kernel<T, true, TENSORS><<<grid, 256, 0, st>>>(t, n, d);
+    else dropout_kernel<T, false, TENSORS><<<grid, 256, 0, st>>>(t, n, d);
     return launch_status();
+}
+template <typename T>
+int launch(const Tensors& t, int tensors, long long n, const Drop& d, cudaStream_t st) {
+    return tensors == 1 ? launch<T, 1>(t, n, d, st) : tensors == 2 ? launch<T, 2>(t, n, d, st) : launch<T, 3>(t, n, d, st);
 }
 
 }  // namespace
@@ -86,7 +97,7 @@ int launch(const Tensors& t, int tensors, long long n, const Drop& d, cudaStream
 int dropout(const void* const* in, void* const* out, int tensors, long long n, int type, double rate, const long long* rng, cudaStream_t st) {
     Drop d;
     if (!make_drop(rate, rng, &d)) return LINF_ERR_RATE;
-    if (d.rng == nullptr) {                                     // nothing is dropped: every element as it is, a NaN's bits included
+    if (!d.on) {                                     // nothing is dropped: every element as it is, a NaN's bits included
         for (int k = 0; k < tensors; ++k)
             if (out[k] != in[k] &&
                 cudaMemcpyAsync(out[k], in[k], (size_t)n * (type == LINF_F32 ? 4 : 2), cudaMemcpyDeviceToDevice, st) != cudaSuccess)

@@ -4,247 +4,575 @@
 //   dbeta = sum du, dgamma = sum du h (over samples and positions),
 //   dx = (gamma du - mean(gamma du) - h mean(gamma du h)) / sqrt(var + eps)
 //
-// Two passes: sums of each (sample, row range, group), then the elementwise pass, whose CTAs first add up the few sums of
-// their groups.  The order of every addition is fixed by the shape alone.
-//
-// The forward sums are x and x^2 in 64 bits: (sum x^2) / M - mean^2 then keeps the variance of data whose mean is up to 10^6 times
-// their spread, in one pass over them (activations of distance layers are all positive, far from 0 against their spread).
+// Bound by HBM: every tensor once in or out (16-bit types come near the issue limit as well).  The sums of the kept form are a mean and a
+// sum of squared deviations (of a thread's values, of a column's, of a group's), joined by
+//   mean = sum n_i mean_i / n,  M2 = sum M2_i + sum n_i (mean_i - mean)^2;
+// row ranges of the two passes are joined as sums of x and x^2 in 64 bits: so data far from 0 against their spread (activations of distance layers are all
+// positive) lose nothing of their variance.  The order of every addition is fixed by the shape alone.
 #include "group_norm.cuh"
 
 namespace linf {
 namespace {
 
-// ---- forward ------------------------------------------------------------------------------------------------------
+// The values that stand for a gamma or beta that was not given.
+struct Own { float one, zero; };
+__device__ Own g_own = {1.f, 0.f};
 
+// What a thread's column needs for u = (x - m) a + o.
+template <int V> struct Column { float m[V], a[V], o[V]; };
+template <int V>
+__device__ __forceinline__ void load_column(Column<V>& k, const float2* stat, const Param& gamma, const Param& beta, const NormDims& d,
+                                            const NormPlan& p, const NormBlock& b, int cv) {
+    int g[V];
+    groups_of<V>(d, p, cv * V, g);
+    load_params<V>(gamma, b.c0 + cv * V, k.a);
+    load_params<V>(beta, b.c0 + cv * V, k.o);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 s = stat[g[j]];
+        k.m[j] = s.x;
+        k.a[j] *= s.y;
+    }
+}
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads)
-norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __restrict__ part) {
-    extern __shared__ double2 red[];                            // [rt][tx * V]
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
-    double s[V], q[V];
+__device__ __forceinline__ void write_vector(const Raw<T, V>& v, const Column<V>& col, int act, const Drop& drop, const DropKey& key, size_t i, T* y) {
+    float f[V];
+    unpack<T, V>(v, f);
+    sub_all<V>(f, f, col.m);
+    fma_all<V>(f, f, col.a, col.o);
+    activate_all<sizeof(T) == 4, V>(f, act);
+    if (drop.on) drop_apply<V>(drop, key, i, f);
+    store_once<T, V>(y + i, pack<T, V>(f));
+}
+__device__ __forceinline__ float2 finish_stat(double mean, double var, double eps) {
+    return make_float2((float)mean, 1.f / sqrtf((float)(var + eps)));
+}
+
+// A thread's sums of its column about its first row: s = sum (x - k), q = sum (x - k)^2.
+template <typename T, int V> struct Vec { float f[V]; };
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> load_raw_as(const T* p) { Vec<T, V> v; unpack<T, V>(load_raw<T, V>(p), v.f); return v; }
+template <typename T, int V>
+__device__ __forceinline__ Vec<T, V> as_vec(const Raw<T, V>& raw) { Vec<T, V> v; unpack<T, V>(raw, v.f); return v; }
+
+template <int V> struct Moments {
+    float k[V], s[V], q[V];
+    __device__ __forceinline__ Moments() {
 #pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = q[j] = 0.0;
-    if (rt < p.rt && cv < b.nvec) {
-        const int r1 = min(d.L, (split + 1) * p.rows);
-        const T* at = x + ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-        for (int r = split * p.rows + rt; r < r1; r += 4 * p.rt) {
-            Raw<T, V> v[4];
+        for (int j = 0; j < V; ++j) k[j] = s[j] = q[j] = 0.f;
+    }
+    template <typename T> __device__ __forceinline__ void start(const Vec<T, V>& v) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (r + k * p.rt < r1) v[k] = load_raw<T, V>(at + (size_t)(r + k * p.rt) * d.C);
+        for (int j = 0; j < V; ++j) k[j] = v.f[j];
+    }
+    template <typename T> __device__ __forceinline__ void add(Vec<T, V> v) {
+        sub_all<V>(v.f, v.f, k);
+        add_all<V>(s, s, v.f);
+        fma_all<V>(q, v.f, v.f, q);
+    }
+    // (mean, M2) of `count` rows into red: one pair for each channel, or for the vector where it lies in one group
+    __device__ __forceinline__ void put(float2* red, const NormPlan& p, int rt, int cv, int count) {
+        const float inv = count > 0 ? 1.f / (float)count : 0.f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (r + k * p.rt < r1) {
-                    float f[V];
-                    unpack<T, V>(v[k], f);
+        for (int j = 0; j < V; ++j) {
+            q[j] = fmaf(-s[j] * inv, s[j], q[j]);
+            s[j] = fmaf(s[j], inv, k[j]);
+        }
+        if (p.same) {
+            float m = s[0], t = q[0];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) { const double e = f[j]; s[j] += e; q[j] = fma(e, e, q[j]); }
-                }
+            for (int j = 1; j < V; ++j) { m += s[j]; t += q[j]; }
+            m *= 1.f / V;
+#pragma unroll
+            for (int j = 0; j < V; ++j) t = fmaf((float)count * (s[j] - m), s[j] - m, t);
+            red[rt * p.tx + cv] = make_float2(m, t);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) red[(rt * p.tx + cv) * V + j] = make_float2(s[j], q[j]);
         }
     }
-    const int width = p.tx * V;
-    if (rt < p.rt) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) red[rt * width + cv * V + j] = make_double2(s[j], q[j]);
-    }
+};
+
+// (mean, M2) of each group of the block over `rows` rows from what the threads put into red; done(g, mean, M2) in one lane.
+template <int V, typename Done>
+__device__ __forceinline__ void join_moments(float2* red, const NormDims& d, const NormPlan& p, const NormBlock& b, int rows, Done done) {
+    const int each = p.same ? V : 1, width = p.same ? p.tx : p.tx * V, lane = threadIdx.x & 31;
+    const int per = (p.pieces == 1 ? d.Cg : b.nvec * V) / each;         // columns of red of a group
     __syncthreads();
-    const int lane = threadIdx.x & 31;
-    const int per = p.pieces == 1 ? d.Cg : b.nvec * V;          // channels of a group in this block
-    for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        double a = 0.0, e = 0.0;
-        for (int c = lane; c < per; c += 32)
-            for (int r = 0; r < p.rt; ++r) {
-                const double2 v = red[r * width + g * per + c];
-                a += v.x;
-                e += v.y;
+    if (p.rt > 1) {
+        // columns along the rows, about the first row's mean
+        const int base = rows / p.rt, more = rows - base * p.rt;     // rows of a thread: one more in the first `more` of them
+        by_columns(width, p.rt, [&](int c, int first, int step, auto join) {
+            const float k0 = c < width ? red[c].x : 0.f, one = 1.f / (float)each;
+            float s = 0.f, q = 0.f;
+            for (int r = first; r < p.rt; r += step) {
+                const float2 v = red[r * width + c];
+                const float count = (float)(base + (r < more)), e = v.x - k0;
+                s = fmaf(count, e, s);
+                q = fmaf(count * e, e, fmaf(v.y, one, q));
             }
-        a = warp_sum(a);
-        e = warp_sum(e);
-        if (lane == 0) part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_double2(a, e);
+            if (join(s, q)) {
+                const float inv = 1.f / (float)rows;
+                red[c] = make_float2(fmaf(s, inv, k0), fmaf(-s * inv, s, q) * (float)each);
+            }
+        });
+        __syncthreads();
+    }
+    // groups along their columns, about the first column's mean: as many lanes to a group as the group has columns, up to a warp
+    int wide = 1;
+    while (wide < per && wide < 32) wide *= 2;
+    const float weight = 1.f / (float)(rows * each), share = 1.f / (float)per;
+    for (int g0 = (threadIdx.x >> 5) * (32 / wide); g0 < b.ng; g0 += (blockDim.x >> 5) * (32 / wide)) {
+        const int g = g0 + lane / wide;
+        float s = 0.f, q = 0.f, k0 = 0.f;
+        if (g < b.ng) {
+            k0 = red[g * per].x;
+            for (int c = lane & (wide - 1); c < per; c += wide) {
+                const float2 v = red[g * per + c];
+                const float e = v.x - k0;
+                s += e;
+                q = fmaf(e, e, fmaf(v.y, weight, q));
+            }
+        }
+        for (int o = 1; o < wide; o *= 2) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            q += __shfl_xor_sync(0xffffffffu, q, o);
+        }
+        if (g < b.ng && (lane & (wide - 1)) == 0) done(g, fmaf(s, share, k0), fmaf(-s * share, s, q) * (float)rows * (float)each);
     }
 }
 
+// ---- forward, kept --------------------------------------------------------------------------------------------------
+
+// Shared memory: the rows of all tensors, a pair for each thread and channel (or vector), the statistics of each group, and where elements are
+// dropped in a backward pass a byte for each vector: which of its elements are kept.  Offsets in bytes.
+struct KeptSpace { int red, stat, mask, bytes; };
+KeptSpace kept_space(const NormPlan& p, int elem_bytes, int tensors, bool by_vector, bool masks) {
+    KeptSpace s;
+    s.red = (p.rows * p.tx * p.V * elem_bytes * tensors + 15) / 16 * 16;
+    s.stat = s.red + (int)sizeof(float2) * p.rt * p.tx * (by_vector ? 1 : p.V);
+    s.mask = s.stat + (int)sizeof(float2) * p.groups;
+    s.bytes = s.mask + (masks ? p.rows * p.tx : 0);
+    return s;
+}
+template <typename X> __device__ __forceinline__ X* space_at(uint4* space, int at) { return reinterpret_cast<X*>(reinterpret_cast<char*>(space) + at); }
+
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads)
-norm_apply_kernel(const T* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta, int ptype,
-                  const double2* __restrict__ part, NormDims d, NormPlan p, double eps, int act, Drop drop,
-                  T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-    __shared__ float2 stat[kNormMaxGroups];
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
-    const int lane = threadIdx.x & 31;
-    for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        double a = 0.0, e = 0.0;
-        for (int k = lane; k < p.splits * p.pieces; k += 32) {
-            const int s = k / p.pieces, piece = k - s * p.pieces;
-            const double2 v = part[(((size_t)n * p.splits + s) * d.G + b.g0 + g) * p.pieces + piece];
-            a += v.x;
-            e += v.y;
+__global__ void __launch_bounds__(kNormThreads, 3)
+norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, NormPlan p, KeptSpace sp, double eps, int act, Drop drop,
+                 T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+    extern __shared__ uint4 space[];
+    T* data = reinterpret_cast<T*>(space);
+    float2* red = space_at<float2>(space, sp.red);
+    float2* stat = space_at<float2>(space, sp.stat);
+    const int n = p.by_blocks(blockIdx.x);
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const int rows = d.L, r1 = in ? rows : 0;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
+    T* own = data + cv * V;
+    const int pitch = p.tx * V;
+    for (int r = rt; r < r1; r += p.rt) keep_vector<T, V>(own + r * pitch, x + at + (size_t)r * d.C);
+    keep_wait();
+    if (in) {
+        Moments<V> t;
+        if (rt < r1) t.start(load_raw_as<T, V>(own + rt * pitch));
+#pragma unroll 4
+        for (int r = rt + p.rt; r < r1; r += p.rt) t.add(load_raw_as<T, V>(own + r * pitch));
+        t.put(red, p, rt, cv, rows_of(rows, rt, p));
+    }
+    join_moments<V>(red, d, p, b, rows, [&](int g, float mu, float m2) {
+        const float2 s = finish_stat(mu, (double)m2 * d.inv_m, eps);
+        stat[g] = s;
+        if (mean != nullptr) {
+            mean[(size_t)n * d.G + b.g0 + g] = s.x;
+            rstd[(size_t)n * d.G + b.g0 + g] = s.y;
         }
-        a = warp_sum(a) * d.inv_m;
-        e = warp_sum(e) * d.inv_m - a * a;
-        if (lane == 0) {
-            const float m = (float)a, r = (float)(1.0 / sqrt((e > 0.0 || e != e ? e : 0.0) + eps));
-            stat[g] = make_float2(m, r);
+    });
+    __syncthreads();
+    if (in) {
+        Column<V> col;
+        load_column<V>(col, stat, gamma, beta, d, p, b, cv);
+        const DropKey key = drop.on ? drop_key(drop) : DropKey{};
+#pragma unroll 2
+        for (int r = rt; r < r1; r += p.rt)
+            write_vector<T, V>(load_raw<T, V>(own + r * pitch), col, act, drop, key, at + (size_t)r * d.C, y);
+    }
+}
+
+// ---- forward, two passes ----------------------------------------------------------------------------------------------
+
+constexpr int kSumRows = 8;               // rows of a thread that are on their way at a time
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormThreads, 3)
+norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __restrict__ part) {
+    extern __shared__ float2 red2[];                            // [rt][tx] or [rt][tx * V]
+    const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
+    const int r0 = split * p.rows, rows = min(p.rows, d.L - r0);
+    if (rt < p.rt && cv < b.nvec) {
+        const T* at = x + ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+        Moments<V> t;
+        for (int r = rt; r < rows; r += kSumRows * p.rt) {
+            Raw<T, V> v[kSumRows];
+#pragma unroll
+            for (int k = 0; k < kSumRows; ++k)
+                if (r + k * p.rt < rows) v[k] = load_raw<T, V>(at + (size_t)(r + k * p.rt) * d.C);
+            if (r == rt) t.start(as_vec<T, V>(v[0]));
+#pragma unroll
+            for (int k = 0; k < kSumRows; ++k)
+                if (r + k * p.rt < rows) t.add(as_vec<T, V>(v[k]));
+        }
+        t.put(red2, p, rt, cv, rows_of(rows, rt, p));
+    }
+    const double count = (double)rows * (p.pieces == 1 ? d.Cg : b.nvec * V);
+    join_moments<V>(red2, d, p, b, rows, [&](int g, float mu, float m2) {
+        part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_double2(count * mu, m2 + count * mu * mu);
+    });
+}
+
+// The two sums of a group over its row ranges and pieces, in all lanes.
+__device__ __forceinline__ double2 add_parts(const double2* part, const NormDims& d, const NormPlan& p, int n, int g) {
+    double a = 0.0, e = 0.0;
+    for (int k = threadIdx.x & 31; k < p.splits * p.pieces; k += 32) {
+        const int s = k / p.pieces, piece = k - s * p.pieces;
+        const double2 v = part[(((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece];
+        a += v.x;
+        e += v.y;
+    }
+    return make_double2(warp_sum(a) * d.inv_m, warp_sum(e) * d.inv_m);
+}
+
+constexpr int kApplyRows = 4;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormThreads, 3)
+norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double2* __restrict__ part, NormDims d, NormPlan p, double eps, int act,
+                  Drop drop, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ float2 stat[kNormMaxGroups];
+    const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
+    for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
+        const double2 v = add_parts(part, d, p, n, b.g0 + g);
+        const double var = v.y - v.x * v.x;
+        if ((threadIdx.x & 31) == 0) {
+            const float2 f = finish_stat(v.x, var > 0.0 || var != var ? var : 0.0, eps);
+            stat[g] = f;
             if (split == 0 && b.piece == 0 && mean != nullptr) {
-                mean[(size_t)n * d.G + b.g0 + g] = m;
-                rstd[(size_t)n * d.G + b.g0 + g] = r;
+                mean[(size_t)n * d.G + b.g0 + g] = f.x;
+                rstd[(size_t)n * d.G + b.g0 + g] = f.y;
             }
         }
     }
     __syncthreads();
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     if (rt >= p.rt || cv >= b.nvec) return;
-    float m[V], r[V], w[V], o[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = cv * V + j, g = p.pieces == 1 ? c / d.Cg : 0;
-        m[j] = stat[g].x;
-        r[j] = stat[g].y;
-        w[j] = gamma != nullptr ? load_param(gamma, b.c0 + c, ptype) : 1.f;
-        o[j] = beta != nullptr ? load_param(beta, b.c0 + c, ptype) : 0.f;
-    }
-    DropKey key = {};
-    if (drop.rng != nullptr) key = drop_key(drop);
+    Column<V> col;
+    load_column<V>(col, stat, gamma, beta, d, p, b, cv);
+    const DropKey key = drop.on ? drop_key(drop) : DropKey{};
     const int r1 = min(d.L, (split + 1) * p.rows);
     const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-    for (int l = split * p.rows + rt; l < r1; l += p.rt) {
-        const size_t i = at + (size_t)l * d.C;
-        float f[V];
-        unpack<T, V>(load_raw<T, V>(x + i), f);
+    for (int r = split * p.rows + rt; r < r1; r += kApplyRows * p.rt) {
+        Raw<T, V> v[kApplyRows];
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = activate(fmaf((f[j] - m[j]) * r[j], w[j], o[j]), act);
-        if (drop.rng != nullptr) drop_apply<V>(drop, key, i, f);
-        store_once<T, V>(y + i, pack<T, V>(f));
+        for (int k = 0; k < kApplyRows; ++k)
+            if (r + k * p.rt < r1) v[k] = load_once<T, V>(x + at + (size_t)(r + k * p.rt) * d.C);
+#pragma unroll
+        for (int k = 0; k < kApplyRows; ++k)
+            if (r + k * p.rt < r1) write_vector<T, V>(v[k], col, act, drop, key, at + (size_t)(r + k * p.rt) * d.C, y);
     }
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
 
-// the gradient at u and the normalised value h of V elements
-template <typename T, int V>
-__device__ __forceinline__ void norm_du(const Raw<T, V>& xv, const Raw<T, V>& gv, const float (&m)[V], const float (&r)[V], const float (&w)[V],
-                                        const float (&o)[V], int act, const Drop& drop, const DropKey& key, size_t i, float (&du)[V], float (&h)[V]) {
-    unpack<T, V>(xv, h);
-    unpack<T, V>(gv, du);
-    if (drop.rng != nullptr) drop_apply<V>(drop, key, i, du);
+// What a thread's column needs for u, and for dx = a du + ra + (x - m) rb.
+template <int V> struct BackColumn { float m[V], a[V], o[V], r[V]; };
+template <int V>
+__device__ __forceinline__ void load_back_column(BackColumn<V>& k, const float* mean, const float* rstd, const Param& gamma, const Param& beta,
+                                                 const NormDims& d, const NormPlan& p, const NormBlock& b, int n, int cv) {
+    int g[V];
+    groups_of<V>(d, p, cv * V, g);
+    load_params<V>(gamma, b.c0 + cv * V, k.a);
+    load_params<V>(beta, b.c0 + cv * V, k.o);
+    mean += (size_t)n * d.G + b.g0;
+    rstd += (size_t)n * d.G + b.g0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        h[j] = (h[j] - m[j]) * r[j];
-        du[j] *= slope(fmaf(h[j], w[j], o[j]), act);
+        k.m[j] = __ldg(mean + g[j]);
+        k.r[j] = __ldg(rstd + g[j]);
+        k.a[j] *= k.r[j];
+    }
+}
+
+// du of V elements (the gradient at u) from that at y, which has been dropped already, and x - mean
+template <typename T, int V>
+__device__ __forceinline__ void back_du(const Raw<T, V>& xv, const BackColumn<V>& k, int act, float (&du)[V], float (&e)[V]) {
+    unpack<T, V>(xv, e);
+    sub_all<V>(e, e, k.m);
+    if (act == LINF_ACT_IDENTITY) return;
+    float s[V];
+    fma_all<V>(s, e, k.a, k.o);
+    slope_all<sizeof(T) == 4, V>(s, act);
+    mul_all<V>(du, du, s);
+}
+template <typename T, int V>
+__device__ __forceinline__ void back_du(const Raw<T, V>& xv, const Raw<T, V>& gv, const BackColumn<V>& k, int act, const Drop& drop, const DropKey& key,
+                                        size_t i, float (&du)[V], float (&e)[V]) {
+    unpack<T, V>(gv, du);
+    if (drop.on) drop_apply<V>(drop, key, i, du);
+    back_du<T, V>(xv, k, act, du, e);
+}
+
+// Sums of gamma du and gamma du h over each group of the block from its channels' sums (du, du h), which `sums` holds by channel.
+template <typename Done>
+__device__ __forceinline__ void group_sums(const float2* sums, const Param& gamma, const NormDims& d, const NormPlan& p, const NormBlock& b, Done done) {
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int per = p.pieces == 1 ? d.Cg : b.nvec * p.V;
+    int wide = 1;                                               // as many lanes to a group as it has channels, up to a warp
+    while (wide < per && wide < 32) wide *= 2;
+    for (int g0 = (threadIdx.x >> 5) * (32 / wide); g0 < b.ng; g0 += warps * (32 / wide)) {
+        const int g = g0 + lane / wide, first = g < b.ng ? lane & (wide - 1) : per;
+        double s = 0.0, t = 0.0;
+        for (int c = first; c < per; c += wide) {
+            const float w = load_param(gamma, b.c0 + g * per + c);
+            const float2 v = sums[g * per + c];
+            s += (double)w * v.x;
+            t += (double)w * v.y;
+        }
+        for (int o = 1; o < wide; o *= 2) {
+            s += __shfl_xor_sync(0xffffffffu, s, o);
+            t += __shfl_xor_sync(0xffffffffu, t, o);
+        }
+        if (g < b.ng && (lane & (wide - 1)) == 0) done(g, make_double2(s, t));
+    }
+}
+
+// Adds the threads' channel sums up along the rows; they end in red's first row.
+__device__ __forceinline__ void fold_rows(float2* red, int width, int rt) {
+    by_columns(width, rt, [&](int c, int first, int step, auto join) {
+        float s = 0.f, t = 0.f;
+        for (int r = first; r < rt; r += step) { const float2 v = red[r * width + c]; s += v.x; t += v.y; }
+        if (join(s, t)) red[c] = make_float2(s, t);
+    });
+}
+
+// dx of V elements from du and x - mean
+template <typename T, int V>
+__device__ __forceinline__ void write_dx(const float (&du)[V], const float (&e)[V], const BackColumn<V>& k, const float (&ra)[V], const float (&rb)[V],
+                                         T* to) {
+    float f[V];
+    fma_all<V>(f, k.a, du, ra);
+    fma_all<V>(f, e, rb, f);
+    store_once<T, V>(to, pack<T, V>(f));
+}
+template <int V>
+__device__ __forceinline__ void load_means(const float2* stat, const NormDims& d, const NormPlan& p, int cv, const BackColumn<V>& k, float (&ra)[V],
+                                           float (&rb)[V]) {
+    int g[V];
+    groups_of<V>(d, p, cv * V, g);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float2 s = stat[g[j]];
+        ra[j] = -k.r[j] * s.x;
+        rb[j] = -k.r[j] * k.r[j] * s.y;
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads)
-norm_back_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta, int ptype,
-                      const float* __restrict__ mean, const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop,
-                      float2* __restrict__ by_channel, float2* __restrict__ by_group) {
+__global__ void __launch_bounds__(kNormThreads, 2)
+norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param gamma, Param beta, const float* __restrict__ mean,
+                      const float* __restrict__ rstd, NormDims d, NormPlan p, KeptSpace sp, int act, Drop drop, T* __restrict__ dx,
+                      float2* __restrict__ by_channel) {
+    extern __shared__ uint4 space[];
+    T* data = reinterpret_cast<T*>(space);
+    float2* red = space_at<float2>(space, sp.red);
+    float2* stat = space_at<float2>(space, sp.stat);
+    unsigned char* kept = space_at<unsigned char>(space, sp.mask) ;
+    const int chunk = p.by_blocks(blockIdx.x);
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - chunk * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const int r1 = in ? d.L : 0, pitch = p.tx * V;
+    T* own = data + cv * V;                                     // x, and behind its rows dy
+    T* own_g = own + (size_t)p.rows * pitch;
+    const int n1 = min(d.N, (chunk + 1) * p.per_cta);
+    const DropKey key = drop.on ? drop_key(drop) : DropKey{};
+    float2 total[V];                                            // of all samples of this CTA
+#pragma unroll
+    for (int j = 0; j < V; ++j) total[j] = make_float2(0.f, 0.f);
+    for (int n = chunk * p.per_cta; n < n1; ++n) {
+        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
+        for (int r = rt; r < r1; r += p.rt) {
+            keep_vector<T, V>(own + r * pitch, x + at + (size_t)r * d.C);
+            keep_vector<T, V>(own_g + r * pitch, dy + at + (size_t)r * d.C);
+        }
+        BackColumn<V> col;
+        if (in) load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
+        float sa[V], sb[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.f;
+        keep_wait();
+#pragma unroll 2
+        for (int r = rt; r < r1; r += p.rt) {
+            float du[V], e[V];
+            unpack<T, V>(load_raw<T, V>(own_g + r * pitch), du);
+            if (drop.on) {
+                const unsigned mask = drop_mask<V>(drop, key, at + (size_t)r * d.C);
+                if (sizeof(T) == 2) kept[r * p.tx + cv] = (unsigned char)mask;
+                drop_masked<V>(drop, mask, du);
+            }
+            back_du<T, V>(load_raw<T, V>(own + r * pitch), col, act, du, e);
+            add_all<V>(sa, sa, du);
+            fma_all<V>(sb, du, e, sb);
+            // fp32: du takes the place of dy; 16-bit types would round it, and work it out again
+            if (sizeof(T) == 4) *reinterpret_cast<Raw<T, V>*>(own_g + r * pitch) = pack<T, V>(du);
+        }
+        if (in) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                sb[j] *= col.r[j];
+                total[j].x += sa[j];
+                total[j].y += sb[j];
+            }
+        }
+        if (dx == nullptr) continue;                            // the same for every thread
+        if (rt < p.rt) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) red[rt * pitch + cv * V + j] = make_float2(sa[j], sb[j]);
+        }
+        __syncthreads();
+        if (p.rt > 1) {
+            fold_rows(red, pitch, p.rt);
+            __syncthreads();
+        }
+        group_sums(red, gamma, d, p, b, [&](int g, double2 v) { stat[g] = make_float2((float)(v.x * d.inv_m), (float)(v.y * d.inv_m)); });
+        __syncthreads();
+        if (in) {
+            float ra[V], rb[V];
+            load_means<V>(stat, d, p, cv, col, ra, rb);
+#pragma unroll 2
+            for (int r = rt; r < r1; r += p.rt) {
+                const size_t i = at + (size_t)r * d.C;
+                float du[V], e[V];
+                if (sizeof(T) == 4) {
+                    unpack<T, V>(load_raw<T, V>(own + r * pitch), e);
+                    unpack<T, V>(load_raw<T, V>(own_g + r * pitch), du);
+#pragma unroll
+                    for (int j = 0; j < V; ++j) e[j] -= col.m[j];
+                } else {
+                    unpack<T, V>(load_raw<T, V>(own_g + r * pitch), du);
+                    if (drop.on) drop_masked<V>(drop, kept[r * p.tx + cv], du);
+                    back_du<T, V>(load_raw<T, V>(own + r * pitch), col, act, du, e);
+                }
+                write_dx<T, V>(du, e, col, ra, rb, dx + i);
+            }
+        }
+        __syncthreads();
+    }
+    if (rt < p.rt) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[rt * pitch + cv * V + j] = total[j];
+    }
+    __syncthreads();
+    fold_rows(red, pitch, p.rt);
+    __syncthreads();
+    for (int c = threadIdx.x; c < b.nvec * V; c += blockDim.x) by_channel[(size_t)chunk * d.C + b.c0 + c] = red[c];
+}
+
+constexpr int kBackRows = 2;
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kNormThreads, 2)
+norm_back_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param gamma, Param beta, const float* __restrict__ mean,
+                      const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop, float2* __restrict__ by_channel,
+                      double2* __restrict__ by_group) {
     extern __shared__ float2 redf[];                            // [rt][tx * V]
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
+    const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const int width = p.tx * V;
     if (rt < p.rt) {
         float sa[V], sb[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.f;
         if (cv < b.nvec) {
-            float m[V], r[V], w[V], o[V];
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int c = cv * V + j, g = b.g0 + (p.pieces == 1 ? c / d.Cg : 0);
-                m[j] = mean[(size_t)n * d.G + g];
-                r[j] = rstd[(size_t)n * d.G + g];
-                w[j] = gamma != nullptr ? load_param(gamma, b.c0 + c, ptype) : 1.f;
-                o[j] = beta != nullptr ? load_param(beta, b.c0 + c, ptype) : 0.f;
-            }
-            DropKey key = {};
-            if (drop.rng != nullptr) key = drop_key(drop);
+            BackColumn<V> col;
+            load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
+            const DropKey key = drop.on ? drop_key(drop) : DropKey{};
             const int r1 = min(d.L, (split + 1) * p.rows);
             const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-            for (int l = split * p.rows + rt; l < r1; l += p.rt) {
-                const size_t i = at + (size_t)l * d.C;
-                float du[V], h[V];
-                norm_du<T, V>(load_raw<T, V>(x + i), load_raw<T, V>(dy + i), m, r, w, o, act, drop, key, i, du, h);
+            for (int r = split * p.rows + rt; r < r1; r += kBackRows * p.rt) {
+                Raw<T, V> v[kBackRows], g[kBackRows];
 #pragma unroll
-                for (int j = 0; j < V; ++j) { sa[j] += du[j]; sb[j] = fmaf(du[j], h[j], sb[j]); }
+                for (int k = 0; k < kBackRows; ++k)
+                    if (r + k * p.rt < r1) {
+                        v[k] = load_raw<T, V>(x + at + (size_t)(r + k * p.rt) * d.C);
+                        g[k] = load_raw<T, V>(dy + at + (size_t)(r + k * p.rt) * d.C);
+                    }
+#pragma unroll
+                for (int k = 0; k < kBackRows; ++k)
+                    if (r + k * p.rt < r1) {
+                        float du[V], e[V];
+                        back_du<T, V>(v[k], g[k], col, act, drop, key, at + (size_t)(r + k * p.rt) * d.C, du, e);
+                        add_all<V>(sa, sa, du);
+                        fma_all<V>(sb, du, e, sb);
+                    }
             }
+#pragma unroll
+            for (int j = 0; j < V; ++j) sb[j] *= col.r[j];
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) redf[rt * width + cv * V + j] = make_float2(sa[j], sb[j]);
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < b.nvec * V; c += kNormThreads) {
-        float2 t = redf[c];
-        for (int k = 1; k < p.rt; ++k) { t.x += redf[k * width + c].x; t.y += redf[k * width + c].y; }
-        redf[c] = t;
-        by_channel[((size_t)n * p.splits + split) * d.C + b.c0 + c] = t;
-    }
+    fold_rows(redf, width, p.rt);
     __syncthreads();
-    const int lane = threadIdx.x & 31;
-    const int per = p.pieces == 1 ? d.Cg : b.nvec * V;
-    for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        double a = 0.0, e = 0.0;
-        for (int c = lane; c < per; c += 32) {
-            const float w = gamma != nullptr ? load_param(gamma, b.c0 + g * per + c, ptype) : 1.f;
-            a += w * redf[g * per + c].x;
-            e += w * redf[g * per + c].y;
-        }
-        a = warp_sum(a);
-        e = warp_sum(e);
-        if (lane == 0) by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_float2((float)a, (float)e);
-    }
+    for (int c = threadIdx.x; c < b.nvec * V; c += kNormThreads) by_channel[((size_t)n * p.splits + split) * d.C + b.c0 + c] = redf[c];
+    group_sums(redf, gamma, d, p, b,
+               [&](int g, double2 v) { by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = v; });
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads)
-norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, const void* __restrict__ gamma, const void* __restrict__ beta, int ptype,
-                       const float* __restrict__ mean, const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop,
-                       const float2* __restrict__ by_group, T* __restrict__ dx) {
+__global__ void __launch_bounds__(kNormThreads, 2)
+norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param gamma, Param beta, const float* __restrict__ mean,
+                       const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop, const double2* __restrict__ by_group,
+                       T* __restrict__ dx) {
     __shared__ float2 stat[kNormMaxGroups];
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
-    const int lane = threadIdx.x & 31;
+    const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        double a = 0.0, e = 0.0;
-        for (int k = lane; k < p.splits * p.pieces; k += 32) {
-            const int s = k / p.pieces, piece = k - s * p.pieces;
-            const float2 v = by_group[(((size_t)n * p.splits + s) * d.G + b.g0 + g) * p.pieces + piece];
-            a += v.x;
-            e += v.y;
-        }
-        a = warp_sum(a) * d.inv_m;
-        e = warp_sum(e) * d.inv_m;
-        if (lane == 0) stat[g] = make_float2((float)a, (float)e);
+        const double2 v = add_parts(by_group, d, p, n, b.g0 + g);
+        if ((threadIdx.x & 31) == 0) stat[g] = make_float2((float)v.x, (float)v.y);
     }
     __syncthreads();
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     if (rt >= p.rt || cv >= b.nvec) return;
-    float m[V], r[V], w[V], o[V], ma[V], mb[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = cv * V + j, g = p.pieces == 1 ? c / d.Cg : 0;
-        m[j] = mean[(size_t)n * d.G + b.g0 + g];
-        r[j] = rstd[(size_t)n * d.G + b.g0 + g];
-        ma[j] = stat[g].x;
-        mb[j] = stat[g].y;
-        w[j] = gamma != nullptr ? load_param(gamma, b.c0 + c, ptype) : 1.f;
-        o[j] = beta != nullptr ? load_param(beta, b.c0 + c, ptype) : 0.f;
-    }
-    DropKey key = {};
-    if (drop.rng != nullptr) key = drop_key(drop);
+    BackColumn<V> col;
+    load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
+    float ra[V], rb[V];
+    load_means<V>(stat, d, p, cv, col, ra, rb);
+    const DropKey key = drop.on ? drop_key(drop) : DropKey{};
     const int r1 = min(d.L, (split + 1) * p.rows);
     const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-    for (int l = split * p.rows + rt; l < r1; l += p.rt) {
-        const size_t i = at + (size_t)l * d.C;
-        float du[V], h[V];
-        norm_du<T, V>(load_raw<T, V>(x + i), load_raw<T, V>(dy + i), m, r, w, o, act, drop, key, i, du, h);
+    for (int r = split * p.rows + rt; r < r1; r += kBackRows * p.rt) {
+        Raw<T, V> v[kBackRows], g[kBackRows];
 #pragma unroll
-        for (int j = 0; j < V; ++j) du[j] = r[j] * (fmaf(w[j], du[j], -ma[j]) - h[j] * mb[j]);
-        store_once<T, V>(dx + i, pack<T, V>(du));
+        for (int k = 0; k < kBackRows; ++k)
+            if (r + k * p.rt < r1) {
+                v[k] = load_once<T, V>(x + at + (size_t)(r + k * p.rt) * d.C);
+                g[k] = load_once<T, V>(dy + at + (size_t)(r + k * p.rt) * d.C);
+            }
+#pragma unroll
+        for (int k = 0; k < kBackRows; ++k)
+            if (r + k * p.rt < r1) {
+                const size_t i = at + (size_t)(r + k * p.rt) * d.C;
+                float du[V], e[V];
+                back_du<T, V>(v[k], g[k], col, act, drop, key, i, du, e);
+                write_dx<T, V>(du, e, col, ra, rb, dx + i);
+            }
     }
 }
 
@@ -273,39 +601,74 @@ norm_params_kernel(const float2* __restrict__ by_channel, long long count, int C
     }
 }
 
+// ---- launches -----------------------------------------------------------------------------------------------------
+
+NormKind forward_kind(int type) { return {type == LINF_F32 ? 4 : 2, 1, false}; }
+NormKind backward_kind(int type) { return {type == LINF_F32 ? 4 : 2, 2, true}; }
+
+// The workspace of a call: forward, two passes: the parts; backward: the channels' sums, and the parts of two passes.
+size_t parts_bytes(const NormDims& d, const NormPlan& p) { return p.kept ? 0 : sizeof(double2) * (size_t)d.N * p.splits * d.G * p.pieces; }
+long long channel_rows(const NormPlan& p) { return (long long)p.chunks * p.splits; }
+size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
+    return parts_bytes(d, p) + (back ? sizeof(float2) * (size_t)channel_rows(p) * d.C : 0);
+}
+
 template <typename T, int V>
-int forward(const T* x, const void* gamma, const void* beta, int ptype, const NormDims& d, const NormPlan& p, double eps, int act,
-            const Drop& drop, T* y, float* mean, float* rstd, void* ws, cudaStream_t st) {
+int forward(const T* x, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, const Drop& drop, T* y, float* mean,
+            float* rstd, void* ws, cudaStream_t st) {
+    if (p.kept) {
+        const KeptSpace sp = kept_space(p, sizeof(T), 1, p.same, false);
+        return launch_kept(norm_kept_kernel<T, V>, p, sp.bytes, st, x, given.gamma, given.beta, d, p, sp, eps, act, drop, y, mean, rstd);
+    }
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     double2* part = static_cast<double2*>(ws);
-    norm_sums_kernel<T, V><<<grid, kNormThreads, sizeof(double2) * p.rt * p.tx * V, st>>>(x, d, p, part);
-    norm_apply_kernel<T, V><<<grid, kNormThreads, 0, st>>>(x, gamma, beta, ptype, part, d, p, eps, act, drop, y, mean, rstd);
+    norm_sums_kernel<T, V><<<grid, kNormThreads, sizeof(float2) * p.rt * p.tx * (p.same ? 1 : V), st>>>(x, d, p, part);
+    norm_apply_kernel<T, V><<<grid, kNormThreads, 0, st>>>(x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
     return launch_status(2);
 }
 
 template <typename T, int V>
-int backward(const T* dy, const T* x, const void* gamma, const void* beta, int ptype, const float* mean, const float* rstd, const NormDims& d,
-             const NormPlan& p, int act, const Drop& drop, T* dx, void* dgamma, void* dbeta, void* ws, cudaStream_t st) {
-    const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
-    float2* by_channel = static_cast<float2*>(ws);
-    float2* by_group = by_channel + (size_t)d.N * p.splits * d.C;
-    int launched = 1;
-    norm_back_sums_kernel<T, V><<<grid, kNormThreads, sizeof(float2) * p.rt * p.tx * V, st>>>(dy, x, gamma, beta, ptype, mean, rstd, d, p, act,
-                                                                                                 drop, by_channel, by_group);
-    if (dx != nullptr) {
-        norm_back_apply_kernel<T, V><<<grid, kNormThreads, 0, st>>>(dy, x, gamma, beta, ptype, mean, rstd, d, p, act, drop, by_group, dx);
-        ++launched;
+int backward(const T* dy, const T* x, const NormGiven& given, int ptype, const float* mean, const float* rstd, const NormDims& d, const NormPlan& p,
+             int act, const Drop& drop, T* dx, void* dgamma, void* dbeta, void* ws, cudaStream_t st) {
+    double2* by_group = static_cast<double2*>(ws);
+    float2* by_channel = reinterpret_cast<float2*>(static_cast<char*>(ws) + parts_bytes(d, p));
+    if (p.kept) {
+        const KeptSpace sp = kept_space(p, sizeof(T), 2, false, drop.on && sizeof(T) == 2);
+        const int rc = launch_kept(norm_back_kept_kernel<T, V>, p, sp.bytes, st, dy, x, given.gamma, given.beta, mean, rstd, d, p, sp, act, drop,
+                                   dx, by_channel);
+        if (rc) return rc;
+    } else {
+        const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
+        norm_back_sums_kernel<T, V><<<grid, kNormThreads, sizeof(float2) * p.rt * p.tx * V, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act,
+                                                                                                     drop, by_channel, by_group);
+        if (dx != nullptr)
+            norm_back_apply_kernel<T, V><<<grid, kNormThreads, 0, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_group, dx);
+        if (launch_status(dx != nullptr ? 2 : 1)) return LINF_ERR_LAUNCH;
     }
-    if (launch_status(launched)) return LINF_ERR_LAUNCH;
-    return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, (long long)d.N * p.splits, d.C, dgamma, dbeta, ptype, st) : LINF_OK;
-}
-
-size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
-    const size_t groups = (size_t)d.N * p.splits * d.G * p.pieces;
-    return back ? sizeof(float2) * ((size_t)d.N * p.splits * d.C + groups) : sizeof(double2) * groups;
+    return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, channel_rows(p), d.C, dgamma, dbeta, ptype, st) : LINF_OK;
 }
 
 }  // namespace
+
+bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g) {
+    static std::atomic<void*> known[kMaxDevices];
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess) { cudaGetLastError(); return false; }
+    void* at = dev < kMaxDevices ? known[dev].load(std::memory_order_relaxed) : nullptr;
+    if (at == nullptr) {
+        if (cudaGetSymbolAddress(&at, g_own) != cudaSuccess) { cudaGetLastError(); return false; }
+        if (dev < kMaxDevices) known[dev].store(at, std::memory_order_relaxed);
+    }
+    Own* own = static_cast<Own*>(at);
+    auto given = [&](const void* v, const float* instead) {
+        if (v == nullptr) return Param{instead, PARAM_ONE};
+        if (ptype == LINF_F32) return Param{v, aligned16(v) ? PARAM_WIDE : PARAM_F32};
+        return Param{v, ptype == LINF_F16 ? PARAM_F16 : PARAM_BF16};
+    };
+    g->gamma = given(gamma, &own->one);
+    g->beta = given(beta, &own->zero);
+    return true;
+}
 
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st) {
     norm_params_kernel<<<(C + 31) / 32, 1024, 0, st>>>(by_channel, count, C, dgamma, dbeta, ptype);
@@ -318,7 +681,7 @@ size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back) {
     for (int k = 0; k < 2; ++k) {
         NormDims d;
         NormPlan p;
-        if (norm_make(N, C, G, L, type == LINF_F32 ? 4 : 2, k == 0, &d, &p) != LINF_OK) return 0;
+        if (norm_make(N, C, G, L, back ? backward_kind(type) : forward_kind(type), k == 0, &d, &p) != LINF_OK) return 0;
         const size_t need = workspace(d, p, back);
         if (need > most) most = need;
     }
@@ -346,10 +709,13 @@ int group_norm_forward(const void* x, const void* gamma, const void* beta, int N
     NormPlan p;
     Drop drop;
     if (!make_drop(rate, rng, &drop)) return LINF_ERR_RATE;
-    const int rc = norm_make(N, C, G, L, type == LINF_F32 ? 4 : 2, aligned16(x) && aligned16(y), &d, &p);
+    const int rc = norm_make(N, C, G, L, forward_kind(type), aligned16(x) && aligned16(y), &d, &p);
     if (rc) return rc;
-    if (ws == nullptr || !aligned16(ws) || ws_bytes < workspace(d, p, false)) return LINF_ERR_WORKSPACE;
-#define LINF_CALL(T, V) forward<T, V>(static_cast<const T*>(x), gamma, beta, ptype, d, p, eps, act, drop, static_cast<T*>(y), mean, rstd, ws, st)
+    const size_t need = workspace(d, p, false);
+    if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need)) return LINF_ERR_WORKSPACE;
+    NormGiven given;
+    if (!norm_given(gamma, beta, ptype, &given)) return LINF_ERR_LAUNCH;
+#define LINF_CALL(T, V) forward<T, V>(static_cast<const T*>(x), given, d, p, eps, act, drop, static_cast<T*>(y), mean, rstd, ws, st)
     LINF_BY_VECTOR(LINF_CALL, LINF_CALL)
 #undef LINF_CALL
 }
@@ -361,11 +727,13 @@ int group_norm_backward(const void* dy, const void* x, const void* gamma, const 
     NormPlan p;
     Drop drop;
     if (!make_drop(rate, rng, &drop)) return LINF_ERR_RATE;
-    const int rc = norm_make(N, C, G, L, type == LINF_F32 ? 4 : 2, aligned16(x) && aligned16(dy) && aligned16(dx), &d, &p);
+    const int rc = norm_make(N, C, G, L, backward_kind(type), aligned16(x) && aligned16(dy) && aligned16(dx), &d, &p);
     if (rc) return rc;
     if (ws == nullptr || !aligned16(ws) || ws_bytes < workspace(d, p, true)) return LINF_ERR_WORKSPACE;
+    NormGiven given;
+    if (!norm_given(gamma, beta, ptype, &given)) return LINF_ERR_LAUNCH;
 #define LINF_CALL(T, V)                                                                                                                   \
-    backward<T, V>(static_cast<const T*>(dy), static_cast<const T*>(x), gamma, beta, ptype, mean, rstd, d, p, act, drop, static_cast<T*>(dx), \
+    backward<T, V>(static_cast<const T*>(dy), static_cast<const T*>(x), given, ptype, mean, rstd, d, p, act, drop, static_cast<T*>(dx), \
                    dgamma, dbeta, ws, st)
     LINF_BY_VECTOR(LINF_CALL, LINF_CALL)
 #undef LINF_CALL

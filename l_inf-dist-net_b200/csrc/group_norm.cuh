@@ -1,16 +1,17 @@
 // How the group-norm kernels deal a [N, L, C] activation (channels last) out to CTAs.
 //
-// A CTA takes a column block -- some whole groups, or a piece of one group -- and a range of rows (positions) of one sample.
-// Its threads form RT rows of TX vectors; a thread keeps its column, so that parameters and per-channel sums stay in registers.
+// A CTA works on a column block -- some whole groups, or a piece of one group -- of a range of rows (positions) of one sample.
+// Its threads form `rt` rows of `tx` vectors; a thread keeps its column, so that parameters and per-channel sums stay in registers.
 // Vectors are as wide as C, the groups and the pointers' alignment allow: a block of whole groups starts and ends on a vector.
+//
+// Where a CTA's shared memory holds a sample's column block, the CTA keeps it there ("kept"): every tensor is read once, reduced and
+// written.  What is larger takes two passes over memory: sums of row ranges, then, in a second launch whose CTAs add those up first and
+// which takes the ranges in the opposite order, the results: what was read last is still in L2.
 #pragma once
 
 #include "vec.cuh"
 
 namespace linf {
-
-constexpr int kNormThreads = 256;
-constexpr int kNormMaxGroups = 2048;      // groups of one column block: 256 vectors of at most 8 channels
 
 struct NormDims {
     int N, C, G, L;             // samples, channels, groups, positions
@@ -18,109 +19,250 @@ struct NormDims {
     double inv_m;               // 1 / (L * Cg)
 };
 
+// n / d of 0 <= n < 2^31 by a multiplication.
+struct Divider {
+    unsigned by, mul, shift;
+    __device__ __forceinline__ int operator()(int n) const { return (int)((__umulhi((unsigned)n, mul) + (unsigned)n) >> shift); }
+};
+inline Divider make_divider(int by) {
+    Divider d = {(unsigned)by, 0, 0};
+    while ((1ull << d.shift) < (unsigned long long)by) ++d.shift;
+    d.mul = (unsigned)(((1ull << 32) * ((1ull << d.shift) - (unsigned)by)) / (unsigned)by + 1);
+    return d;
+}
+
 struct NormPlan {
     int V;                      // channels of a vector
     int groups;                 // groups of a column block (1 where a group is cut into pieces)
     int pieces, piece;          // column blocks of one group, vectors of such a block (pieces = 1: whole groups)
     int blocks;                 // column blocks
     int tx, rt;                 // threads along the channels and along the rows
-    int splits, rows;           // row ranges of a sample, rows of a range
+    int same;                   // 1: all channels of a vector belong to one group
+    int threads;                // of a CTA
+    int kept;                   // 1: a CTA keeps a column block of a sample in shared memory, 0: two passes
+    int splits, rows;           // row ranges of a column block (kept: 1), rows of a range
+    int per_cta, chunks;        // samples that a CTA takes one after the other (kept), CTAs along the samples
+    Divider by_tx, by_blocks, by_cg;
 };
 
 // The column block of a CTA.
 struct NormBlock { int c0, nvec, g0, ng, piece; };
+template <int V>
 __device__ __forceinline__ NormBlock norm_block(const NormDims& d, const NormPlan& p, int bx) {
     NormBlock b;
     if (p.pieces == 1) {
         b.g0 = bx * p.groups;
         b.ng = min(p.groups, d.G - b.g0);
         b.c0 = b.g0 * d.Cg;
-        b.nvec = b.ng * d.Cg / p.V;
+        b.nvec = b.ng * d.Cg / V;
         b.piece = 0;
     } else {
         b.g0 = bx / p.pieces;
         b.ng = 1;
         b.piece = bx - b.g0 * p.pieces;
-        b.c0 = b.g0 * d.Cg + b.piece * p.piece * p.V;
-        b.nvec = min(p.piece, d.Cg / p.V - b.piece * p.piece);
+        b.c0 = b.g0 * d.Cg + b.piece * p.piece * V;
+        b.nvec = min(p.piece, d.Cg / V - b.piece * p.piece);
     }
     return b;
 }
 
-// The largest vector of {16 bytes, 4 bytes, one element} that the call allows; cap = vectors along the channels of a CTA.
-inline NormPlan norm_plan(const NormDims& d, int elem_bytes, bool aligned, int cap) {
-    NormPlan p = {};
+// The groups (within the block) of channels c .. c + V - 1 of a block of whole groups; all 0 in a piece of a group.
+template <int V>
+__device__ __forceinline__ void groups_of(const NormDims& d, const NormPlan& p, int c, int (&g)[V]) {
+    int at = 0, left = V;
+    if (p.pieces == 1) {
+        at = p.by_cg(c);
+        left = (at + 1) * d.Cg - c;                               // channels of this group from c on
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        if (p.pieces == 1 && j > 0 && left == 0) { ++at; left = d.Cg; }
+        --left;
+        g[j] = at;
+    }
+}
+
+// What a call reads: bytes of an element, tensors; whether it leaves per-channel sums behind (then a CTA takes several small samples).
+struct NormKind { int elem_bytes, tensors; bool sums; };
+
+constexpr int kNormThreads = 256;
+constexpr int kNormMaxGroups = kNormThreads * 8;
+constexpr int kNormKeepBytes = 64 * 1024; // of a CTA, so that an SM has three
+constexpr int kNormSplits = 64;           // row ranges of the two passes: a CTA of the second adds up that many
+constexpr int kNormWaves = 6;             // CTAs of the two passes for each SM
+
+inline int norm_ceil(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// widest vector of {16 bytes, 4 bytes, one element} that the call allows, and the least number of groups whose channels make whole
+// vectors; `cap`: vectors along the channels of a CTA.  One group may be wider than `cap`: *kmin = 0 then (it has to be cut).
+inline int norm_vector(const NormDims& d, int elem_bytes, bool aligned, int cap, int* kmin) {
     const int widths[3] = {16 / elem_bytes, 4 / elem_bytes, 1};
     for (int k = 0; k < 3; ++k) {
         const int V = widths[k];
-        if (k > 0 && V == widths[k - 1]) continue;
         if (V > 1 && (!aligned || d.C % V != 0)) continue;
         int a = d.Cg, b = V;
         while (b != 0) { const int r = a % b; a = b; b = r; }
-        const int kmin = V / a;                                   // groups whose channels make whole vectors
-        const long long need = (long long)kmin * d.Cg / V;
-        if (need > cap) {
-            if (kmin != 1) continue;                              // narrower vectors divide the group
-            p.V = V;
-            p.groups = 1;
-            const int vecs = d.Cg / V;
-            p.pieces = (vecs + cap - 1) / cap;
-            p.piece = (vecs + p.pieces - 1) / p.pieces;
-            p.pieces = (vecs + p.piece - 1) / p.piece;
-            p.blocks = d.G * p.pieces;
-            p.tx = p.piece;
-        } else {
-            p.V = V;
-            const int units = d.G / kmin;                         // kmin divides G, for V divides G * Cg
-            const int per = (int)(cap / need);
-            int blocks = (units + per - 1) / per;
-            const int each = (units + blocks - 1) / blocks;
-            blocks = (units + each - 1) / each;
-            p.groups = each * kmin;
-            p.pieces = 1;
-            p.piece = 0;
-            p.blocks = blocks;
-            p.tx = p.groups * d.Cg / V;
-        }
-        break;
+        *kmin = V / a;                                            // divides G, for V divides G * Cg
+        if ((long long)*kmin * d.Cg / V <= cap) return V;
+        if (*kmin == 1) { *kmin = 0; return V; }                  // else narrower vectors divide the group
     }
-    p.rt = cap / p.tx;
-    return p;
+    return 1;                                                     // not reached: V = 1 has kmin = 1
 }
 
-// Row ranges: enough CTAs for the GPU, at least four rows for each thread, at most `most` ranges (whoever adds them up reads that many).
-inline void norm_split_rows(const NormDims& d, NormPlan* p, int most) {
-    const long long ctas = (long long)p->blocks * d.N, want = (long long)sm_count() * 8;
-    long long s = ctas >= want ? 1 : (want + ctas - 1) / ctas;
-    const long long by_rows = (d.L + 4LL * p->rt - 1) / (4LL * p->rt);
+inline void norm_columns(const NormDims& d, NormPlan* p, int kmin, int units) {
+    const int all = d.G / kmin;
+    int blocks = norm_ceil(all, units);
+    const int each = norm_ceil(all, blocks);
+    p->blocks = norm_ceil(all, each);
+    p->groups = each * kmin;
+    p->pieces = 1;
+    p->piece = 0;
+    p->tx = (int)((long long)p->groups * d.Cg / p->V);
+}
+
+inline bool norm_keep(const NormDims& d, const NormKind& kind, bool aligned, NormPlan* p) {
+    int kmin;
+    p->V = norm_vector(d, kind.elem_bytes, aligned, kNormThreads, &kmin);
+    if (kmin == 0) return false;
+    const long long unit = (long long)kmin * d.Cg / p->V;                   // vectors of the narrowest column block
+    const long long row_bytes = unit * p->V * kind.elem_bytes;
+    auto bytes = [&](long long units) { return units * row_bytes * kind.tensors * d.L; };
+    if (bytes(1) > kNormKeepBytes) return false;
+    // Wider blocks while a row's piece is under 64 bytes (two sectors of L2), or while there are CTAs enough for the whole GPU several times
+    // over with few bytes each
+    int units = 1;
+    while (units * kmin < d.G && 2 * units * unit <= kNormThreads && bytes(2 * units) <= kNormKeepBytes) {
+        const long long ctas = (long long)d.N * norm_ceil(d.G / kmin, units);
+        const bool narrow = units * row_bytes < 64, many = ctas > 8LL * sm_count() && bytes(2 * units) <= 16 * 1024;
+        if (!narrow && !many) break;
+        units *= 2;
+    }
+    if (units * row_bytes < 32 && units * kmin < d.G && d.L > 1) return false;      // half a sector: two passes over whole rows are faster
+    norm_columns(d, p, kmin, units);
+    p->rows = d.L;
+    p->splits = 1;
+    // about four vectors to a thread where there are few, 256 threads otherwise
+    long long threads = (long long)p->tx * norm_ceil(p->rows, 4);
+    if (threads < 64) threads = 64;
+    if (threads > kNormThreads) threads = kNormThreads;
+    if (threads < p->tx) threads = p->tx;
+    p->rt = (int)(threads / p->tx);
+    if (p->rt > p->rows) p->rt = p->rows;
+    p->threads = norm_ceil((long long)p->tx * p->rt, 32) * 32;
+    p->kept = 1;
+    // with per-channel sums: as many CTAs as run at a time, twice over; a CTA adds its samples up in order
+    const long long resident = (long long)sm_count() * (2048 / p->threads < 16 ? 2048 / p->threads : 16) * 2;
+    p->per_cta = kind.sums ? norm_ceil((long long)d.N * p->blocks, resident) : 1;
+    p->chunks = norm_ceil(d.N, p->per_cta);
+    return true;
+}
+
+inline void norm_two_passes(const NormDims& d, const NormKind& kind, bool aligned, NormPlan* p) {
+    int kmin;
+    const int cap = kNormThreads;
+    p->V = norm_vector(d, kind.elem_bytes, aligned, cap, &kmin);
+    if (kmin == 0) {
+        p->groups = 1;
+        const int vecs = d.Cg / p->V;
+        p->pieces = norm_ceil(vecs, cap);
+        p->piece = norm_ceil(vecs, p->pieces);
+        p->pieces = norm_ceil(vecs, p->piece);
+        p->blocks = d.G * p->pieces;
+        p->tx = p->piece;
+    } else {
+        norm_columns(d, p, kmin, (int)(cap / ((long long)kmin * d.Cg / p->V)));
+    }
+    p->threads = kNormThreads;
+    p->rt = cap / p->tx;
+    if (p->rt > d.L) p->rt = d.L;
+    // CTAs for the whole GPU, with at least four rows for each thread
+    const long long ctas = (long long)p->blocks * d.N, want = (long long)sm_count() * kNormWaves;
+    long long s = ctas >= want ? 1 : norm_ceil(want, ctas);
+    const long long by_rows = norm_ceil(d.L, 4LL * p->rt);
     if (s > by_rows) s = by_rows;
-    if (s > most) s = most;
-    if (s < 1) s = 1;
-    p->rows = (int)((d.L + s - 1) / s);
-    p->splits = (d.L + p->rows - 1) / p->rows;
+    if (s > kNormSplits) s = kNormSplits;
+    p->rows = norm_ceil(d.L, s);
+    p->splits = norm_ceil(d.L, p->rows);
+    p->per_cta = 1;
+    p->chunks = d.N;
 }
 
 // A call's dimensions and plan: LINF_OK or the refusal.
-constexpr int kNormSplits = 64;           // row ranges of a sample at most
-
-inline int norm_make(int N, int C, int G, int L, int elem_bytes, bool aligned, NormDims* d, NormPlan* p) {
+inline int norm_make(int N, int C, int G, int L, const NormKind& kind, bool aligned, NormDims* d, NormPlan* p) {
     if (N <= 0 || C <= 0 || G <= 0 || L <= 0) return LINF_ERR_DIMS;
     if (C % G != 0) return LINF_ERR_GROUP;
+    if (L > (1 << 30)) return LINF_ERR_TOO_LARGE;
     d->N = N; d->C = C; d->G = G; d->L = L; d->Cg = C / G;
     d->inv_m = 1.0 / ((double)L * d->Cg);
-    *p = norm_plan(*d, elem_bytes, aligned, kNormThreads);
-    if (L > (1 << 30) || (long long)N * p->blocks > 0x7fffffffLL) return LINF_ERR_TOO_LARGE;
-    norm_split_rows(*d, p, kNormSplits);
+    *p = NormPlan{};
+    if (!norm_keep(*d, kind, aligned, p)) {
+        *p = NormPlan{};
+        norm_two_passes(*d, kind, aligned, p);
+    }
+    p->same = d->Cg % p->V == 0;
+    p->by_tx = make_divider(p->tx);
+    p->by_blocks = make_divider(p->blocks);
+    p->by_cg = make_divider(d->Cg);
+    if ((long long)N * p->blocks * p->splits > 0x7fffffffLL) return LINF_ERR_TOO_LARGE;
     return LINF_OK;
 }
 
 // dgamma and dbeta from `count` rows of per-channel sums (du, du h); either may be null (group_norm.cu)
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st);
 
+// gamma and beta, or what stands for them where they are null, on the current device; false if CUDA refused (group_norm.cu)
+struct NormGiven { Param gamma, beta; };
+bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g);
+
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// rows rt, rt + p.rt, ... of [0, rows): how many
+__device__ __forceinline__ int rows_of(int rows, int rt, const NormPlan& p) { return rt < rows ? (rows - rt - 1) / p.rt + 1 : 0; }
+
+// Columns c of [0, width), each with as many neighbouring lanes as the CTA has to spare, up to a warp: body(c, first row, step, join) adds the
+// rows first, first + step, ... up and calls join(s, t), which adds both over the lanes and is true in the one that keeps them.  c >= width
+// comes with no rows.
+template <typename Body>
+__device__ __forceinline__ void by_columns(int width, int rows, Body body) {
+    int lanes = 1;
+    while (lanes < 32 && 2 * lanes * width <= (int)blockDim.x && lanes < rows) lanes *= 2;
+    const int at_a_time = blockDim.x / lanes, mine = threadIdx.x / lanes, part = threadIdx.x - mine * lanes;
+    for (int c0 = 0; c0 < width; c0 += at_a_time) {
+        const int c = c0 + mine;
+        body(c, c < width ? part : rows, lanes, [&](float& s, float& t) {
+            for (int o = 1; o < lanes; o *= 2) {
+                s += __shfl_xor_sync(0xffffffffu, s, o);
+                t += __shfl_xor_sync(0xffffffffu, t, o);
+            }
+            return c < width && part == 0;
+        });
+    }
+}
+
+// One vector of a kept row from global to shared memory, asynchronously where its size allows.
+template <typename T, int V>
+__device__ __forceinline__ void keep_vector(T* to, const T* from) {
+    if (sizeof(T) * V == 16) cp_async16(to, from, 16);
+    else if (sizeof(T) * V == 4) cp_async4(to, from, 4);
+    else *to = *from;
+}
+__device__ __forceinline__ void keep_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <typename F>
+bool allow_shared(F kernel, size_t bytes) {
+    return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+}
+
+// A kept call.
+template <typename... A, typename... B>
+int launch_kept(void (*kernel)(A...), const NormPlan& p, size_t shared, cudaStream_t st, B... args) {
+    if (!allow_shared(kernel, shared)) return LINF_ERR_LAUNCH;
+    kernel<<<(unsigned)(p.chunks * p.blocks), p.threads, shared, st>>>(args...);
+    return launch_status();
 }
 
 }  // namespace linf

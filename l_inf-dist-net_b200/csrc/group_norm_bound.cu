@@ -91,56 +91,166 @@ __device__ __forceinline__ void bound_slope(double v0, double v1, int act, float
     d1 = (double)(g1 * slope((float)v1, act));
 }
 
-// adds up a CTA's per-thread values [rt][tx * V] of a group: lanes along the channels, rows in order
+// A thread's sums into red: one for each channel, or one for its vector where that lies in one group.
 template <int V>
-__device__ __forceinline__ Sum4 group_sum(const Sum4* red, const NormPlan& p, int per, int g) {
-    Sum4 t = {0.0, 0.0, 0.0, 0.0};
-    for (int c = threadIdx.x & 31; c < per; c += 32)
-        for (int r = 0; r < p.rt; ++r) t = add4(t, red[r * p.tx * V + g * per + c]);
-    return warp_sum4(t);
+__device__ __forceinline__ void put_sums(Sum4* red, const NormPlan& p, int rt, int cv, const Sum4 (&s)[V]) {
+    if (p.same) {
+        Sum4 t = s[0];
+#pragma unroll
+        for (int j = 1; j < V; ++j) t = add4(t, s[j]);
+        red[rt * p.tx + cv] = t;
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[(rt * p.tx + cv) * V + j] = s[j];
+    }
+}
+// Adds the threads' sums of each group of the block up, one warp to a group; done(g, sum) in its lane 0.
+template <typename Done>
+__device__ __forceinline__ void group_sums(const Sum4* red, const NormDims& d, const NormPlan& p, const NormBlock& b, Done done) {
+    const int per = (p.pieces == 1 ? d.Cg : b.nvec * p.V) / (p.same ? p.V : 1), width = p.same ? p.tx : p.tx * p.V;
+    for (int g = threadIdx.x >> 5; g < b.ng; g += blockDim.x >> 5) {
+        Sum4 t = {0.0, 0.0, 0.0, 0.0};
+        for (int i = threadIdx.x & 31; i < per * p.rt; i += 32) {
+            const int r = i / per;
+            t = add4(t, red[r * width + g * per + (i - r * per)]);
+        }
+        t = warp_sum4(t);
+        if ((threadIdx.x & 31) == 0) done(g, t);
+    }
+}
+// What the elements of a group share in the backward pass.
+struct Back {
+    double s0, s1;              // means of the gradients at n- and n+
+    double by_c, by_r;          // factor of c - mean(c), and of r
+};
+// from the group's sums of the gradients at n-, n+, s_lo, s_hi
+__device__ __forceinline__ Back make_back(const Box& x, const Sum4& t, const NormDims& d) {
+    Back k;
+    k.s0 = t.a * d.inv_m;
+    k.s1 = t.b * d.inv_m;
+    const double lo = t.c * x.s_lo * x.s_lo * x.s_lo * (x.sd + x.rho), hi = t.d * x.s_hi * x.s_hi * x.s_hi * fmax(x.sd - x.rho, 0.0);
+    // std and rho have no slope at 0, where all centres are one or all radii are 0: none is passed on
+    k.by_c = x.sd > 0.0 ? -(lo + hi) * d.inv_m / x.sd : 0.0;
+    k.by_r = x.rho > 0.0 ? (hi - lo) * d.inv_m / x.rho : 0.0;
+    return k;
+}
+
+__device__ __forceinline__ int group_of(const NormDims& d, const NormPlan& p, int c) { return p.pieces == 1 ? p.by_cg(c) : 0; }
+
+// Adds l, u, (l + u)^2, (u - l)^2 of a vector up.
+template <int V>
+__device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<float, V>& uv, Sum4 (&s)[V]) {
+    float l[V], u[V];
+    unpack<float, V>(lv, l);
+    unpack<float, V>(uv, u);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const double a = l[j], e = u[j];
+        s[j].a += a;
+        s[j].b += e;
+        s[j].c = fma(a + e, a + e, s[j].c);
+        s[j].d = fma(e - a, e - a, s[j].d);
+    }
+}
+
+template <int V>
+__device__ __forceinline__ void write_bounds(const Raw<float, V>& lv, const Raw<float, V>& uv, const Box* box, const float (&w)[V], const float (&o)[V],
+                                             const NormDims& d, const NormPlan& p, int c, size_t i, int act, float* out_l, float* out_u) {
+    float l[V], u[V];
+    unpack<float, V>(lv, l);
+    unpack<float, V>(uv, u);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const Ends e = make_ends(box[group_of(d, p, c + j)], l[j], u[j], d.inv_m);
+        const bool turned = w[j] < 0.f;
+        bound_act(fma(turned ? e.z1 : e.z0, (double)w[j], (double)o[j]), fma(turned ? e.z0 : e.z1, (double)w[j], (double)o[j]), act, l[j], u[j]);
+    }
+    store_once<float, V>(out_l + i, pack<float, V>(l));
+    store_once<float, V>(out_u + i, pack<float, V>(u));
+}
+
+// Shared memory: the rows of `tensors` tensors, the threads' sums, then what the groups share.
+struct BoundSpace { size_t red, box, back, bytes; };
+template <int V>
+__host__ __device__ inline BoundSpace bound_space(const NormPlan& p, int tensors) {
+    BoundSpace s;
+    const size_t four = sizeof(Sum4) * p.rt * p.tx * (p.same ? 1 : V), two = sizeof(float2) * p.rt * p.tx * V;
+    s.red = tensors > 0 ? ((size_t)p.rows * p.tx * V * sizeof(float) * tensors + 15) / 16 * 16 : 0;
+    s.box = s.red + ((four > two ? four : two) + 15) / 16 * 16;
+    s.back = s.box + sizeof(Box) * p.groups;
+    s.bytes = s.back + sizeof(Back) * p.groups;
+    return s;
+}
+
+template <int V>
+__global__ void __launch_bounds__(kNormThreads)
+bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upper, Param gamma, Param beta, NormDims d, NormPlan p, double eps, int act,
+                  float* __restrict__ out_l, float* __restrict__ out_u, Sum4* __restrict__ sums) {
+    extern __shared__ uint4 space[];
+    const BoundSpace at_ = bound_space<V>(p, 2);
+    float* data = reinterpret_cast<float*>(space);
+    Sum4* red = reinterpret_cast<Sum4*>(reinterpret_cast<char*>(space) + at_.red);
+    Box* box = reinterpret_cast<Box*>(reinterpret_cast<char*>(space) + at_.box);
+    const int n = p.by_blocks(blockIdx.x);
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const int r1 = in ? d.L : 0, pitch = p.tx * V;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
+    float* own_l = data + c;
+    float* own_u = own_l + (size_t)p.rows * pitch;
+    for (int r = rt; r < r1; r += p.rt) {
+        keep_vector<float, V>(own_l + r * pitch, lower + at + (size_t)r * d.C);
+        keep_vector<float, V>(own_u + r * pitch, upper + at + (size_t)r * d.C);
+    }
+    keep_wait();
+    if (in) {
+        Sum4 s[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
+#pragma unroll 2
+        for (int r = rt; r < r1; r += p.rt) sum_vector<V>(load_raw<float, V>(own_l + r * pitch), load_raw<float, V>(own_u + r * pitch), s);
+        put_sums<V>(red, p, rt, cv, s);
+    }
+    __syncthreads();
+    group_sums(red, d, p, b, [&](int g, const Sum4& s) {
+        box[g] = make_box(s, d, eps);
+        if (sums != nullptr) sums[(size_t)n * d.G + b.g0 + g] = s;
+    });
+    __syncthreads();
+    if (in) {
+        float w[V], o[V];
+        load_params<V>(gamma, b.c0 + c, w);
+        load_params<V>(beta, b.c0 + c, o);
+        for (int r = rt; r < r1; r += p.rt)
+            write_bounds<V>(load_raw<float, V>(own_l + r * pitch), load_raw<float, V>(own_u + r * pitch), box, w, o, d, p, c, at + (size_t)r * d.C, act,
+                            out_l, out_u);
+    }
 }
 
 template <int V>
 __global__ void __launch_bounds__(kNormThreads)
 bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upper, NormDims d, NormPlan p, Sum4* __restrict__ part) {
-    extern __shared__ Sum4 red[];
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
-    Sum4 s[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
+    extern __shared__ Sum4 red4[];
+    const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     if (rt < p.rt && cv < b.nvec) {
+        Sum4 s[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
         const int r1 = min(d.L, (split + 1) * p.rows);
         const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-#pragma unroll 2
-        for (int r = split * p.rows + rt; r < r1; r += p.rt) {
-            float l[V], u[V];
-            unpack<float, V>(load_raw<float, V>(lower + at + (size_t)r * d.C), l);
-            unpack<float, V>(load_raw<float, V>(upper + at + (size_t)r * d.C), u);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const double a = l[j], e = u[j];
-                s[j].a += a;
-                s[j].b += e;
-                s[j].c = fma(a + e, a + e, s[j].c);
-                s[j].d = fma(e - a, e - a, s[j].d);
-            }
-        }
-    }
-    if (rt < p.rt) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) red[rt * p.tx * V + cv * V + j] = s[j];
+#pragma unroll 4
+        for (int r = split * p.rows + rt; r < r1; r += p.rt)
+            sum_vector<V>(load_raw<float, V>(lower + at + (size_t)r * d.C), load_raw<float, V>(upper + at + (size_t)r * d.C), s);
+        put_sums<V>(red4, p, rt, cv, s);
     }
     __syncthreads();
-    const int per = p.pieces == 1 ? d.Cg : b.nvec * V;
-    for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        const Sum4 t = group_sum<V>(red, p, per, g);
-        if ((threadIdx.x & 31) == 0) part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = t;
-    }
+    group_sums(red4, d, p, b, [&](int g, const Sum4& s) { part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = s; });
 }
 
-// sums of a group over its row ranges and pieces
+// The sums of a group over its row ranges and pieces, in all lanes.
 __device__ __forceinline__ Sum4 all_parts(const Sum4* part, const NormDims& d, const NormPlan& p, int n, int g) {
     Sum4 t = {0.0, 0.0, 0.0, 0.0};
     for (int k = threadIdx.x & 31; k < p.splits * p.pieces; k += 32) {
@@ -152,48 +262,34 @@ __device__ __forceinline__ Sum4 all_parts(const Sum4* part, const NormDims& d, c
 
 template <int V>
 __global__ void __launch_bounds__(kNormThreads)
-bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ upper, const float* __restrict__ gamma, const float* __restrict__ beta,
-                   const Sum4* __restrict__ part, NormDims d, NormPlan p, double eps, int act, float* __restrict__ out_l, float* __restrict__ out_u,
-                   Sum4* __restrict__ sums) {
-    extern __shared__ Box box[];                                // [groups of the block]
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
+bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ upper, Param gamma, Param beta, const Sum4* __restrict__ part, NormDims d,
+                   NormPlan p, double eps, int act, float* __restrict__ out_l, float* __restrict__ out_u, Sum4* __restrict__ sums) {
+    extern __shared__ Box box1[];                               // [groups of the block]
+    const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(part, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
-            box[g] = make_box(t, d, eps);
+            box1[g] = make_box(t, d, eps);
             if (split == 0 && b.piece == 0 && sums != nullptr) sums[(size_t)n * d.G + b.g0 + g] = t;
         }
     }
     __syncthreads();
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
     if (rt >= p.rt || cv >= b.nvec) return;
     float w[V], o[V];
-    const Box* bx[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = cv * V + j;
-        bx[j] = box + (p.pieces == 1 ? c / d.Cg : 0);
-        w[j] = gamma != nullptr ? __ldg(gamma + b.c0 + c) : 1.f;
-        o[j] = beta != nullptr ? __ldg(beta + b.c0 + c) : 0.f;
-    }
+    load_params<V>(gamma, b.c0 + c, w);
+    load_params<V>(beta, b.c0 + c, o);
     const int r1 = min(d.L, (split + 1) * p.rows);
-    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
+#pragma unroll 2
     for (int r = split * p.rows + rt; r < r1; r += p.rt) {
         const size_t i = at + (size_t)r * d.C;
-        float l[V], u[V];
-        unpack<float, V>(load_raw<float, V>(lower + i), l);
-        unpack<float, V>(load_raw<float, V>(upper + i), u);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const Ends e = make_ends(*bx[j], l[j], u[j], d.inv_m);
-            const double z0 = w[j] < 0.f ? e.z1 : e.z0, z1 = w[j] < 0.f ? e.z0 : e.z1;
-            bound_act(fma(z0, (double)w[j], (double)o[j]), fma(z1, (double)w[j], (double)o[j]), act, l[j], u[j]);
-        }
-        store_once<float, V>(out_l + i, pack<float, V>(l));
-        store_once<float, V>(out_u + i, pack<float, V>(u));
+        write_bounds<V>(load_raw<float, V>(lower + i), load_raw<float, V>(upper + i), box1, w, o, d, p, c, i, act, out_l, out_u);
     }
 }
+
+// ---- backward -----------------------------------------------------------------------------------------------------
 
 // gradients at z- and z+ of one element, and what they add to those of gamma and beta
 __device__ __forceinline__ void bound_dz(const Ends& e, float w, float o, int act, float g0, float g1, double& q0, double& q1, double& dw, double& db) {
@@ -207,186 +303,257 @@ __device__ __forceinline__ void bound_dz(const Ends& e, float w, float o, int ac
     q1 = e.cut1 ? 0.0 : (turned ? d0 : d1) * (double)w;
 }
 
+
+struct In4 { const float *g_l, *g_u, *lower, *upper; };
+
+// What one vector adds to its group's sums (gradients at n-, n+, s_lo, s_hi) and to its channels' (beta, gamma).
 template <int V>
-__global__ void __launch_bounds__(kNormThreads)
-bound_back_sums_kernel(const float* __restrict__ g_l, const float* __restrict__ g_u, const float* __restrict__ lower, const float* __restrict__ upper,
-                       const float* __restrict__ gamma, const float* __restrict__ beta, const Sum4* __restrict__ sums, NormDims d, NormPlan p,
-                       double eps, int act, float2* __restrict__ by_channel, Sum4* __restrict__ by_group) {
-    extern __shared__ Sum4 red[];                               // [rt][tx * V], then the boxes
-    Box* box = reinterpret_cast<Box*>(red + p.rt * p.tx * V);
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
-    for (int g = threadIdx.x; g < b.ng; g += kNormThreads) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
-    __syncthreads();
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
-    const int width = p.tx * V;
-    double sw[V], sb[V];
-    Sum4 s[V];
+__device__ __forceinline__ void sum_back(const Raw<float, V>& lv, const Raw<float, V>& uv, const Raw<float, V>& glv, const Raw<float, V>& guv,
+                                         const Box* box, const float (&w)[V], const float (&o)[V], const NormDims& d, const NormPlan& p, int c, int act,
+                                         Sum4 (&s)[V], float2 (&by)[V]) {
+    float l[V], u[V], gl[V], gu[V];
+    unpack<float, V>(lv, l);
+    unpack<float, V>(uv, u);
+    unpack<float, V>(glv, gl);
+    unpack<float, V>(guv, gu);
 #pragma unroll
-    for (int j = 0; j < V; ++j) { s[j] = Sum4{0.0, 0.0, 0.0, 0.0}; sw[j] = sb[j] = 0.0; }
-    if (rt < p.rt && cv < b.nvec) {
-        float w[V], o[V];
-        const Box* bx[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int c = cv * V + j;
-            bx[j] = box + (p.pieces == 1 ? c / d.Cg : 0);
-            w[j] = gamma != nullptr ? __ldg(gamma + b.c0 + c) : 1.f;
-            o[j] = beta != nullptr ? __ldg(beta + b.c0 + c) : 0.f;
-        }
-        const int r1 = min(d.L, (split + 1) * p.rows);
-        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-        for (int r = split * p.rows + rt; r < r1; r += p.rt) {
-            const size_t i = at + (size_t)r * d.C;
-            float l[V], u[V], gl[V], gu[V];
-            unpack<float, V>(load_raw<float, V>(lower + i), l);
-            unpack<float, V>(load_raw<float, V>(upper + i), u);
-            unpack<float, V>(load_raw<float, V>(g_l + i), gl);
-            unpack<float, V>(load_raw<float, V>(g_u + i), gu);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const Ends e = make_ends(*bx[j], l[j], u[j], d.inv_m);
-                double q0, q1, dw, db;
-                bound_dz(e, w[j], o[j], act, gl[j], gu[j], q0, q1, dw, db);
-                sw[j] += dw;
-                sb[j] += db;
-                s[j].a = fma(q0, e.s0, s[j].a);                 // the gradients at n- and n+
-                s[j].b = fma(q1, e.s1, s[j].b);
-                const double t0 = q0 * e.n0, t1 = q1 * e.n1;    // at s_lo and s_hi
-                s[j].c += (e.n0 >= 0.0 ? t0 : 0.0) + (e.n1 >= 0.0 ? 0.0 : t1);
-                s[j].d += (e.n0 >= 0.0 ? 0.0 : t0) + (e.n1 >= 0.0 ? t1 : 0.0);
-            }
-        }
-    }
-    // the channels' sums first, in the same memory
-    double2* red2 = reinterpret_cast<double2*>(red);
-    if (rt < p.rt) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) red2[rt * width + cv * V + j] = make_double2(sb[j], sw[j]);
-    }
-    __syncthreads();
-    for (int c = threadIdx.x; c < b.nvec * V; c += kNormThreads) {
-        double2 t = red2[c];
-        for (int k = 1; k < p.rt; ++k) { t.x += red2[k * width + c].x; t.y += red2[k * width + c].y; }
-        by_channel[((size_t)n * p.splits + split) * d.C + b.c0 + c] = make_float2((float)t.x, (float)t.y);
-    }
-    __syncthreads();
-    if (rt < p.rt) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) red[rt * width + cv * V + j] = s[j];
-    }
-    __syncthreads();
-    const int per = p.pieces == 1 ? d.Cg : b.nvec * V;
-    for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        const Sum4 t = group_sum<V>(red, p, per, g);
-        if ((threadIdx.x & 31) == 0) by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = t;
+    for (int j = 0; j < V; ++j) {
+        const Ends e = make_ends(box[group_of(d, p, c + j)], l[j], u[j], d.inv_m);
+        double q0, q1, dw, db;
+        bound_dz(e, w[j], o[j], act, gl[j], gu[j], q0, q1, dw, db);
+        by[j].x += (float)db;
+        by[j].y += (float)dw;
+        s[j].a = fma(q0, e.s0, s[j].a);
+        s[j].b = fma(q1, e.s1, s[j].b);
+        const double t0 = q0 * e.n0, t1 = q1 * e.n1;
+        s[j].c += (e.n0 >= 0.0 ? t0 : 0.0) + (e.n1 >= 0.0 ? 0.0 : t1);
+        s[j].d += (e.n0 >= 0.0 ? 0.0 : t0) + (e.n1 >= 0.0 ? t1 : 0.0);
     }
 }
 
-// What the elements of a group share in the backward pass.
-struct Back {
-    Box box;
-    double s0, s1;              // means of the gradients at n- and n+
-    double by_c, by_r;          // factor of c - mean(c), and of r
-};
+template <int V>
+__device__ __forceinline__ void write_back(const Raw<float, V>& lv, const Raw<float, V>& uv, const Raw<float, V>& glv, const Raw<float, V>& guv,
+                                           const Box* box, const Back* back, const float (&w)[V], const float (&o)[V], const NormDims& d,
+                                           const NormPlan& p, int c, size_t i, int act, float* d_l, float* d_u) {
+    float l[V], u[V], gl[V], gu[V];
+    unpack<float, V>(lv, l);
+    unpack<float, V>(uv, u);
+    unpack<float, V>(glv, gl);
+    unpack<float, V>(guv, gu);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int g = group_of(d, p, c + j);
+        const Box& x = box[g];
+        const Back& m = back[g];
+        const double a = l[j], e = u[j];
+        const Ends s = make_ends(x, a, e, d.inv_m);
+        double q0, q1, dw, db;
+        bound_dz(s, w[j], o[j], act, gl[j], gu[j], q0, q1, dw, db);
+        q0 *= s.s0;
+        q1 *= s.s1;
+        const double dc = m.by_c * ((a + e) - (x.mean_l + x.mean_u)) * 0.5, dr = m.by_r * (e - a) * 0.5;
+        gl[j] = (float)(q0 + (q1 - q0) * d.inv_m - m.s1 + (dc - dr) * 0.5);
+        gu[j] = (float)(q1 + (q0 - q1) * d.inv_m - m.s0 + (dc + dr) * 0.5);
+    }
+    store_once<float, V>(d_l + i, pack<float, V>(gl));
+    store_once<float, V>(d_u + i, pack<float, V>(gu));
+}
+
+// Per-channel sums of a CTA's threads, added up along the rows and written to `to`; red is free before and after.
+template <int V>
+__device__ __forceinline__ void put_channels(float2* red, const NormPlan& p, const NormBlock& b, int rt, int cv, const float2 (&by)[V], float2* to) {
+    const int width = p.tx * V;
+    __syncthreads();
+    if (rt < p.rt) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) red[rt * width + cv * V + j] = by[j];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < b.nvec * V; c += blockDim.x) {
+        double s = 0.0, t = 0.0;
+        for (int r = 0; r < p.rt; ++r) { s += red[r * width + c].x; t += red[r * width + c].y; }
+        __stcg(to + c, make_float2((float)s, (float)t));
+    }
+    __syncthreads();
+}
 
 template <int V>
 __global__ void __launch_bounds__(kNormThreads)
-bound_back_apply_kernel(const float* __restrict__ g_l, const float* __restrict__ g_u, const float* __restrict__ lower, const float* __restrict__ upper,
-                        const float* __restrict__ gamma, const float* __restrict__ beta, const Sum4* __restrict__ sums,
-                        const Sum4* __restrict__ by_group, NormDims d, NormPlan p, double eps, int act, float* __restrict__ d_l, float* __restrict__ d_u) {
-    extern __shared__ Back back[];
-    const int n = blockIdx.x / p.blocks, split = blockIdx.y;
-    const NormBlock b = norm_block(d, p, blockIdx.x - n * p.blocks);
+bound_back_kept_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict__ sums, NormDims d, NormPlan p, double eps, int act,
+                       float* __restrict__ d_l, float* __restrict__ d_u, float2* __restrict__ by_channel) {
+    extern __shared__ uint4 space[];
+    const BoundSpace at_ = bound_space<V>(p, 4);
+    float* data = reinterpret_cast<float*>(space);
+    Sum4* red = reinterpret_cast<Sum4*>(reinterpret_cast<char*>(space) + at_.red);
+    Box* box = reinterpret_cast<Box*>(reinterpret_cast<char*>(space) + at_.box);
+    Back* back = reinterpret_cast<Back*>(reinterpret_cast<char*>(space) + at_.back);
+    const int chunk = p.by_blocks(blockIdx.x);
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - chunk * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const int r1 = in ? d.L : 0, pitch = p.tx * V;
+    const int n1 = min(d.N, (chunk + 1) * p.per_cta);
+    const size_t tensor = (size_t)p.rows * pitch;
+    float* own = data + c;                                      // lower, upper and their gradients, one behind the other
+    float w[V], o[V];
+    float2 by[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        w[j] = in ? load_param(gamma, b.c0 + c + j) : 1.f;
+        o[j] = in ? load_param(beta, b.c0 + c + j) : 0.f;
+        by[j] = make_float2(0.f, 0.f);
+    }
+    for (int n = chunk * p.per_cta; n < n1; ++n) {
+        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
+        for (int r = rt; r < r1; r += p.rt) {
+            const size_t i = at + (size_t)r * d.C;
+            keep_vector<float, V>(own + r * pitch, in4.lower + i);
+            keep_vector<float, V>(own + tensor + r * pitch, in4.upper + i);
+            keep_vector<float, V>(own + 2 * tensor + r * pitch, in4.g_l + i);
+            keep_vector<float, V>(own + 3 * tensor + r * pitch, in4.g_u + i);
+        }
+        for (int g = threadIdx.x; g < b.ng; g += blockDim.x) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
+        keep_wait();
+        __syncthreads();
+        if (in) {
+            Sum4 s[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
+            for (int r = rt; r < r1; r += p.rt) {
+                const float* at_r = own + r * pitch;
+                sum_back<V>(load_raw<float, V>(at_r), load_raw<float, V>(at_r + tensor), load_raw<float, V>(at_r + 2 * tensor),
+                            load_raw<float, V>(at_r + 3 * tensor), box, w, o, d, p, c, act, s, by);
+            }
+            put_sums<V>(red, p, rt, cv, s);
+        }
+        __syncthreads();
+        if (d_l == nullptr) continue;                           // the same for every thread
+        group_sums(red, d, p, b, [&](int g, const Sum4& s) { back[g] = make_back(box[g], s, d); });
+        __syncthreads();
+        if (in)
+            for (int r = rt; r < r1; r += p.rt) {
+                const float* at_r = own + r * pitch;
+                write_back<V>(load_raw<float, V>(at_r), load_raw<float, V>(at_r + tensor), load_raw<float, V>(at_r + 2 * tensor),
+                              load_raw<float, V>(at_r + 3 * tensor), box, back, w, o, d, p, c, at + (size_t)r * d.C, act, d_l, d_u);
+            }
+        __syncthreads();
+    }
+    put_channels<V>(reinterpret_cast<float2*>(red), p, b, rt, cv, by, by_channel + (size_t)chunk * d.C + b.c0);
+}
+
+template <int V>
+__global__ void __launch_bounds__(kNormThreads)
+bound_back_sums_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict__ sums, NormDims d, NormPlan p, double eps, int act,
+                       float2* __restrict__ by_channel, Sum4* __restrict__ by_group) {
+    extern __shared__ uint4 space[];
+    const BoundSpace at_ = bound_space<V>(p, 0);
+    Sum4* red = reinterpret_cast<Sum4*>(space);
+    Box* box = reinterpret_cast<Box*>(reinterpret_cast<char*>(space) + at_.box);
+    const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
+    for (int g = threadIdx.x; g < b.ng; g += kNormThreads) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
+    __syncthreads();
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
+    const bool in = rt < p.rt && cv < b.nvec;
+    Sum4 s[V];
+    float2 by[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) { s[j] = Sum4{0.0, 0.0, 0.0, 0.0}; by[j] = make_float2(0.f, 0.f); }
+    if (in) {
+        float w[V], o[V];
+        load_params<V>(gamma, b.c0 + c, w);
+        load_params<V>(beta, b.c0 + c, o);
+        const int r1 = min(d.L, (split + 1) * p.rows);
+        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
+        for (int r = split * p.rows + rt; r < r1; r += p.rt) {
+            const size_t i = at + (size_t)r * d.C;
+            sum_back<V>(load_raw<float, V>(in4.lower + i), load_raw<float, V>(in4.upper + i), load_raw<float, V>(in4.g_l + i),
+                        load_raw<float, V>(in4.g_u + i), box, w, o, d, p, c, act, s, by);
+        }
+    }
+    put_channels<V>(reinterpret_cast<float2*>(red), p, b, rt, cv, by, by_channel + ((size_t)n * p.splits + split) * d.C + b.c0);
+    if (in) put_sums<V>(red, p, rt, cv, s);
+    __syncthreads();
+    group_sums(red, d, p, b, [&](int g, const Sum4& q) { by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = q; });
+}
+
+template <int V>
+__global__ void __launch_bounds__(kNormThreads)
+bound_back_apply_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict__ sums, const Sum4* __restrict__ by_group, NormDims d, NormPlan p,
+                        double eps, int act, float* __restrict__ d_l, float* __restrict__ d_u) {
+    extern __shared__ uint4 space[];
+    const BoundSpace at_ = bound_space<V>(p, 0);
+    Box* box = reinterpret_cast<Box*>(reinterpret_cast<char*>(space) + at_.box);
+    Back* back = reinterpret_cast<Back*>(reinterpret_cast<char*>(space) + at_.back);
+    const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
+    const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(by_group, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
-            Back k;
-            k.box = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
-            const Box& x = k.box;
-            k.s0 = t.a * d.inv_m;
-            k.s1 = t.b * d.inv_m;
-            const double lo = t.c * x.s_lo * x.s_lo * x.s_lo * (x.sd + x.rho), hi = t.d * x.s_hi * x.s_hi * x.s_hi * fmax(x.sd - x.rho, 0.0);
-            // std and rho have no slope at 0, where all centres are one or all radii are 0: none is passed on
-            k.by_c = x.sd > 0.0 ? -(lo + hi) * d.inv_m / x.sd : 0.0;
-            k.by_r = x.rho > 0.0 ? (hi - lo) * d.inv_m / x.rho : 0.0;
-            back[g] = k;
+            const Box x = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
+            box[g] = x;
+            back[g] = make_back(x, t, d);
         }
     }
     __syncthreads();
-    const int rt = threadIdx.x / p.tx, cv = threadIdx.x - rt * p.tx;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
     if (rt >= p.rt || cv >= b.nvec) return;
     float w[V], o[V];
-    const Back* bk[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-        const int c = cv * V + j;
-        bk[j] = back + (p.pieces == 1 ? c / d.Cg : 0);
-        w[j] = gamma != nullptr ? __ldg(gamma + b.c0 + c) : 1.f;
-        o[j] = beta != nullptr ? __ldg(beta + b.c0 + c) : 0.f;
-    }
+    load_params<V>(gamma, b.c0 + c, w);
+    load_params<V>(beta, b.c0 + c, o);
     const int r1 = min(d.L, (split + 1) * p.rows);
-    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
     for (int r = split * p.rows + rt; r < r1; r += p.rt) {
         const size_t i = at + (size_t)r * d.C;
-        float l[V], u[V], gl[V], gu[V];
-        unpack<float, V>(load_raw<float, V>(lower + i), l);
-        unpack<float, V>(load_raw<float, V>(upper + i), u);
-        unpack<float, V>(load_raw<float, V>(g_l + i), gl);
-        unpack<float, V>(load_raw<float, V>(g_u + i), gu);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const Back& k = *bk[j];
-            const double a = l[j], e = u[j];
-            const Ends s = make_ends(k.box, a, e, d.inv_m);
-            double q0, q1, dw, db;
-            bound_dz(s, w[j], o[j], act, gl[j], gu[j], q0, q1, dw, db);
-            q0 *= s.s0;
-            q1 *= s.s1;
-            const double dc = k.by_c * ((a + e) * 0.5 - (k.box.mean_l + k.box.mean_u) * 0.5), dr = k.by_r * (e - a) * 0.5;
-            gl[j] = (float)(q0 - q0 * d.inv_m + q1 * d.inv_m - k.s1 + (dc - dr) * 0.5);
-            gu[j] = (float)(q1 - q1 * d.inv_m + q0 * d.inv_m - k.s0 + (dc + dr) * 0.5);
-        }
-        store_once<float, V>(d_l + i, pack<float, V>(gl));
-        store_once<float, V>(d_u + i, pack<float, V>(gu));
+        write_back<V>(load_raw<float, V>(in4.lower + i), load_raw<float, V>(in4.upper + i), load_raw<float, V>(in4.g_l + i),
+                      load_raw<float, V>(in4.g_u + i), box, back, w, o, d, p, c, i, act, d_l, d_u);
     }
 }
 
+// ---- launches -----------------------------------------------------------------------------------------------------
+
+NormKind bound_kind(bool back) { return {4, back ? 4 : 2, back}; }
+
+size_t parts_bytes(const NormDims& d, const NormPlan& p) { return p.kept ? 0 : sizeof(Sum4) * (size_t)d.N * p.splits * d.G * p.pieces; }
+long long channel_rows(const NormPlan& p) { return (long long)p.chunks * p.splits; }
+size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
+    return parts_bytes(d, p) + (back ? sizeof(float2) * (size_t)channel_rows(p) * d.C : 0);
+}
+
 template <int V>
-int forward(const float* lower, const float* upper, const float* gamma, const float* beta, const NormDims& d, const NormPlan& p, double eps, int act,
-            float* out_l, float* out_u, Sum4* sums, void* ws, cudaStream_t st) {
+int forward(const float* lower, const float* upper, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, float* out_l,
+            float* out_u, Sum4* sums, void* ws, cudaStream_t st) {
+    if (p.kept)
+        return launch_kept(bound_kept_kernel<V>, p, bound_space<V>(p, 2).bytes, st, lower, upper, given.gamma, given.beta, d, p, eps, act, out_l,
+                           out_u, sums);
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     Sum4* part = static_cast<Sum4*>(ws);
-    bound_sums_kernel<V><<<grid, kNormThreads, sizeof(Sum4) * p.rt * p.tx * V, st>>>(lower, upper, d, p, part);
-    const size_t boxes = sizeof(Box) * p.groups;
-    if (boxes > 48 * 1024 && cudaFuncSetAttribute(bound_apply_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)boxes) != cudaSuccess)
-        return LINF_ERR_LAUNCH;
-    bound_apply_kernel<V><<<grid, kNormThreads, boxes, st>>>(lower, upper, gamma, beta, part, d, p, eps, act, out_l, out_u, sums);
+    const size_t one = bound_space<V>(p, 0).box, two = sizeof(Box) * p.groups;
+    if (!allow_shared(bound_sums_kernel<V>, one) || !allow_shared(bound_apply_kernel<V>, two)) return LINF_ERR_LAUNCH;
+    bound_sums_kernel<V><<<grid, kNormThreads, one, st>>>(lower, upper, d, p, part);
+    bound_apply_kernel<V><<<grid, kNormThreads, two, st>>>(lower, upper, given.gamma, given.beta, part, d, p, eps, act, out_l, out_u, sums);
     return launch_status(2);
 }
 
 template <int V>
-int backward(const float* g_l, const float* g_u, const float* lower, const float* upper, const float* gamma, const float* beta, const Sum4* sums,
-             const NormDims& d, const NormPlan& p, double eps, int act, float* d_l, float* d_u, float* dgamma, float* dbeta, void* ws, cudaStream_t st) {
-    const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
+int backward(const In4& in4, const NormGiven& given, const Sum4* sums, const NormDims& d, const NormPlan& p, double eps, int act, float* d_l,
+             float* d_u, float* dgamma, float* dbeta, void* ws, cudaStream_t st) {
     Sum4* by_group = static_cast<Sum4*>(ws);
-    float2* by_channel = reinterpret_cast<float2*>(by_group + (size_t)d.N * p.splits * d.G * p.pieces);
-    const size_t one = sizeof(Sum4) * p.rt * p.tx * V + sizeof(Box) * p.groups, two = sizeof(Back) * p.groups;
-    if ((one > 48 * 1024 && cudaFuncSetAttribute(bound_back_sums_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)one) != cudaSuccess) ||
-        (two > 48 * 1024 && cudaFuncSetAttribute(bound_back_apply_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)two) != cudaSuccess))
-        return LINF_ERR_LAUNCH;
-    int launched = 1;
-    bound_back_sums_kernel<V><<<grid, kNormThreads, one, st>>>(g_l, g_u, lower, upper, gamma, beta, sums, d, p, eps, act, by_channel, by_group);
-    if (d_l != nullptr) {
-        bound_back_apply_kernel<V><<<grid, kNormThreads, two, st>>>(g_l, g_u, lower, upper, gamma, beta, sums, by_group, d, p, eps, act, d_l, d_u);
-        ++launched;
+    float2* by_channel = reinterpret_cast<float2*>(static_cast<char*>(ws) + parts_bytes(d, p));
+    if (p.kept) {
+        const int rc = launch_kept(bound_back_kept_kernel<V>, p, bound_space<V>(p, 4).bytes, st, in4, given.gamma, given.beta, sums, d, p, eps,
+                                   act, d_l, d_u, by_channel);
+        if (rc) return rc;
+    } else {
+        const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
+        const size_t shared = bound_space<V>(p, 0).bytes;
+        if (!allow_shared(bound_back_sums_kernel<V>, shared) || !allow_shared(bound_back_apply_kernel<V>, shared)) return LINF_ERR_LAUNCH;
+        bound_back_sums_kernel<V><<<grid, kNormThreads, shared, st>>>(in4, given.gamma, given.beta, sums, d, p, eps, act, by_channel, by_group);
+        if (d_l != nullptr)
+            bound_back_apply_kernel<V><<<grid, kNormThreads, shared, st>>>(in4, given.gamma, given.beta, sums, by_group, d, p, eps, act, d_l, d_u);
+        if (launch_status(d_l != nullptr ? 2 : 1)) return LINF_ERR_LAUNCH;
     }
-    if (launch_status(launched)) return LINF_ERR_LAUNCH;
-    return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, (long long)d.N * p.splits, d.C, dgamma, dbeta, LINF_F32, st) : LINF_OK;
-}
-
-size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
-    return sizeof(Sum4) * (size_t)d.N * p.splits * d.G * p.pieces + (back ? sizeof(float2) * (size_t)d.N * p.splits * d.C : 0);
+    return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, channel_rows(p), d.C, dgamma, dbeta, LINF_F32, st) : LINF_OK;
 }
 
 }  // namespace
@@ -396,7 +563,7 @@ size_t group_norm_bound_workspace(int N, int C, int G, int L, bool back) {
     for (int k = 0; k < 2; ++k) {
         NormDims d;
         NormPlan p;
-        if (norm_make(N, C, G, L, 4, k == 0, &d, &p) != LINF_OK) return 0;
+        if (norm_make(N, C, G, L, bound_kind(back), k == 0, &d, &p) != LINF_OK) return 0;
         const size_t need = workspace(d, p, back);
         if (need > most) most = need;
     }
@@ -407,12 +574,15 @@ int group_norm_bound_forward(const float* lower, const float* upper, const float
                              int act, float* out_l, float* out_u, double* sums, void* ws, size_t ws_bytes, cudaStream_t st) {
     NormDims d;
     NormPlan p;
-    const int rc = norm_make(N, C, G, L, 4, aligned16(lower) && aligned16(upper) && aligned16(out_l) && aligned16(out_u), &d, &p);
+    const int rc = norm_make(N, C, G, L, bound_kind(false), aligned16(lower) && aligned16(upper) && aligned16(out_l) && aligned16(out_u), &d, &p);
     if (rc) return rc;
-    if (ws == nullptr || !aligned16(ws) || ws_bytes < workspace(d, p, false)) return LINF_ERR_WORKSPACE;
+    const size_t need = workspace(d, p, false);
+    if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need)) return LINF_ERR_WORKSPACE;
+    NormGiven given;
+    if (!norm_given(gamma, beta, LINF_F32, &given)) return LINF_ERR_LAUNCH;
     Sum4* s = reinterpret_cast<Sum4*>(sums);
-    return p.V == 4 ? forward<4>(lower, upper, gamma, beta, d, p, eps, act, out_l, out_u, s, ws, st)
-                    : forward<1>(lower, upper, gamma, beta, d, p, eps, act, out_l, out_u, s, ws, st);
+    return p.V == 4 ? forward<4>(lower, upper, given, d, p, eps, act, out_l, out_u, s, ws, st)
+                    : forward<1>(lower, upper, given, d, p, eps, act, out_l, out_u, s, ws, st);
 }
 
 int group_norm_bound_backward(const float* g_l, const float* g_u, const float* lower, const float* upper, const float* gamma, const float* beta,
@@ -420,12 +590,17 @@ int group_norm_bound_backward(const float* g_l, const float* g_u, const float* l
                               float* dbeta, void* ws, size_t ws_bytes, cudaStream_t st) {
     NormDims d;
     NormPlan p;
-    const int rc = norm_make(N, C, G, L, 4, aligned16(g_l) && aligned16(g_u) && aligned16(lower) && aligned16(upper) && aligned16(d_l) && aligned16(d_u), &d, &p);
+    const int rc = norm_make(N, C, G, L, bound_kind(true),
+                             aligned16(g_l) && aligned16(g_u) && aligned16(lower) && aligned16(upper) && aligned16(d_l) && aligned16(d_u), &d, &p);
     if (rc) return rc;
-    if (ws == nullptr || !aligned16(ws) || ws_bytes < workspace(d, p, true)) return LINF_ERR_WORKSPACE;
+    const size_t need = workspace(d, p, true);
+    if (ws == nullptr || !aligned16(ws) || ws_bytes < need) return LINF_ERR_WORKSPACE;
+    NormGiven given;
+    if (!norm_given(gamma, beta, LINF_F32, &given)) return LINF_ERR_LAUNCH;
     const Sum4* s = reinterpret_cast<const Sum4*>(sums);
-    return p.V == 4 ? backward<4>(g_l, g_u, lower, upper, gamma, beta, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st)
-                    : backward<1>(g_l, g_u, lower, upper, gamma, beta, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st);
+    const In4 in4 = {g_l, g_u, lower, upper};
+    return p.V == 4 ? backward<4>(in4, given, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st)
+                    : backward<1>(in4, given, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st);
 }
 
 }  // namespace linf

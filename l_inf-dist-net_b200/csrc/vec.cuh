@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace linf {
@@ -30,15 +32,38 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(f
 template <typename T, int V>
 __device__ __forceinline__ void unpack(const Raw<T, V>& raw, float (&f)[V]) {
     const T* e = reinterpret_cast<const T*>(&raw);
+    const unsigned* w = reinterpret_cast<const unsigned*>(&raw);
+    if (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = to_float<T>(e[j]);
+        for (int j = 0; j < V / 2; ++j) {                           // two elements of a word: one operation each
+            if (std::is_same<T, __nv_bfloat16>::value) {
+                f[2 * j] = __uint_as_float(w[j] << 16);
+                f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+            } else {
+                const float2 p = __half22float2(*reinterpret_cast<const __half2*>(w + j));
+                f[2 * j] = p.x;
+                f[2 * j + 1] = p.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = to_float<T>(e[j]);
+    }
 }
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> pack(const float (&f)[V]) {
     Raw<T, V> raw;
     T* e = reinterpret_cast<T*>(&raw);
+    if (sizeof(T) == 2 && V > 1) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) e[j] = from_float<T>(f[j]);
+        for (int j = 0; j < V / 2; ++j) {
+            if (std::is_same<T, __nv_bfloat16>::value) reinterpret_cast<__nv_bfloat162*>(&raw)[j] = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+            else reinterpret_cast<__half2*>(&raw)[j] = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) e[j] = from_float<T>(f[j]);
+    }
     return raw;
 }
 template <typename T, int V>
@@ -48,11 +73,32 @@ __device__ __forceinline__ Raw<T, V> load_once(const T* p) { return __ldcs(reint
 template <typename T, int V>
 __device__ __forceinline__ void store_once(T* p, const Raw<T, V>& v) { __stcs(reinterpret_cast<Raw<T, V>*>(p), v); }
 
-// a parameter vector of float or of the activations' 16-bit type
-__device__ __forceinline__ float load_param(const void* p, int c, int type) {
-    if (type == LINF_F32) return __ldg(static_cast<const float*>(p) + c);
-    if (type == LINF_F16) return __half2float(__ldg(static_cast<const __half*>(p) + c));
-    return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p) + c));
+// A parameter vector, fp32 or of the activations' 16-bit type; kind PARAM_ONE: one value in the place of a vector that was not given, so
+// that no kernel holds a pointer that it must not follow; PARAM_WIDE: fp32 on a 16-byte boundary.
+enum { PARAM_ONE, PARAM_WIDE, PARAM_F32, PARAM_F16, PARAM_BF16 };
+struct Param { const void* at; int kind; };
+__device__ __forceinline__ float load_param(const Param& p, int c) {
+    if (p.kind == PARAM_ONE) return __ldg(static_cast<const float*>(p.at));
+    if (p.kind <= PARAM_F32) return __ldg(static_cast<const float*>(p.at) + c);
+    if (p.kind == PARAM_F16) return __half2float(__ldg(static_cast<const __half*>(p.at) + c));
+    return __bfloat162float(__ldg(static_cast<const __nv_bfloat16*>(p.at) + c));
+}
+// the values of channels c .. c + V - 1 (c a multiple of V)
+template <int V>
+__device__ __forceinline__ void load_params(const Param& p, int c, float (&f)[V]) {
+    if (V % 4 == 0 && p.kind == PARAM_WIDE) {
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.at) + c) + j);
+            f[4 * j] = q.x;
+            f[4 * j + 1] = q.y;
+            f[4 * j + 2] = q.z;
+            f[4 * j + 3] = q.w;
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = load_param(p, c + j);
 }
 __device__ __forceinline__ void store_param(void* p, int c, int type, float v) {
     if (type == LINF_F32) static_cast<float*>(p)[c] = v;
@@ -60,28 +106,105 @@ __device__ __forceinline__ void store_param(void* p, int c, int type, float v) {
     else static_cast<__nv_bfloat16*>(p)[c] = __float2bfloat16_rn(v);
 }
 
+// ---- V values at a time, two to an instruction ------------------------------------------------------------------
+template <int V> __device__ __forceinline__ void add_all(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
+    if (V == 1) { r[0] = a[0] + b[0]; return; }
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(add_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), r[j], r[j + 1]);
+}
+template <int V> __device__ __forceinline__ void sub_all(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
+    if (V == 1) { r[0] = a[0] - b[0]; return; }
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(sub_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), r[j], r[j + 1]);
+}
+template <int V> __device__ __forceinline__ void mul_all(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
+    if (V == 1) { r[0] = a[0] * b[0]; return; }
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(mul_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), r[j], r[j + 1]);
+}
+template <int V> __device__ __forceinline__ void mul_all(float (&r)[V], const float (&a)[V], float b) {
+    if (V == 1) { r[0] = a[0] * b; return; }
+    const unsigned long long two = pack_f32x2(b, b);
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(mul_f32x2(pack_f32x2(a[j], a[j + 1]), two), r[j], r[j + 1]);
+}
+template <int V> __device__ __forceinline__ void fma_all(float (&r)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+    if (V == 1) { r[0] = fmaf(a[0], b[0], c[0]); return; }
+#pragma unroll
+    for (int j = 0; j + 1 < V; j += 2)
+        unpack_f32x2(fma_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1]), pack_f32x2(c[j], c[j + 1])), r[j], r[j + 1]);
+}
+
 // ---- activations: the value, and the value's derivative ---------------------------------------------------------
 // silu(u) = u / (1 + e^-u) has one minimum, at u = kSiluArg; it falls before and rises behind it
 constexpr double kSiluArg64 = -1.278464542761074;
 constexpr float kSiluArg = (float)kSiluArg64;
 
-__device__ __forceinline__ float sigmoid(float u) { return __fdividef(1.f, 1.f + __expf(-u)); }   // both ends come out as 1 and 0
-__device__ __forceinline__ float activate(float u, int act) {
-    switch (act) {
-        case LINF_ACT_RELU: return u < 0.f ? 0.f : u;            // keeps a NaN
-        case LINF_ACT_TANH: return tanhf(u);
-        case LINF_ACT_SILU: return u * sigmoid(u);
-        default: return u;
+// 2^x and 1 / x of the special-function unit (relative error 2^-22 and 2^-23 by their specification; subnormals count as 0)
+__device__ __forceinline__ float exp2_unit(float x) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+__device__ __forceinline__ float rcp_unit(float x) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x)); return r; }
+constexpr float kLog2E = 1.44269504088896f;
+
+// tanh for results that are rounded to 16 bits: 1 - 2 / (1 + e^2u) is off by up to 2^-22, which is below a half step of the
+// result's type from |u| = 2^-4 on; below, the series to u^5 is off by 17/315 u^7, less than 2^-28 of u
+__device__ __forceinline__ float tanh16(float u) {
+    const float s = u * u, series = u * fmaf(s, fmaf(s, 2.f / 15.f, -1.f / 3.f), 1.f);
+    const float far = fmaf(-2.f, rcp_unit(1.f + exp2_unit(2.f * kLog2E * u)), 1.f);
+    return s < 1.f / 256.f ? series : far;
+}
+template <bool WIDE> __device__ __forceinline__ float tanh_of(float u) { return WIDE ? tanhf(u) : tanh16(u); }
+
+// 1 / (1 + e^-u): both ends come out as 1 and 0
+template <int V> __device__ __forceinline__ void sigmoid_all(float (&q)[V], const float (&u)[V]) {
+    float one[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) one[j] = 1.f;
+    mul_all<V>(q, u, -kLog2E);
+#pragma unroll
+    for (int j = 0; j < V; ++j) q[j] = exp2_unit(q[j]);
+    add_all<V>(q, q, one);
+#pragma unroll
+    for (int j = 0; j < V; ++j) q[j] = rcp_unit(q[j]);
+}
+
+// WIDE: the results stay fp32.
+template <bool WIDE, int V>
+__device__ __forceinline__ void activate_all(float (&f)[V], int act) {
+    if (act == LINF_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = f[j] < 0.f ? 0.f : f[j];          // keeps a NaN
+    } else if (act == LINF_ACT_TANH) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = tanh_of<WIDE>(f[j]);
+    } else if (act == LINF_ACT_SILU) {
+        float q[V];
+        sigmoid_all<V>(q, f);
+        mul_all<V>(f, f, q);
     }
 }
-__device__ __forceinline__ float slope(float u, int act) {
-    switch (act) {
-        case LINF_ACT_RELU: return u > 0.f ? 1.f : 0.f;
-        case LINF_ACT_TANH: { const float t = tanhf(u); return 1.f - t * t; }
-        case LINF_ACT_SILU: { const float q = sigmoid(u); return q * (1.f + u * (1.f - q)); }
-        default: return 1.f;
+template <bool WIDE, int V>
+__device__ __forceinline__ void slope_all(float (&f)[V], int act) {
+    if (act == LINF_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = f[j] > 0.f ? 1.f : 0.f;
+    } else if (act == LINF_ACT_TANH) {
+#pragma unroll
+        for (int j = 0; j < V; ++j) { const float t = tanh_of<WIDE>(f[j]); f[j] = fmaf(-t, t, 1.f); }
+    } else if (act == LINF_ACT_SILU) {
+        float q[V], one[V], rest[V];
+        sigmoid_all<V>(q, f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) one[j] = 1.f;
+        sub_all<V>(rest, one, q);
+        fma_all<V>(f, f, rest, one);
+        mul_all<V>(f, f, q);
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] = 1.f;
     }
 }
+__device__ __forceinline__ float activate(float u, int act) { float f[1] = {u}; activate_all<true, 1>(f, act); return f[0]; }
+__device__ __forceinline__ float slope(float u, int act) { float f[1] = {u}; slope_all<true, 1>(f, act); return f[0]; }
 
 // ---- counter-based dropout --------------------------------------------------------------------------------------
 // Philox4x32 with 7 rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011; 7 is the least
@@ -92,7 +215,8 @@ __device__ __forceinline__ float slope(float u, int act) {
 // makes up for the rounded rate, so that the expectation is exact.  With 32 bits and 10 rounds a pass over 64 Mi bf16 values took 72 us
 // for the integer multiplications alone, with 16 bits 49 us, without a generator 44 us.
 struct Drop {
-    const long long* rng;       // {seed, offset} on the device, null = no dropout
+    const long long* rng;       // {seed, offset} on the device
+    int on;                     // 0: no dropout
     unsigned threshold;         // 0 .. 65536
     float scale;
 };
@@ -114,24 +238,46 @@ __device__ __forceinline__ uint4 drop_words(const DropKey& k, unsigned long long
     }
     return c;
 }
-// f[j] of element i0 + j (i0 a multiple of V): scaled where it is kept, 0 where not (whatever the value was, a NaN included)
+// Bit j: element i0 + j (i0 a multiple of V) is kept.
+template <int V>
+__device__ __forceinline__ unsigned drop_mask(const Drop& d, const DropKey& k, unsigned long long i0) {
+    const uint4 w = drop_words(k, i0 >> 3);
+    unsigned mask = 0;
+    if (V == 8) {
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < V; ++j) mask |= (((j & 1) ? u[(j >> 1) & 3] >> 16 : u[(j >> 1) & 3] & 0xffffu) >= d.threshold ? 1u : 0u) << j;
+    } else {
+        const bool second = (i0 & 4) != 0;
+        unsigned long long bits = second ? ((unsigned long long)w.w << 32 | w.z) : ((unsigned long long)w.y << 32 | w.x);
+        if (V < 4) bits >>= 16 * (unsigned)(i0 & 3);
+#pragma unroll
+        for (int j = 0; j < V; ++j) mask |= ((unsigned)((bits >> (16 * (j & 3))) & 0xffffu) >= d.threshold ? 1u : 0u) << j;
+    }
+    return mask;
+}
+template <int V>
+__device__ __forceinline__ void drop_masked(const Drop& d, unsigned mask, float (&f)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = (mask >> j & 1u) ? f[j] * d.scale : 0.f;
+}
+// scaled where the piece keeps it, 0 where not (whatever the value was, a NaN included)
+__device__ __forceinline__ float drop_one(const Drop& d, unsigned piece, float f) { return piece >= d.threshold ? f * d.scale : 0.f; }
+// f[j] of element i0 + j (i0 a multiple of V)
 template <int V>
 __device__ __forceinline__ void drop_apply(const Drop& d, const DropKey& k, unsigned long long i0, float (&f)[V]) {
     const uint4 w = drop_words(k, i0 >> 3);
     if (V == 8) {
         const unsigned u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const unsigned piece = (j & 1) ? u[(j >> 1) & 3] >> 16 : u[(j >> 1) & 3] & 0xffffu;
-            f[j] = piece >= d.threshold ? f[j] * d.scale : 0.f;
-        }
+        for (int j = 0; j < V; ++j) f[j] = drop_one(d, (j & 1) ? u[(j >> 1) & 3] >> 16 : u[(j >> 1) & 3] & 0xffffu, f[j]);
     } else {
         // the 64 bits that hold the pieces of this element's half of the block, shifted to its first piece
         const bool second = (i0 & 4) != 0;
         unsigned long long bits = second ? ((unsigned long long)w.w << 32 | w.z) : ((unsigned long long)w.y << 32 | w.x);
         if (V < 4) bits >>= 16 * (unsigned)(i0 & 3);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = (unsigned)((bits >> (16 * (j & 3))) & 0xffffu) >= d.threshold ? f[j] * d.scale : 0.f;
+        for (int j = 0; j < V; ++j) f[j] = drop_one(d, (unsigned)((bits >> (16 * (j & 3))) & 0xffffu), f[j]);
     }
 }
 
@@ -140,7 +286,8 @@ inline bool make_drop(double rate, const long long* rng, Drop* d) {
     if (!(rate >= 0.0 && rate <= 1.0)) return false;
     d->threshold = (unsigned)(rate * 65536.0 + 0.5);
     d->scale = d->threshold < 65536u ? (float)(65536.0 / (65536.0 - (double)d->threshold)) : 0.f;
-    d->rng = d->threshold > 0 ? rng : nullptr;      // a threshold of 0 keeps every element as it is
+    d->rng = rng;
+    d->on = d->threshold > 0;                       // a threshold of 0 keeps every element as it is
     return true;
 }
 

@@ -14,6 +14,15 @@ from .norm_dist import _on, _stream
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # LINF_F32, LINF_F16, LINF_BF16
 
 
+def _once(backward):
+    """A backward pass that may be differentiated no further (once_differentiable, without its guard where no graph is made of it)."""
+    checked = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 def _floating(t, name):
     if t.dtype not in _TYPES:
         raise RuntimeError(f"{name} must have dtype torch.float32, torch.float16 or torch.bfloat16")
@@ -47,38 +56,53 @@ def _as_stored(t, last):
     return t.contiguous() if not last else t.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-def _launch(tensors, rate, rng):
-    outs = [None if t is None else torch.empty_like(t) for t in tensors]
-    some = next(t for t in tensors if t is not None)
-    if some.numel() == 0:
-        return outs
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    with _on(some.device):
-        rc = _lib.load().linf_dropout(*map(ptr, tensors), some.numel(), _TYPES[some.dtype], rate, rng.data_ptr(), *map(ptr, outs), _stream())
-    _lib.check(rc, "dropout")
+def _launch(rate, rng, a, b=None, c=None):
+    """The mask on up to three tensors (each may be None); as many results."""
+    some = a if a is not None else b if b is not None else c
+    if some is None:
+        return None, None, None
+    outs = [None if t is None else torch.empty_like(t) for t in (a, b, c)]
+    if some.numel() > 0:
+        ptr = [None if t is None else t.data_ptr() for t in (a, b, c, *outs)]
+        with _on(some.device):
+            rc = _lib.load().linf_dropout(*ptr[:3], some.numel(), _TYPES[some.dtype], rate, rng.data_ptr(), *ptr[3:], _stream())
+        _lib.check(rc, "dropout")
     return outs
 
 
 class DropoutF(torch.autograd.Function):
-    """The same mask on each of up to three tensors; the backward pass drops the gradients under it."""
 
     @staticmethod
-    def forward(ctx, rate, rng, *tensors):
-        ctx.set_materialize_grads(False)
-        last = not tensors[0].is_contiguous() and _is_last(tensors[0])
+    def forward(ctx, x, rate, rng):
+        last = not x.is_contiguous() and _is_last(x)
         ctx.last, ctx.rate = last, rate
         ctx.save_for_backward(rng)
-        return tuple(_launch([_as_stored(t, last) for t in tensors] + [None] * (3 - len(tensors)), rate, rng)[:len(tensors)])
+        return _launch(rate, rng, _as_stored(x, last))[0]
 
     @staticmethod
-    @once_differentiable
+    @_once
+    def backward(ctx, grad):
+        rng, = ctx.saved_tensors
+        return _launch(ctx.rate, rng, _as_stored(grad, ctx.last))[0], None, None
+
+
+class DropoutTripleF(torch.autograd.Function):
+    """The same mask on up to three tensors (c may be None)."""
+
+    @staticmethod
+    def forward(ctx, rate, rng, a, b, c):
+        ctx.set_materialize_grads(False)
+        last = not a.is_contiguous() and _is_last(a)
+        ctx.last, ctx.rate = last, rate
+        ctx.save_for_backward(rng)
+        return tuple(_launch(rate, rng, *[None if t is None else _as_stored(t, last) for t in (a, b, c)]))
+
+    @staticmethod
+    @_once
     def backward(ctx, *grads):
         rng, = ctx.saved_tensors
-        asked = [g if need else None for g, need in zip(grads, ctx.needs_input_grad[2:])]
-        given = [None if g is None else _as_stored(g, ctx.last) for g in asked]
-        if all(g is None for g in given):
-            return (None, None, *given)
-        return (None, None, *_launch(given + [None] * (3 - len(given)), ctx.rate, rng)[:len(given)])
+        given = [_as_stored(g, ctx.last) if need and g is not None else None for g, need in zip(grads, ctx.needs_input_grad[2:])]
+        return (None, None, *_launch(ctx.rate, rng, *given))
 
 
 def dropout_next(state):
@@ -104,16 +128,17 @@ def dropout(x, rate, rng, lower=None, upper=None):
     in memory where x is contiguous or has its channels last; another layout is copied to a contiguous one first, and
     lower / upper to the layout of x."""
     rate = _rate(rate)
-    tensors = [x] + [t for t in (lower, upper) if t is not None]
     if (lower is None) != (upper is None):
         raise RuntimeError("lower and upper are given together")
-    for t, name in zip(tensors[1:], ("lower", "upper")):
-        if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
-            raise RuntimeError(f"{name} must have the shape, dtype and device of x")
+    if lower is not None:
+        for t, name in ((lower, "lower"), (upper, "upper")):
+            if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+                raise RuntimeError(f"{name} must have the shape, dtype and device of x")
     _generator_state(rng, x.device)
     _floating(x, "x")
-    outs = DropoutF.apply(rate, rng, *tensors)
-    return outs[0] if lower is None else outs
+    if lower is None:
+        return DropoutF.apply(x, rate, rng)
+    return DropoutTripleF.apply(rate, rng, x, lower, upper)
 
 
 class _Masks(nn.Module):

@@ -9,156 +9,187 @@ import math
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .dropout import DropoutF, _Masks, _TYPES, _floating, _generator_state, _rate, dropout_next
+from .dropout import DropoutTripleF, _Masks, _TYPES, _floating, _generator_state, _once, _rate, dropout_next
 from .norm_dist import _on, _scratch, _stream, skips_values
 
 ACTIVATIONS = {"identity": 0, "relu": 1, "tanh": 2, "silu": 3}        # LINF_ACT_*
 
 
 def _rows(t):
-    """[N, C, ...] -> its memory as [N, ..., C]: the tensor itself where the channels lie last, or a copy."""
-    t = t.movedim(1, -1)
-    return t if t.is_contiguous() else t.contiguous()
+    """[N, C, ...] -> the tensor itself where its channels lie last in memory, or a copy for which they do."""
+    if t.is_contiguous() if t.dim() == 2 else t.movedim(1, -1).is_contiguous():
+        return t
+    return t.movedim(1, -1).contiguous().movedim(-1, 1)
 
 
-def _empty(shape, like):
-    """[N, C, ...] with the channels last in memory."""
-    if len(shape) == 2:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
-    strides, step = [0] * len(shape), shape[1]
-    strides[1] = 1
-    for k in range(len(shape) - 1, 1, -1):
-        strides[k] = step
-        step *= shape[k]
-    strides[0] = step
-    return torch.empty_strided(shape, strides, dtype=like.dtype, device=like.device)
+class _Call:
+    """What a call has besides its tensors.  sizes: (N, C, groups, positions)."""
+    __slots__ = ("sizes", "type", "param_type", "eps", "act", "rate", "rng")
 
 
-def _sizes(shape, groups):
-    return shape[0], shape[1], groups, math.prod(shape[2:])
+_workspace_bytes = {}
+
+
+def _work_space(query, device, *key):
+    """Scratch of a call (from the current stream's pool), or None where it needs none; what a call needs is asked once."""
+    need = _workspace_bytes.get((query, device.index, key))
+    if need is None:
+        need = _workspace_bytes[query, device.index, key] = getattr(_lib.load(), query)(*key)
+    return _scratch(device, need) if need else None, need
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _norm_forward(call, x, weight, bias, keep):
+    """The result, and with `keep` what the backward pass needs of it."""
+    rows = _rows(x)
+    y = torch.empty_like(rows)
+    sizes = call.sizes
+    stats = torch.empty(2, sizes[0], sizes[2], device=x.device, dtype=torch.float32) if keep else None
+    if x.numel() > 0:
+        with _on(x.device):
+            ws, need = _work_space("linf_group_norm_workspace_bytes", x.device, *sizes, call.type, 0)
+            at = stats.data_ptr() if keep else 0
+            rc = _lib.load().linf_group_norm_forward(
+                rows.data_ptr(), _ptr(weight), _ptr(bias), *sizes, call.type, call.param_type, call.eps, call.act, call.rate, _ptr(call.rng),
+                y.data_ptr(), at or None, at + 4 * sizes[0] * sizes[2] if keep else None, _ptr(ws), need, _stream())
+        _lib.check(rc, "group_norm_forward")
+    return y, rows, stats
+
+
 class GroupNormF(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, rate, rng):
-        lib = _lib.load()
-        rows = _rows(x)
-        y = _empty(x.shape, x)
-        sizes = _sizes(x.shape, groups)
-        kept = any(ctx.needs_input_grad[:3])
-        stats = torch.empty((2, sizes[0], groups) if kept else (0,), device=x.device, dtype=torch.float32)
-        ctx.call = (sizes, _TYPES[x.dtype], _TYPES[weight.dtype] if weight is not None else _TYPES[bias.dtype] if bias is not None else 0, act, rate)
-        if x.numel() > 0:
-            with _on(x.device):
-                need = lib.linf_group_norm_workspace_bytes(*sizes, ctx.call[1], 0)
-                ws = _scratch(x.device, need)
-                rc = lib.linf_group_norm_forward(rows.data_ptr(), _ptr(weight), _ptr(bias), *sizes, *ctx.call[1:3], eps, act, rate, _ptr(rng),
-                                                 y.data_ptr(), stats[0].data_ptr() if kept else None, stats[1].data_ptr() if kept else None,
-                                                 ws.data_ptr(), need, _stream())
-            _lib.check(rc, "group_norm_forward")
-        if kept:
-            ctx.save_for_backward(rows, weight, bias, stats, rng)
+    def forward(ctx, x, weight, bias, call):
+        y, rows, stats = _norm_forward(call, x, weight, bias, True)
+        ctx.call, ctx.stats = call, stats
+        ctx.save_for_backward(rows, weight, bias, call.rng)
         return y
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_output):
-        lib = _lib.load()
-        rows, weight, bias, stats, rng = ctx.saved_tensors
-        sizes, kind, ptype, act, rate = ctx.call
+        call = ctx.call
+        rows, weight, bias, rng = ctx.saved_tensors
+        sizes = call.sizes
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         g = _rows(grad_output)
-        gx = _empty(grad_output.shape, rows) if ctx.needs_input_grad[0] else None
-        gw = torch.empty_like(weight) if ctx.needs_input_grad[1] else None
-        gb = torch.empty_like(bias) if ctx.needs_input_grad[2] else None
+        gx = torch.empty_like(rows) if need_x else None
+        gw = torch.empty_like(weight) if need_w else None
+        gb = torch.empty_like(bias) if need_b else None
         if rows.numel() == 0:
-            return gx, gw if gw is None else gw.zero_(), gb if gb is None else gb.zero_(), None, None, None, None, None
+            return gx, gw if gw is None else gw.zero_(), gb if gb is None else gb.zero_(), None
         with _on(rows.device):
-            need = lib.linf_group_norm_workspace_bytes(*sizes, kind, 1)
-            ws = _scratch(rows.device, need)
-            rc = lib.linf_group_norm_backward(g.data_ptr(), rows.data_ptr(), _ptr(weight), _ptr(bias), stats[0].data_ptr(), stats[1].data_ptr(),
-                                              *sizes, kind, ptype, act, rate, _ptr(rng), _ptr(gx), _ptr(gw), _ptr(gb), ws.data_ptr(), need, _stream())
+            ws, need = _work_space("linf_group_norm_workspace_bytes", rows.device, *sizes, call.type, 1)
+            at = ctx.stats.data_ptr()
+            rc = _lib.load().linf_group_norm_backward(
+                g.data_ptr(), rows.data_ptr(), _ptr(weight), _ptr(bias), at, at + 4 * sizes[0] * sizes[2], *sizes, call.type, call.param_type,
+                call.act, call.rate, _ptr(rng), _ptr(gx), _ptr(gw), _ptr(gb), _ptr(ws), need, _stream())
         _lib.check(rc, "group_norm_backward")
-        return gx, gw, gb, None, None, None, None, None
+        return gx, gw, gb, None
+
+
+def _bound_forward(call, lower, upper, weight, bias, keep):
+    l, u = _rows(lower), _rows(upper)
+    lo, up = torch.empty_like(l), torch.empty_like(l)
+    sizes = call.sizes
+    sums = torch.empty(sizes[0], sizes[2], 4, device=l.device, dtype=torch.float64) if keep else None
+    if l.numel() > 0:
+        with _on(l.device):
+            ws, need = _work_space("linf_group_norm_bound_workspace_bytes", l.device, *sizes, 0)
+            rc = _lib.load().linf_group_norm_bound_forward(l.data_ptr(), u.data_ptr(), _ptr(weight), _ptr(bias), *sizes, call.eps, call.act,
+                                                           lo.data_ptr(), up.data_ptr(), _ptr(sums), _ptr(ws), need, _stream())
+        _lib.check(rc, "group_norm_bound_forward")
+    return lo, up, l, u, sums
 
 
 class GroupNormBoundF(torch.autograd.Function):
 
     @staticmethod
-    def forward(ctx, lower, upper, weight, bias, groups, eps, act):
-        lib = _lib.load()
-        l, u = _rows(lower), _rows(upper)
-        lo, up = _empty(lower.shape, lower), _empty(lower.shape, lower)
-        sizes = _sizes(lower.shape, groups)
-        kept = any(ctx.needs_input_grad[:4])
-        sums = torch.empty((sizes[0], groups, 4) if kept else (0,), device=lower.device, dtype=torch.float64)
-        ctx.call = (sizes, eps, act)
-        if lower.numel() > 0:
-            with _on(lower.device):
-                need = lib.linf_group_norm_bound_workspace_bytes(*sizes, 0)
-                ws = _scratch(lower.device, need)
-                rc = lib.linf_group_norm_bound_forward(l.data_ptr(), u.data_ptr(), _ptr(weight), _ptr(bias), *sizes, eps, act, lo.data_ptr(),
-                                                       up.data_ptr(), sums.data_ptr() if kept else None, ws.data_ptr(), need, _stream())
-            _lib.check(rc, "group_norm_bound_forward")
-        if kept:
-            ctx.save_for_backward(l, u, weight, bias, sums)
+    def forward(ctx, lower, upper, weight, bias, call):
+        lo, up, l, u, sums = _bound_forward(call, lower, upper, weight, bias, True)
+        ctx.call, ctx.sums = call, sums
+        ctx.save_for_backward(l, u, weight, bias)
         return lo, up
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_lower, grad_upper):
-        lib = _lib.load()
-        l, u, weight, bias, sums = ctx.saved_tensors
-        sizes, eps, act = ctx.call
+        call = ctx.call
+        l, u, weight, bias = ctx.saved_tensors
+        sizes = call.sizes
+        need_l, need_u, need_w, need_b, _ = ctx.needs_input_grad
         gl, gu = _rows(grad_lower), _rows(grad_upper)
-        box = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        dl, du = (_empty(grad_lower.shape, l), _empty(grad_lower.shape, l)) if box else (None, None)
-        gw = torch.empty_like(weight) if ctx.needs_input_grad[2] else None
-        gb = torch.empty_like(bias) if ctx.needs_input_grad[3] else None
+        dl, du = (torch.empty_like(l), torch.empty_like(l)) if need_l or need_u else (None, None)
+        gw = torch.empty_like(weight) if need_w else None
+        gb = torch.empty_like(bias) if need_b else None
         if l.numel() == 0:
-            return dl, du, gw if gw is None else gw.zero_(), gb if gb is None else gb.zero_(), None, None, None
+            return dl, du, gw if gw is None else gw.zero_(), gb if gb is None else gb.zero_(), None
         with _on(l.device):
-            need = lib.linf_group_norm_bound_workspace_bytes(*sizes, 1)
-            ws = _scratch(l.device, need)
-            rc = lib.linf_group_norm_bound_backward(gl.data_ptr(), gu.data_ptr(), l.data_ptr(), u.data_ptr(), _ptr(weight), _ptr(bias),
-                                                    sums.data_ptr(), *sizes, eps, act, _ptr(dl), _ptr(du), _ptr(gw), _ptr(gb), ws.data_ptr(),
-                                                    need, _stream())
+            ws, need = _work_space("linf_group_norm_bound_workspace_bytes", l.device, *sizes, 1)
+            rc = _lib.load().linf_group_norm_bound_backward(gl.data_ptr(), gu.data_ptr(), l.data_ptr(), u.data_ptr(), _ptr(weight), _ptr(bias),
+                                                            ctx.sums.data_ptr(), *sizes, call.eps, call.act, _ptr(dl), _ptr(du), _ptr(gw), _ptr(gb),
+                                                            _ptr(ws), need, _stream())
         _lib.check(rc, "group_norm_bound_backward")
-        return (dl if ctx.needs_input_grad[0] else None, du if ctx.needs_input_grad[1] else None, gw, gb, None, None, None)
+        return dl if need_l else None, du if need_u else None, gw, gb, None
 
 
-def _check_norm(x, name, groups, weight, bias, eps, activation):
-    if x.dim() < 2:
+_checked = {}
+
+
+def _check_sizes(shape, name, groups, eps, activation):
+    """(sizes, activation's number, eps) of a call; what was found once for a shape is kept."""
+    key = (shape, groups, eps, activation)
+    found = _checked.get(key)
+    if found is not None:
+        return found
+    if len(shape) < 2:
         raise RuntimeError(f"{name} must be [N, C, ...]")
-    groups, C = int(groups), x.size(1)
+    groups, C, positions = int(groups), shape[1], math.prod(shape[2:])
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("the channel count must be a multiple of the group count")
-    if max(x.size(0), C, math.prod(x.shape[2:])) >= 2 ** 31:
+    if max(shape[0], C, positions) >= 2 ** 31:
         raise RuntimeError(f"each size of {name} must be below 2^31")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
     if not (math.isfinite(eps) and eps > 0):
         raise ValueError("eps must be finite and greater than 0")
+    if len(_checked) >= 4096:
+        _checked.clear()
+    found = _checked[key] = ((shape[0], C, groups, positions), ACTIVATIONS[activation], float(eps))
+    return found
+
+
+def _make_call(x, name, groups, weight, bias, eps, activation):
+    """Checks the arguments; what the kernels are to be told of them."""
+    call = _Call()
+    call.sizes, call.act, call.eps = _check_sizes(x.shape, name, groups, eps, activation)
+    call.rate, call.rng, call.param_type = 0.0, None, 0
+    C, dtype, device = call.sizes[1], x.dtype, x.device
     for v, what in ((weight, "weight"), (bias, "bias")):
         if v is None:
             continue
-        if v.shape != (C,) or not v.is_contiguous():
+        if v.dim() != 1 or v.size(0) != C or not v.is_contiguous():
             raise RuntimeError(f"{what} must be contiguous, with one element for each of the {C} channels")
-        if v.device != x.device:
+        if v.device != device:
             raise RuntimeError(f"{what} must be on the device of {name}")
-        if v.dtype not in (torch.float32, x.dtype):
-            raise RuntimeError(f"{what} must have dtype torch.float32 or that of {name}")
+        if v.dtype != torch.float32:
+            if v.dtype != dtype:
+                raise RuntimeError(f"{what} must have dtype torch.float32 or that of {name}")
+            call.param_type = _TYPES.get(dtype, 0)
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise RuntimeError("weight and bias must have one dtype")
     _floating(x, name)
-    return groups, float(eps), ACTIVATIONS[activation]
+    call.type = _TYPES[dtype]
+    return call
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation="identity", rate=0.0, rng=None):
@@ -173,8 +204,12 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation="identity
         if rng is None:
             raise RuntimeError("a rate above 0 needs rng, an int64 tensor of seed and offset")
         _generator_state(rng, x.device)
-    groups, eps, act = _check_norm(x, "x", groups, weight, bias, eps, activation)
-    return GroupNormF.apply(x, weight, bias, groups, eps, act, rate, rng if rate > 0 else None)
+    call = _make_call(x, "x", groups, weight, bias, eps, activation)
+    if rate > 0:
+        call.rate, call.rng = rate, rng
+    if _wants_grad(x, weight, bias):
+        return GroupNormF.apply(x, weight, bias, call)
+    return _norm_forward(call, x, weight, bias, False)[0]
 
 
 def group_norm_bound(lower, upper, groups, weight=None, bias=None, eps=1e-5, activation="identity"):
@@ -187,8 +222,10 @@ def group_norm_bound(lower, upper, groups, weight=None, bias=None, eps=1e-5, act
         raise RuntimeError("upper must have the shape, dtype and device of lower")
     if lower.dtype != torch.float32:
         raise RuntimeError("bounds must have dtype torch.float32")
-    groups, eps, act = _check_norm(lower, "lower", groups, weight, bias, eps, activation)
-    return GroupNormBoundF.apply(lower, upper, weight, bias, groups, eps, act)
+    call = _make_call(lower, "lower", groups, weight, bias, eps, activation)
+    if _wants_grad(lower, upper, weight, bias):
+        return GroupNormBoundF.apply(lower, upper, weight, bias, call)
+    return _bound_forward(call, lower, upper, weight, bias, False)[:2]
 
 
 class BoundGroupNorm(_Masks):
@@ -214,7 +251,7 @@ class BoundGroupNorm(_Masks):
             return group_norm(x, *args, rate, used), None, None
         lo, up = group_norm_bound(lower, upper, *args)
         if rate > 0:
-            lo, up = DropoutF.apply(rate, used, lo, up)
+            lo, up, _ = DropoutTripleF.apply(rate, used, lo, up, None)
         if skips_values() and not self.training and not torch.is_grad_enabled():
             return lo, lo, up                 # nobody reads the value in such a pass
         return group_norm(x, *args, rate, used), lo, up

@@ -151,7 +151,7 @@ def test_library_refuses(lib):
     p = ctypes.c_void_p(4096)          # never followed: each call is refused before a launch
     inf, nan = float("inf"), float("nan")
     sizes = [(dict(N=0), 2), (dict(C=-4), 2), (dict(G=0), 2), (dict(L=0), 2), (dict(G=3), 3), (dict(L=(1 << 30) + 1), 7)]
-    common = sizes + [(dict(act=4), 11), (dict(act=-1), 11), (dict(ws=None), 6), (dict(ws=ctypes.c_void_p(4097)), 6), (dict(ws_bytes=8), 6)]
+    common = sizes + [(dict(act=4), 11), (dict(act=-1), 11), (dict(L=1 << 20, ws=None), 6), (dict(L=1 << 20, ws=ctypes.c_void_p(4097)), 6), (dict(L=1 << 20, ws_bytes=8), 6)]
     eps = [(dict(eps=0.0), 10), (dict(eps=-1.0), 10), (dict(eps=inf), 10), (dict(eps=nan), 10)]
     kinds = [(dict(type=3), 8), (dict(type=-1), 8), (dict(ptype=2), 8), (dict(rate=-1.0), 9), (dict(rate=nan), 9), (dict(rate=0.5), 9), (dict(rate=2.0), 9)]
     fwd = dict(x=p, w=p, b=p, N=2, C=8, G=2, L=4, type=0, ptype=0, eps=1e-5, act=0, rate=0.0, rng=None, y=p, mean=p, rstd=p, ws=p, ws_bytes=1 << 20, st=None)
