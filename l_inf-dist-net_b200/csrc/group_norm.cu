@@ -18,29 +18,31 @@ namespace {
 struct Own { float one, zero; };
 __device__ Own g_own = {1.f, 0.f};
 
-// What a thread's column needs for u = (x - m) a + o.
-template <int V> struct Column { float m[V], a[V], o[V]; };
+// What a thread's column needs for u = (x + m) a + o: m is the mean with its sign turned.
+template <int V> struct Column { Lanes<V> m, a, o; };
 template <int V>
 __device__ __forceinline__ void load_column(Column<V>& k, const float2* stat, const Param& gamma, const Param& beta, const NormDims& d,
                                             const NormPlan& p, const NormBlock& b, int cv) {
     int g[V];
     groups_of<V>(d, p, cv * V, g);
-    load_params<V>(gamma, b.c0 + cv * V, k.a);
-    load_params<V>(beta, b.c0 + cv * V, k.o);
+    float m[V], a[V], o[V];
+    load_params<V>(gamma, b.c0 + cv * V, a);
+    load_params<V>(beta, b.c0 + cv * V, o);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const float2 s = stat[g[j]];
-        k.m[j] = s.x;
-        k.a[j] *= s.y;
+        m[j] = -s.x;
+        a[j] *= s.y;
     }
+    k.m.set(m);
+    k.a.set(a);
+    k.o.set(o);
 }
 template <typename T, int V>
 __device__ __forceinline__ void write_vector(const Raw<T, V>& v, const Column<V>& col, int act, const Drop& drop, const DropKey& key, size_t i, T* y) {
+    const Lanes<V> u = activate<sizeof(T) == 4, V>(fma(add(lanes_of<T, V>(v), col.m), col.a, col.o), act);
     float f[V];
-    unpack<T, V>(v, f);
-    sub_all<V>(f, f, col.m);
-    fma_all<V>(f, f, col.a, col.o);
-    activate_all<sizeof(T) == 4, V>(f, act);
+    u.get(f);
     if (drop.on) drop_apply<V>(drop, key, i, f);
     store_once<T, V>(y + i, pack<T, V>(f));
 }
@@ -48,47 +50,39 @@ __device__ __forceinline__ float2 finish_stat(double mean, double var, double ep
     return make_float2((float)mean, 1.f / sqrtf((float)(var + eps)));
 }
 
-// A thread's sums of its column about its first row: s = sum (x - k), q = sum (x - k)^2.
-template <typename T, int V> struct Vec { float f[V]; };
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> load_raw_as(const T* p) { Vec<T, V> v; unpack<T, V>(load_raw<T, V>(p), v.f); return v; }
-template <typename T, int V>
-__device__ __forceinline__ Vec<T, V> as_vec(const Raw<T, V>& raw) { Vec<T, V> v; unpack<T, V>(raw, v.f); return v; }
-
+// A thread's sums of its column about its first row: s = sum (x + k), q = sum (x + k)^2, k the first row with its sign turned.
 template <int V> struct Moments {
-    float k[V], s[V], q[V];
-    __device__ __forceinline__ Moments() {
-#pragma unroll
-        for (int j = 0; j < V; ++j) k[j] = s[j] = q[j] = 0.f;
-    }
-    template <typename T> __device__ __forceinline__ void start(const Vec<T, V>& v) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) k[j] = v.f[j];
-    }
-    template <typename T> __device__ __forceinline__ void add(Vec<T, V> v) {
-        sub_all<V>(v.f, v.f, k);
-        add_all<V>(s, s, v.f);
-        fma_all<V>(q, v.f, v.f, q);
+    Lanes<V> k, s, q;
+    __device__ __forceinline__ Moments() { k = s = q = filled<V>(0.f); }
+    __device__ __forceinline__ void start(const Lanes<V>& v) { k = mul(v, filled<V>(-1.f)); }
+    __device__ __forceinline__ void add(const Lanes<V>& v) {
+        const Lanes<V> e = linf::add(v, k);
+        s = linf::add(s, e);
+        q = fma(e, e, q);
     }
     // (mean, M2) of `count` rows into red: one pair for each channel, or for the vector where it lies in one group
-    __device__ __forceinline__ void put(float2* red, const NormPlan& p, int rt, int cv, int count) {
+    __device__ __forceinline__ void put(float2* red, const NormPlan& p, int rt, int cv, int count) const {
         const float inv = count > 0 ? 1.f / (float)count : 0.f;
+        float m[V], m2[V], first[V];
+        s.get(m);
+        q.get(m2);
+        k.get(first);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            q[j] = fmaf(-s[j] * inv, s[j], q[j]);
-            s[j] = fmaf(s[j], inv, k[j]);
+            m2[j] = fmaf(-m[j] * inv, m[j], m2[j]);
+            m[j] = fmaf(m[j], inv, -first[j]);
         }
         if (p.same) {
-            float m = s[0], t = q[0];
+            float all = m[0], t = m2[0];
 #pragma unroll
-            for (int j = 1; j < V; ++j) { m += s[j]; t += q[j]; }
-            m *= 1.f / V;
+            for (int j = 1; j < V; ++j) { all += m[j]; t += m2[j]; }
+            all *= 1.f / V;
 #pragma unroll
-            for (int j = 0; j < V; ++j) t = fmaf((float)count * (s[j] - m), s[j] - m, t);
-            red[rt * p.tx + cv] = make_float2(m, t);
+            for (int j = 0; j < V; ++j) t = fmaf((float)count * (m[j] - all), m[j] - all, t);
+            red[rt * p.tx + cv] = make_float2(all, t);
         } else {
 #pragma unroll
-            for (int j = 0; j < V; ++j) red[(rt * p.tx + cv) * V + j] = make_float2(s[j], q[j]);
+            for (int j = 0; j < V; ++j) red[(rt * p.tx + cv) * V + j] = make_float2(m[j], m2[j]);
         }
     }
 };
@@ -155,7 +149,6 @@ KeptSpace kept_space(const NormPlan& p, int elem_bytes, int tensors, bool by_vec
     s.bytes = s.mask + (masks ? p.rows * p.tx : 0);
     return s;
 }
-template <typename X> __device__ __forceinline__ X* space_at(uint4* space, int at) { return reinterpret_cast<X*>(reinterpret_cast<char*>(space) + at); }
 
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 3)
@@ -177,9 +170,9 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
     keep_wait();
     if (in) {
         Moments<V> t;
-        if (rt < r1) t.start(load_raw_as<T, V>(own + rt * pitch));
+        if (rt < r1) t.start(load_lanes<T, V>(own + rt * pitch));
 #pragma unroll 4
-        for (int r = rt + p.rt; r < r1; r += p.rt) t.add(load_raw_as<T, V>(own + r * pitch));
+        for (int r = rt + p.rt; r < r1; r += p.rt) t.add(load_lanes<T, V>(own + r * pitch));
         t.put(red, p, rt, cv, rows_of(rows, rt, p));
     }
     join_moments<V>(red, d, p, b, rows, [&](int g, float mu, float m2) {
@@ -203,33 +196,26 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
 
 // ---- forward, two passes ----------------------------------------------------------------------------------------------
 
-constexpr int kSumRows = 8;               // rows of a thread that are on their way at a time
+constexpr int kRing = 8, kBackRing = 4;    // rows that are on their way at a time
 
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3)
+__global__ void __launch_bounds__(kNormThreads, 4)
 norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __restrict__ part) {
-    extern __shared__ float2 red2[];                            // [rt][tx] or [rt][tx * V]
+    extern __shared__ uint4 space[];                            // the ring, then [rt][tx] or [rt][tx * V]
+    float2* red = space_at<float2>(space, norm_ring_bytes<T, V, 1, kRing>());
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const int r0 = split * p.rows, rows = min(p.rows, d.L - r0);
     if (rt < p.rt && cv < b.nvec) {
-        const T* at = x + ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+        const T* const at[1] = {x + ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V};
         Moments<V> t;
-        for (int r = rt; r < rows; r += kSumRows * p.rt) {
-            Raw<T, V> v[kSumRows];
-#pragma unroll
-            for (int k = 0; k < kSumRows; ++k)
-                if (r + k * p.rt < rows) v[k] = load_raw<T, V>(at + (size_t)(r + k * p.rt) * d.C);
-            if (r == rt) t.start(as_vec<T, V>(v[0]));
-#pragma unroll
-            for (int k = 0; k < kSumRows; ++k)
-                if (r + k * p.rt < rows) t.add(as_vec<T, V>(v[k]));
-        }
-        t.put(red2, p, rt, cv, rows_of(rows, rt, p));
+        if (rt < rows) t.start(load_lanes<T, V>(at[0] + (size_t)rt * d.C));
+        norm_stream<T, V, 1, kRing>(space, at, rt, rows, p.rt, d.C, [&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); });
+        t.put(red, p, rt, cv, rows_of(rows, rt, p));
     }
     const double count = (double)rows * (p.pieces == 1 ? d.Cg : b.nvec * V);
-    join_moments<V>(red2, d, p, b, rows, [&](int g, float mu, float m2) {
+    join_moments<V>(red, d, p, b, rows, [&](int g, float mu, float m2) {
         part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_double2(count * mu, m2 + count * mu * mu);
     });
 }
@@ -246,13 +232,12 @@ __device__ __forceinline__ double2 add_parts(const double2* part, const NormDims
     return make_double2(warp_sum(a) * d.inv_m, warp_sum(e) * d.inv_m);
 }
 
-constexpr int kApplyRows = 4;
-
 template <typename T, int V>
-__global__ void __launch_bounds__(kNormThreads, 3)
+__global__ void __launch_bounds__(kNormThreads, 4)
 norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double2* __restrict__ part, NormDims d, NormPlan p, double eps, int act,
                   Drop drop, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
-    __shared__ float2 stat[kNormMaxGroups];
+    extern __shared__ uint4 space[];                            // the ring, then the groups' mean and 1 / deviation
+    float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 1, kRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
@@ -273,56 +258,58 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
     Column<V> col;
     load_column<V>(col, stat, gamma, beta, d, p, b, cv);
     const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-    const int r1 = min(d.L, (split + 1) * p.rows);
-    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-    for (int r = split * p.rows + rt; r < r1; r += kApplyRows * p.rt) {
-        Raw<T, V> v[kApplyRows];
-#pragma unroll
-        for (int k = 0; k < kApplyRows; ++k)
-            if (r + k * p.rt < r1) v[k] = load_once<T, V>(x + at + (size_t)(r + k * p.rt) * d.C);
-#pragma unroll
-        for (int k = 0; k < kApplyRows; ++k)
-            if (r + k * p.rt < r1) write_vector<T, V>(v[k], col, act, drop, key, at + (size_t)(r + k * p.rt) * d.C, y);
-    }
+    const int r0 = split * p.rows;
+    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const T* const from[1] = {x + at};
+    norm_stream<T, V, 1, kRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<T, V>(&v)[1]) {
+        write_vector<T, V>(v[0], col, act, drop, key, at + (size_t)r * d.C, y);
+    });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
 
-// What a thread's column needs for u, and for dx = a du + ra + (x - m) rb.
-template <int V> struct BackColumn { float m[V], a[V], o[V], r[V]; };
+// What a thread's column needs for u = (x + m) a + o, and for dx = a du + ra + (x + m) rb; m as above.
+template <int V> struct BackColumn {
+    Lanes<V> m, a, o;
+    float r[V];
+};
 template <int V>
 __device__ __forceinline__ void load_back_column(BackColumn<V>& k, const float* mean, const float* rstd, const Param& gamma, const Param& beta,
                                                  const NormDims& d, const NormPlan& p, const NormBlock& b, int n, int cv) {
     int g[V];
     groups_of<V>(d, p, cv * V, g);
-    load_params<V>(gamma, b.c0 + cv * V, k.a);
-    load_params<V>(beta, b.c0 + cv * V, k.o);
+    float m[V], a[V], o[V];
+    load_params<V>(gamma, b.c0 + cv * V, a);
+    load_params<V>(beta, b.c0 + cv * V, o);
     mean += (size_t)n * d.G + b.g0;
     rstd += (size_t)n * d.G + b.g0;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        k.m[j] = __ldg(mean + g[j]);
+        m[j] = -__ldg(mean + g[j]);
         k.r[j] = __ldg(rstd + g[j]);
-        k.a[j] *= k.r[j];
+        a[j] *= k.r[j];
     }
+    k.m.set(m);
+    k.a.set(a);
+    k.o.set(o);
 }
 
 // du of V elements (the gradient at u) from that at y, which has been dropped already, and x - mean
 template <typename T, int V>
-__device__ __forceinline__ void back_du(const Raw<T, V>& xv, const BackColumn<V>& k, int act, float (&du)[V], float (&e)[V]) {
-    unpack<T, V>(xv, e);
-    sub_all<V>(e, e, k.m);
-    if (act == LINF_ACT_IDENTITY) return;
-    float s[V];
-    fma_all<V>(s, e, k.a, k.o);
-    slope_all<sizeof(T) == 4, V>(s, act);
-    mul_all<V>(du, du, s);
+__device__ __forceinline__ void back_du(const Raw<T, V>& xv, const BackColumn<V>& k, int act, Lanes<V>& du, Lanes<V>& e) {
+    e = add(lanes_of<T, V>(xv), k.m);
+    if (act != LINF_ACT_IDENTITY) du = mul(du, slope<sizeof(T) == 4, V>(fma(e, k.a, k.o), act));
 }
 template <typename T, int V>
 __device__ __forceinline__ void back_du(const Raw<T, V>& xv, const Raw<T, V>& gv, const BackColumn<V>& k, int act, const Drop& drop, const DropKey& key,
-                                        size_t i, float (&du)[V], float (&e)[V]) {
-    unpack<T, V>(gv, du);
-    if (drop.on) drop_apply<V>(drop, key, i, du);
+                                        size_t i, Lanes<V>& du, Lanes<V>& e) {
+    du = lanes_of<T, V>(gv);
+    if (drop.on) {
+        float f[V];
+        du.get(f);
+        drop_apply<V>(drop, key, i, f);
+        du.set(f);
+    }
     back_du<T, V>(xv, k, act, du, e);
 }
 
@@ -359,26 +346,26 @@ __device__ __forceinline__ void fold_rows(float2* red, int width, int rt) {
     });
 }
 
-// dx of V elements from du and x - mean
-template <typename T, int V>
-__device__ __forceinline__ void write_dx(const float (&du)[V], const float (&e)[V], const BackColumn<V>& k, const float (&ra)[V], const float (&rb)[V],
-                                         T* to) {
-    float f[V];
-    fma_all<V>(f, k.a, du, ra);
-    fma_all<V>(f, e, rb, f);
-    store_once<T, V>(to, pack<T, V>(f));
-}
+// ra, rb of a thread's column
+template <int V> struct Means { Lanes<V> ra, rb; };
 template <int V>
-__device__ __forceinline__ void load_means(const float2* stat, const NormDims& d, const NormPlan& p, int cv, const BackColumn<V>& k, float (&ra)[V],
-                                           float (&rb)[V]) {
+__device__ __forceinline__ void load_means(const float2* stat, const NormDims& d, const NormPlan& p, int cv, const BackColumn<V>& k, Means<V>& m) {
     int g[V];
     groups_of<V>(d, p, cv * V, g);
+    float ra[V], rb[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const float2 s = stat[g[j]];
         ra[j] = -k.r[j] * s.x;
         rb[j] = -k.r[j] * k.r[j] * s.y;
     }
+    m.ra.set(ra);
+    m.rb.set(rb);
+}
+// dx of V elements from du and x - mean
+template <typename T, int V>
+__device__ __forceinline__ void write_dx(const Lanes<V>& du, const Lanes<V>& e, const BackColumn<V>& k, const Means<V>& m, T* to) {
+    store_once<T, V>(to, raw_of<T, V>(fma(e, m.rb, fma(k.a, du, m.ra))));
 }
 
 template <typename T, int V>
@@ -411,25 +398,25 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
         }
         BackColumn<V> col;
         if (in) load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
-        float sa[V], sb[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.f;
+        Lanes<V> sum_a = filled<V>(0.f), sum_b = sum_a;
         keep_wait();
 #pragma unroll 2
         for (int r = rt; r < r1; r += p.rt) {
-            float du[V], e[V];
-            unpack<T, V>(load_raw<T, V>(own_g + r * pitch), du);
+            Lanes<V> du = load_lanes<T, V>(own_g + r * pitch), e;
             if (drop.on) {
                 const unsigned mask = drop_mask<V>(drop, key, at + (size_t)r * d.C);
                 if (sizeof(T) == 2) kept[r * p.tx + cv] = (unsigned char)mask;
                 drop_masked<V>(drop, mask, du);
             }
             back_du<T, V>(load_raw<T, V>(own + r * pitch), col, act, du, e);
-            add_all<V>(sa, sa, du);
-            fma_all<V>(sb, du, e, sb);
+            sum_a = add(sum_a, du);
+            sum_b = fma(du, e, sum_b);
             // fp32: du takes the place of dy; 16-bit types would round it, and work it out again
-            if (sizeof(T) == 4) *reinterpret_cast<Raw<T, V>*>(own_g + r * pitch) = pack<T, V>(du);
+            if (sizeof(T) == 4) *reinterpret_cast<Raw<T, V>*>(own_g + r * pitch) = raw_of<T, V>(du);
         }
+        float sa[V], sb[V];
+        sum_a.get(sa);
+        sum_b.get(sb);
         if (in) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -451,23 +438,18 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
         group_sums(red, gamma, d, p, b, [&](int g, double2 v) { stat[g] = make_float2((float)(v.x * d.inv_m), (float)(v.y * d.inv_m)); });
         __syncthreads();
         if (in) {
-            float ra[V], rb[V];
-            load_means<V>(stat, d, p, cv, col, ra, rb);
+            Means<V> means;
+            load_means<V>(stat, d, p, cv, col, means);
 #pragma unroll 2
             for (int r = rt; r < r1; r += p.rt) {
-                const size_t i = at + (size_t)r * d.C;
-                float du[V], e[V];
+                Lanes<V> du = load_lanes<T, V>(own_g + r * pitch), e;
                 if (sizeof(T) == 4) {
-                    unpack<T, V>(load_raw<T, V>(own + r * pitch), e);
-                    unpack<T, V>(load_raw<T, V>(own_g + r * pitch), du);
-#pragma unroll
-                    for (int j = 0; j < V; ++j) e[j] -= col.m[j];
+                    e = add(load_lanes<T, V>(own + r * pitch), col.m);
                 } else {
-                    unpack<T, V>(load_raw<T, V>(own_g + r * pitch), du);
                     if (drop.on) drop_masked<V>(drop, kept[r * p.tx + cv], du);
                     back_du<T, V>(load_raw<T, V>(own + r * pitch), col, act, du, e);
                 }
-                write_dx<T, V>(du, e, col, ra, rb, dx + i);
+                write_dx<T, V>(du, e, col, means, dx + at + (size_t)r * d.C);
             }
         }
         __syncthreads();
@@ -482,45 +464,37 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
     for (int c = threadIdx.x; c < b.nvec * V; c += blockDim.x) by_channel[(size_t)chunk * d.C + b.c0 + c] = red[c];
 }
 
-constexpr int kBackRows = 2;
-
 template <typename T, int V>
 __global__ void __launch_bounds__(kNormThreads, 2)
 norm_back_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param gamma, Param beta, const float* __restrict__ mean,
                       const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop, float2* __restrict__ by_channel,
                       double2* __restrict__ by_group) {
-    extern __shared__ float2 redf[];                            // [rt][tx * V]
+    extern __shared__ uint4 space[];                            // the ring, then [rt][tx * V]
+    float2* redf = space_at<float2>(space, norm_ring_bytes<T, V, 2, kBackRing>());
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const int width = p.tx * V;
     if (rt < p.rt) {
-        float sa[V], sb[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) sa[j] = sb[j] = 0.f;
+        Lanes<V> sum_a = filled<V>(0.f), sum_b = sum_a;
+        BackColumn<V> col;
         if (cv < b.nvec) {
-            BackColumn<V> col;
             load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
             const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-            const int r1 = min(d.L, (split + 1) * p.rows);
-            const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-            for (int r = split * p.rows + rt; r < r1; r += kBackRows * p.rt) {
-                Raw<T, V> v[kBackRows], g[kBackRows];
-#pragma unroll
-                for (int k = 0; k < kBackRows; ++k)
-                    if (r + k * p.rt < r1) {
-                        v[k] = load_raw<T, V>(x + at + (size_t)(r + k * p.rt) * d.C);
-                        g[k] = load_raw<T, V>(dy + at + (size_t)(r + k * p.rt) * d.C);
-                    }
-#pragma unroll
-                for (int k = 0; k < kBackRows; ++k)
-                    if (r + k * p.rt < r1) {
-                        float du[V], e[V];
-                        back_du<T, V>(v[k], g[k], col, act, drop, key, at + (size_t)(r + k * p.rt) * d.C, du, e);
-                        add_all<V>(sa, sa, du);
-                        fma_all<V>(sb, du, e, sb);
-                    }
-            }
+            const int r0 = split * p.rows;
+            const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+            const T* const from[2] = {x + at, dy + at};
+            norm_stream<T, V, 2, kBackRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<T, V>(&v)[2]) {
+                Lanes<V> du, e;
+                back_du<T, V>(v[0], v[1], col, act, drop, key, at + (size_t)r * d.C, du, e);
+                sum_a = add(sum_a, du);
+                sum_b = fma(du, e, sum_b);
+            });
+        }
+        float sa[V], sb[V];
+        sum_a.get(sa);
+        sum_b.get(sb);
+        if (cv < b.nvec) {
 #pragma unroll
             for (int j = 0; j < V; ++j) sb[j] *= col.r[j];
         }
@@ -540,7 +514,8 @@ __global__ void __launch_bounds__(kNormThreads, 2)
 norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param gamma, Param beta, const float* __restrict__ mean,
                        const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop, const double2* __restrict__ by_group,
                        T* __restrict__ dx) {
-    __shared__ float2 stat[kNormMaxGroups];
+    extern __shared__ uint4 space[];                            // the ring, then the groups' two means
+    float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 2, kBackRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
@@ -552,53 +527,40 @@ norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
     if (rt >= p.rt || cv >= b.nvec) return;
     BackColumn<V> col;
     load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
-    float ra[V], rb[V];
-    load_means<V>(stat, d, p, cv, col, ra, rb);
+    Means<V> means;
+    load_means<V>(stat, d, p, cv, col, means);
     const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-    const int r1 = min(d.L, (split + 1) * p.rows);
-    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-    for (int r = split * p.rows + rt; r < r1; r += kBackRows * p.rt) {
-        Raw<T, V> v[kBackRows], g[kBackRows];
-#pragma unroll
-        for (int k = 0; k < kBackRows; ++k)
-            if (r + k * p.rt < r1) {
-                v[k] = load_once<T, V>(x + at + (size_t)(r + k * p.rt) * d.C);
-                g[k] = load_once<T, V>(dy + at + (size_t)(r + k * p.rt) * d.C);
-            }
-#pragma unroll
-        for (int k = 0; k < kBackRows; ++k)
-            if (r + k * p.rt < r1) {
-                const size_t i = at + (size_t)(r + k * p.rt) * d.C;
-                float du[V], e[V];
-                back_du<T, V>(v[k], g[k], col, act, drop, key, i, du, e);
-                write_dx<T, V>(du, e, col, ra, rb, dx + i);
-            }
-    }
+    const int r0 = split * p.rows;
+    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const T* const from[2] = {x + at, dy + at};
+    norm_stream<T, V, 2, kBackRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<T, V>(&v)[2]) {
+        const size_t i = at + (size_t)r * d.C;
+        Lanes<V> du, e;
+        back_du<T, V>(v[0], v[1], col, act, drop, key, i, du, e);
+        write_dx<T, V>(du, e, col, means, dx + i);
+    });
 }
 
-// dgamma, dbeta: the per-channel sums of all samples and row ranges, in 64 bits, 32 channels to a CTA
-__global__ void __launch_bounds__(1024)
+// dgamma, dbeta: the rows of per-channel sums in 64 bits, 8 channels to a CTA (a row's piece is two sectors) and 32 rows at a time
+__global__ void __launch_bounds__(256)
 norm_params_kernel(const float2* __restrict__ by_channel, long long count, int C, void* __restrict__ dgamma, void* __restrict__ dbeta, int ptype) {
-    __shared__ double red[2][32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 32 + lane;
+    __shared__ double2 red[32][8];
+    const int col = threadIdx.x & 7, lane = threadIdx.x >> 3, c = blockIdx.x * 8 + col;
     double a = 0.0, e = 0.0;
-    if (c < C)
-        for (long long k = warp; k < count; k += 32) {
+    if (c < C) {
+#pragma unroll 4
+        for (long long k = lane; k < count; k += 32) {
             const float2 v = __ldg(by_channel + k * C + c);
             a += v.x;
             e += v.y;
         }
-    red[0][warp][lane] = a;
-    red[1][warp][lane] = e;
-    __syncthreads();
-    a = warp_sum(red[0][lane][warp]);
-    e = warp_sum(red[1][lane][warp]);
-    const int out = blockIdx.x * 32 + warp;
-    if (lane == 0 && out < C) {
-        if (dbeta != nullptr) store_param(dbeta, out, ptype, (float)a);
-        if (dgamma != nullptr) store_param(dgamma, out, ptype, (float)e);
     }
+    red[lane][col] = make_double2(a, e);
+    __syncthreads();
+    if (threadIdx.x >= 8 || c >= C) return;
+    for (int k = 1; k < 32; ++k) { a += red[k][col].x; e += red[k][col].y; }
+    if (dbeta != nullptr) store_param(dbeta, c, ptype, (float)a);
+    if (dgamma != nullptr) store_param(dgamma, c, ptype, (float)e);
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------
@@ -609,6 +571,8 @@ NormKind backward_kind(int type) { return {type == LINF_F32 ? 4 : 2, 2, true}; }
 // The workspace of a call: forward, two passes: the parts; backward: the channels' sums, and the parts of two passes.
 size_t parts_bytes(const NormDims& d, const NormPlan& p) { return p.kept ? 0 : sizeof(double2) * (size_t)d.N * p.splits * d.G * p.pieces; }
 long long channel_rows(const NormPlan& p) { return (long long)p.chunks * p.splits; }
+constexpr int kDenseCtas = 8, kDenseBackCtas = 3;      // of each SM
+size_t dense_workspace(const NormDims& d, const DensePlan& p) { return sizeof(float2) * (size_t)p.chunks * p.subs * d.C; }
 size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
     return parts_bytes(d, p) + (back ? sizeof(float2) * (size_t)channel_rows(p) * d.C : 0);
 }
@@ -622,8 +586,11 @@ int forward(const T* x, const NormGiven& given, const NormDims& d, const NormPla
     }
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     double2* part = static_cast<double2*>(ws);
-    norm_sums_kernel<T, V><<<grid, kNormThreads, sizeof(float2) * p.rt * p.tx * (p.same ? 1 : V), st>>>(x, d, p, part);
-    norm_apply_kernel<T, V><<<grid, kNormThreads, 0, st>>>(x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
+    const size_t ring = norm_ring_bytes<T, V, 1, kRing>();
+    const size_t one = ring + sizeof(float2) * p.rt * p.tx * (p.same ? 1 : V), two = ring + sizeof(float2) * p.groups;
+    if (!allow_shared(norm_sums_kernel<T, V>, one) || !allow_shared(norm_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
+    norm_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(x, d, p, part);
+    norm_apply_kernel<T, V><<<grid, kNormThreads, two, st>>>(x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
     return launch_status(2);
 }
 
@@ -639,10 +606,12 @@ int backward(const T* dy, const T* x, const NormGiven& given, int ptype, const f
         if (rc) return rc;
     } else {
         const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
-        norm_back_sums_kernel<T, V><<<grid, kNormThreads, sizeof(float2) * p.rt * p.tx * V, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act,
-                                                                                                     drop, by_channel, by_group);
+        const size_t ring = norm_ring_bytes<T, V, 2, kBackRing>();
+        const size_t one = ring + sizeof(float2) * p.rt * p.tx * V, two = ring + sizeof(float2) * p.groups;
+        if (!allow_shared(norm_back_sums_kernel<T, V>, one) || !allow_shared(norm_back_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
+        norm_back_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_channel, by_group);
         if (dx != nullptr)
-            norm_back_apply_kernel<T, V><<<grid, kNormThreads, 0, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_group, dx);
+            norm_back_apply_kernel<T, V><<<grid, kNormThreads, two, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_group, dx);
         if (launch_status(dx != nullptr ? 2 : 1)) return LINF_ERR_LAUNCH;
     }
     return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, channel_rows(p), d.C, dgamma, dbeta, ptype, st) : LINF_OK;
@@ -671,7 +640,7 @@ bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g) {
 }
 
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st) {
-    norm_params_kernel<<<(C + 31) / 32, 1024, 0, st>>>(by_channel, count, C, dgamma, dbeta, ptype);
+    norm_params_kernel<<<(C + 7) / 8, 256, 0, st>>>(by_channel, count, C, dgamma, dbeta, ptype);
     return launch_status();
 }
 
@@ -681,8 +650,10 @@ size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back) {
     for (int k = 0; k < 2; ++k) {
         NormDims d;
         NormPlan p;
+        DensePlan dp;
         if (norm_make(N, C, G, L, back ? backward_kind(type) : forward_kind(type), k == 0, &d, &p) != LINF_OK) return 0;
-        const size_t need = workspace(d, p, back);
+        const bool dense = dense_plan(d, type == LINF_F32 ? 4 : 2, k == 0, sm_count() * (back ? kDenseBackCtas : kDenseCtas), &dp);
+        const size_t need = dense ? (back ? dense_workspace(d, dp) : 0) : workspace(d, p, back);
         if (need > most) most = need;
     }
     return (most + 255) / 256 * 256;
@@ -711,10 +682,13 @@ int group_norm_forward(const void* x, const void* gamma, const void* beta, int N
     if (!make_drop(rate, rng, &drop)) return LINF_ERR_RATE;
     const int rc = norm_make(N, C, G, L, forward_kind(type), aligned16(x) && aligned16(y), &d, &p);
     if (rc) return rc;
-    const size_t need = workspace(d, p, false);
+    DensePlan dp;
+    const bool dense = dense_plan(d, type == LINF_F32 ? 4 : 2, aligned16(x) && aligned16(y), sm_count() * kDenseCtas, &dp);
+    const size_t need = dense ? 0 : workspace(d, p, false);
     if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need)) return LINF_ERR_WORKSPACE;
     NormGiven given;
     if (!norm_given(gamma, beta, ptype, &given)) return LINF_ERR_LAUNCH;
+    if (dense) return dense_norm_forward(x, given, d, dp, type, eps, act, drop, y, mean, rstd, st);
 #define LINF_CALL(T, V) forward<T, V>(static_cast<const T*>(x), given, d, p, eps, act, drop, static_cast<T*>(y), mean, rstd, ws, st)
     LINF_BY_VECTOR(LINF_CALL, LINF_CALL)
 #undef LINF_CALL
@@ -729,9 +703,17 @@ int group_norm_backward(const void* dy, const void* x, const void* gamma, const 
     if (!make_drop(rate, rng, &drop)) return LINF_ERR_RATE;
     const int rc = norm_make(N, C, G, L, backward_kind(type), aligned16(x) && aligned16(dy) && aligned16(dx), &d, &p);
     if (rc) return rc;
-    if (ws == nullptr || !aligned16(ws) || ws_bytes < workspace(d, p, true)) return LINF_ERR_WORKSPACE;
+    DensePlan dp;
+    const bool dense = dense_plan(d, type == LINF_F32 ? 4 : 2, aligned16(x) && aligned16(dy) && aligned16(dx), sm_count() * kDenseBackCtas, &dp);
+    if (ws == nullptr || !aligned16(ws) || ws_bytes < (dense ? dense_workspace(d, dp) : workspace(d, p, true))) return LINF_ERR_WORKSPACE;
     NormGiven given;
     if (!norm_given(gamma, beta, ptype, &given)) return LINF_ERR_LAUNCH;
+    if (dense) {
+        float2* by_channel = static_cast<float2*>(ws);
+        const int done = dense_norm_backward(dy, x, given, mean, rstd, d, dp, type, act, drop, dx, by_channel, st);
+        if (done || (dgamma == nullptr && dbeta == nullptr)) return done;
+        return norm_params(by_channel, (long long)dp.chunks * dp.subs, C, dgamma, dbeta, ptype, st);
+    }
 #define LINF_CALL(T, V)                                                                                                                   \
     backward<T, V>(static_cast<const T*>(dy), static_cast<const T*>(x), given, ptype, mean, rstd, d, p, act, drop, static_cast<T*>(dx), \
                    dgamma, dbeta, ws, st)

@@ -89,7 +89,7 @@ constexpr int kNormThreads = 256;
 constexpr int kNormMaxGroups = kNormThreads * 8;
 constexpr int kNormKeepBytes = 64 * 1024; // of a CTA, so that an SM has three
 constexpr int kNormSplits = 64;           // row ranges of the two passes: a CTA of the second adds up that many
-constexpr int kNormWaves = 6;             // CTAs of the two passes for each SM
+constexpr int kNormPlaces = 4;            // CTAs of the two passes that an SM has at a time, about
 
 inline int norm_ceil(long long a, long long b) { return (int)((a + b - 1) / b); }
 
@@ -175,12 +175,15 @@ inline void norm_two_passes(const NormDims& d, const NormKind& kind, bool aligne
     p->threads = kNormThreads;
     p->rt = cap / p->tx;
     if (p->rt > d.L) p->rt = d.L;
-    // CTAs for the whole GPU, with at least four rows for each thread
-    const long long ctas = (long long)p->blocks * d.N, want = (long long)sm_count() * kNormWaves;
-    long long s = ctas >= want ? 1 : norm_ceil(want, ctas);
-    const long long by_rows = norm_ceil(d.L, 4LL * p->rt);
-    if (s > by_rows) s = by_rows;
-    if (s > kNormSplits) s = kNormSplits;
+    // as few row ranges as fill the GPU's places for CTAs nearly whole, with at least four rows for each thread
+    const long long ctas = (long long)p->blocks * d.N, places = (long long)sm_count() * kNormPlaces;
+    long long most = norm_ceil(d.L, 4LL * p->rt), s = 1;
+    if (most > kNormSplits) most = kNormSplits;
+    double best = 0.0;
+    for (long long k = 1; k <= most && best < 0.9; ++k) {
+        const double full = (double)(ctas * k) / (double)(norm_ceil(ctas * k, places) * places);
+        if (full > best) { best = full; s = k; }
+    }
     p->rows = norm_ceil(d.L, s);
     p->splits = norm_ceil(d.L, p->rows);
     p->per_cta = 1;
@@ -207,12 +210,25 @@ inline int norm_make(int N, int C, int G, int L, const NormKind& kind, bool alig
     return LINF_OK;
 }
 
+// One position (group_norm_dense.cu): a row of C/G values belongs to a slot of `tpr` threads; a CTA has slots for `groups` groups times `subs`
+// samples, and takes `per` samples.
+struct DensePlan { int V, tpr, threads, groups, subs, blocks, per, chunks; };
+struct NormGiven;
+bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, DensePlan* p);
+int dense_norm_forward(const void* x, const NormGiven& given, const NormDims& d, const DensePlan& p, int type, double eps, int act, const Drop& drop,
+                       void* y, float* mean, float* rstd, cudaStream_t st);
+// by_channel: chunks * subs rows of C
+int dense_norm_backward(const void* dy, const void* x, const NormGiven& given, const float* mean, const float* rstd, const NormDims& d, const DensePlan& p,
+                        int type, int act, const Drop& drop, void* dx, float2* by_channel, cudaStream_t st);
+
 // dgamma and dbeta from `count` rows of per-channel sums (du, du h); either may be null (group_norm.cu)
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st);
 
 // gamma and beta, or what stands for them where they are null, on the current device; false if CUDA refused (group_norm.cu)
 struct NormGiven { Param gamma, beta; };
 bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g);
+
+template <typename X> __device__ __forceinline__ X* space_at(uint4* space, size_t at) { return reinterpret_cast<X*>(reinterpret_cast<char*>(space) + at); }
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -251,6 +267,79 @@ __device__ __forceinline__ void keep_vector(T* to, const T* from) {
     else *to = *from;
 }
 __device__ __forceinline__ void keep_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+template <int BYTES>
+__device__ __forceinline__ void copy_shared(unsigned to, const void* from) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> load_shared(unsigned at) {
+    Raw<T, V> v;
+    if constexpr (sizeof(T) * V == 16) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    return v;
+}
+
+// The rows r, r + step, ... below r1 of a thread's column in each of N tensors (at[k] points at row 0): body(row, vectors).  S rows are on their way
+// to shared memory at a time, each thread's to places of its own (`ring`: norm_ring_bytes), so that neither registers nor barriers
+// limit how much is read ahead.  Elements of two bytes that no wider copy reaches come through registers.
+template <typename T, int V, int N, int S>
+__host__ __device__ constexpr size_t norm_ring_bytes() { return sizeof(T) * V >= 4 ? (size_t)kNormThreads * sizeof(T) * V * N * S : 0; }
+
+template <typename T, int V, int N, int S, typename Body>
+__device__ __forceinline__ void norm_stream(void* ring, const T* const (&at)[N], int r, int r1, int step, size_t C, Body body) {
+    if constexpr (sizeof(T) * V >= 4) {
+        constexpr int bytes = sizeof(T) * V, place = kNormThreads * bytes;      // [S][N][threads]
+        const unsigned own = (unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * bytes;
+        const T* next[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) next[k] = at[k] + (size_t)r * C;
+        const size_t stride = (size_t)step * C;
+        int ahead = r;
+        auto issue = [&](int s) {
+            if (ahead < r1) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    copy_shared<bytes>(own + (s * N + k) * place, next[k]);
+                    next[k] += stride;
+                }
+            }
+            ahead += step;
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S; ++s) issue(s);
+        auto row = [&](int s) {
+            cp_async_wait<S - 1>();
+            Raw<T, V> v[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = load_shared<T, V>(own + (s * N + k) * place);
+            body(r, v);
+            issue(s);                                           // behind body, which has used what it overwrites
+            r += step;
+        };
+        for (int turns = r < r1 ? ((r1 - r - 1) / step + 1) / S : 0; turns > 0; --turns) {
+#pragma unroll
+            for (int s = 0; s < S; ++s) row(s);
+        }
+#pragma unroll 1
+        for (int s = 0; r < r1; ++s) row(s);
+    } else {
+        constexpr int K = 8 / N;
+        for (; r < r1; r += K * step) {
+            Raw<T, V> v[K][N];
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    if (r + j * step < r1) v[j][k] = load_raw<T, V>(at[k] + (size_t)(r + j * step) * C);
+#pragma unroll
+            for (int j = 0; j < K; ++j)
+                if (r + j * step < r1) body(r + j * step, v[j]);
+        }
+    }
+}
 
 template <typename F>
 bool allow_shared(F kernel, size_t bytes) {

@@ -7,8 +7,9 @@
 //   z- = min(n- s_lo, n- s_hi),  z+ = max(n+ s_lo, n+ s_hi), cut at -+sqrt(M - 1), beyond which no normalised value of M can be.
 // gamma < 0 exchanges the ends.  The activations are monotone, but for silu, which has one minimum.
 //
-// All of it is computed in 64 bits and rounded once: which of two ends a bound takes, and with it a gradient, is decided next to 0.
-// The kernels are bound by HBM all the same (16 bytes of a forward pass stand against some 25 operations in 64 bits, and an SM issues 64 a clock).
+// Sums, and all of the backward pass, are computed in 64 bits: which of two ends a bound takes, and with it a gradient, is decided next to
+// 0.  The elements of the forward pass, whose values do not jump there, are fp32, with the means in two parts, so that no bound is off by more
+// than a few roundings of its own terms.  Forward passes are bound by HBM, backward passes by the 64-bit units.
 #include "group_norm.cuh"
 
 namespace linf {
@@ -67,17 +68,6 @@ __device__ __forceinline__ Sides silu_sides(double v0, double v1) {
     return s;
 }
 
-// bounds of f over [v0, v1]
-__device__ __forceinline__ void bound_act(double v0, double v1, int act, float& y0, float& y1) {
-    y0 = activate((float)v0, act);
-    y1 = activate((float)v1, act);
-    if (act == LINF_ACT_SILU && v0 == v0 && v1 == v1) {
-        const Sides s = silu_sides(v0, v1);
-        const float low = s.inside ? activate(kSiluArg, act) : s.top_is_v1 ? y0 : y1, high = s.top_is_v1 ? y1 : y0;
-        y0 = fminf(low, high);                      // one rounding of a flat stretch may turn two values around
-        y1 = high;
-    }
-}
 // gradients (g0, g1) at the bounds -> at v0 and v1
 __device__ __forceinline__ void bound_slope(double v0, double v1, int act, float g0, float g1, double& d0, double& d1) {
     if (act == LINF_ACT_SILU) {
@@ -148,22 +138,63 @@ __device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<fl
         const double a = l[j], e = u[j];
         s[j].a += a;
         s[j].b += e;
-        s[j].c = fma(a + e, a + e, s[j].c);
-        s[j].d = fma(e - a, e - a, s[j].d);
+        s[j].c = ::fma(a + e, a + e, s[j].c);
+        s[j].d = ::fma(e - a, e - a, s[j].d);
     }
 }
 
+// What the forward pass needs of a box, in fp32; the means as a sum of two.
+struct Ends32 { float ml, ml2, mu, mu2, s_lo, s_hi; };
+__device__ __forceinline__ Ends32 make_ends32(const Sum4& s, const NormDims& d, double eps) {
+    const Box b = make_box(s, d, eps);
+    Ends32 e;
+    e.ml = (float)b.mean_l;
+    e.ml2 = (float)(b.mean_l - e.ml);
+    e.mu = (float)b.mean_u;
+    e.mu2 = (float)(b.mean_u - e.mu);
+    e.s_lo = (float)b.s_lo;
+    e.s_hi = (float)b.s_hi;
+    return e;
+}
+// ... and of the channels of a thread's column
+template <int V> struct BoundColumn { Ends32 e[V]; float w[V], o[V], inv_m, cut; };
 template <int V>
-__device__ __forceinline__ void write_bounds(const Raw<float, V>& lv, const Raw<float, V>& uv, const Box* box, const float (&w)[V], const float (&o)[V],
-                                             const NormDims& d, const NormPlan& p, int c, size_t i, int act, float* out_l, float* out_u) {
+__device__ __forceinline__ void load_column(BoundColumn<V>& k, const Ends32* ends, const Param& gamma, const Param& beta, const NormDims& d,
+                                            const NormPlan& p, const NormBlock& b, int c) {
+    int g[V];
+    groups_of<V>(d, p, c, g);
+    load_params<V>(gamma, b.c0 + c, k.w);
+    load_params<V>(beta, b.c0 + c, k.o);
+#pragma unroll
+    for (int j = 0; j < V; ++j) k.e[j] = ends[g[j]];
+    k.inv_m = (float)d.inv_m;
+    k.cut = sqrtf((float)((double)d.L * d.Cg - 1.0));
+}
+
+template <int V>
+__device__ __forceinline__ void write_bounds(const Raw<float, V>& lv, const Raw<float, V>& uv, const BoundColumn<V>& k, size_t i, int act, float* out_l,
+                                             float* out_u) {
     float l[V], u[V];
     unpack<float, V>(lv, l);
     unpack<float, V>(uv, u);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const Ends e = make_ends(box[group_of(d, p, c + j)], l[j], u[j], d.inv_m);
-        const bool turned = w[j] < 0.f;
-        bound_act(fma(turned ? e.z1 : e.z0, (double)w[j], (double)o[j]), fma(turned ? e.z0 : e.z1, (double)w[j], (double)o[j]), act, l[j], u[j]);
+        const Ends32& e = k.e[j];
+        const float own = (u[j] - l[j]) * k.inv_m;
+        const float n0 = ((l[j] - e.mu) - e.mu2) + own, n1 = ((u[j] - e.ml) - e.ml2) - own;
+        float z0 = n0 * (n0 >= 0.f ? e.s_lo : e.s_hi), z1 = n1 * (n1 >= 0.f ? e.s_hi : e.s_lo);
+        z0 = z0 <= -k.cut ? -k.cut : z0;                        // a NaN stays
+        z1 = z1 >= k.cut ? k.cut : z1;
+        const bool turned = k.w[j] < 0.f;
+        const float v0 = fmaf(turned ? z1 : z0, k.w[j], k.o[j]), v1 = fmaf(turned ? z0 : z1, k.w[j], k.o[j]);
+        float y0 = activate(v0, act), y1 = activate(v1, act);
+        if (act == LINF_ACT_SILU) {
+            const float low = v0 < kSiluArg && v1 > kSiluArg ? activate(kSiluArg, act) : y0, high = y0 > y1 ? y0 : y1;
+            y0 = y1 < low ? y1 : low;
+            y1 = high;
+        }
+        l[j] = y0;
+        u[j] = y1;
     }
     store_once<float, V>(out_l + i, pack<float, V>(l));
     store_once<float, V>(out_u + i, pack<float, V>(u));
@@ -190,7 +221,7 @@ bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upp
     const BoundSpace at_ = bound_space<V>(p, 2);
     float* data = reinterpret_cast<float*>(space);
     Sum4* red = reinterpret_cast<Sum4*>(reinterpret_cast<char*>(space) + at_.red);
-    Box* box = reinterpret_cast<Box*>(reinterpret_cast<char*>(space) + at_.box);
+    Ends32* ends = reinterpret_cast<Ends32*>(reinterpret_cast<char*>(space) + at_.box);
     const int n = p.by_blocks(blockIdx.x);
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
@@ -214,24 +245,26 @@ bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upp
     }
     __syncthreads();
     group_sums(red, d, p, b, [&](int g, const Sum4& s) {
-        box[g] = make_box(s, d, eps);
+        ends[g] = make_ends32(s, d, eps);
         if (sums != nullptr) sums[(size_t)n * d.G + b.g0 + g] = s;
     });
     __syncthreads();
     if (in) {
-        float w[V], o[V];
-        load_params<V>(gamma, b.c0 + c, w);
-        load_params<V>(beta, b.c0 + c, o);
+        BoundColumn<V> col;
+        load_column<V>(col, ends, gamma, beta, d, p, b, c);
+#pragma unroll 2
         for (int r = rt; r < r1; r += p.rt)
-            write_bounds<V>(load_raw<float, V>(own_l + r * pitch), load_raw<float, V>(own_u + r * pitch), box, w, o, d, p, c, at + (size_t)r * d.C, act,
-                            out_l, out_u);
+            write_bounds<V>(load_raw<float, V>(own_l + r * pitch), load_raw<float, V>(own_u + r * pitch), col, at + (size_t)r * d.C, act, out_l, out_u);
     }
 }
 
+constexpr int kBoundRing = 4;              // rows that are on their way at a time
+
 template <int V>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, 3)
 bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upper, NormDims d, NormPlan p, Sum4* __restrict__ part) {
-    extern __shared__ Sum4 red4[];
+    extern __shared__ uint4 space[];                            // the ring, then [rt][tx] or [rt][tx * V]
+    Sum4* red4 = space_at<Sum4>(space, norm_ring_bytes<float, V, 2, kBoundRing>());
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
@@ -239,11 +272,11 @@ bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upp
         Sum4 s[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
-        const int r1 = min(d.L, (split + 1) * p.rows);
-        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-#pragma unroll 4
-        for (int r = split * p.rows + rt; r < r1; r += p.rt)
-            sum_vector<V>(load_raw<float, V>(lower + at + (size_t)r * d.C), load_raw<float, V>(upper + at + (size_t)r * d.C), s);
+        const int r0 = split * p.rows;
+        const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+        const float* const from[2] = {lower + at, upper + at};
+        norm_stream<float, V, 2, kBoundRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C,
+                                             [&](int, const Raw<float, V>(&v)[2]) { sum_vector<V>(v[0], v[1], s); });
         put_sums<V>(red4, p, rt, cv, s);
     }
     __syncthreads();
@@ -261,32 +294,31 @@ __device__ __forceinline__ Sum4 all_parts(const Sum4* part, const NormDims& d, c
 }
 
 template <int V>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, 3)
 bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ upper, Param gamma, Param beta, const Sum4* __restrict__ part, NormDims d,
                    NormPlan p, double eps, int act, float* __restrict__ out_l, float* __restrict__ out_u, Sum4* __restrict__ sums) {
-    extern __shared__ Box box1[];                               // [groups of the block]
+    extern __shared__ uint4 space[];                            // the ring, then what the groups share
+    Ends32* ends = space_at<Ends32>(space, norm_ring_bytes<float, V, 2, kBoundRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(part, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
-            box1[g] = make_box(t, d, eps);
+            ends[g] = make_ends32(t, d, eps);
             if (split == 0 && b.piece == 0 && sums != nullptr) sums[(size_t)n * d.G + b.g0 + g] = t;
         }
     }
     __syncthreads();
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     if (rt >= p.rt || cv >= b.nvec) return;
-    float w[V], o[V];
-    load_params<V>(gamma, b.c0 + c, w);
-    load_params<V>(beta, b.c0 + c, o);
-    const int r1 = min(d.L, (split + 1) * p.rows);
-    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
-#pragma unroll 2
-    for (int r = split * p.rows + rt; r < r1; r += p.rt) {
-        const size_t i = at + (size_t)r * d.C;
-        write_bounds<V>(load_raw<float, V>(lower + i), load_raw<float, V>(upper + i), box1, w, o, d, p, c, i, act, out_l, out_u);
-    }
+    BoundColumn<V> col;
+    load_column<V>(col, ends, gamma, beta, d, p, b, cv * V);
+    const int r0 = split * p.rows;
+    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const float* const from[2] = {lower + at, upper + at};
+    norm_stream<float, V, 2, kBoundRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<float, V>(&v)[2]) {
+        write_bounds<V>(v[0], v[1], col, at + (size_t)r * d.C, act, out_l, out_u);
+    });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
@@ -296,7 +328,7 @@ __device__ __forceinline__ void bound_dz(const Ends& e, float w, float o, int ac
     const bool turned = w < 0.f;
     const double z0 = turned ? e.z1 : e.z0, z1 = turned ? e.z0 : e.z1;
     double d0, d1;
-    bound_slope(fma(z0, (double)w, (double)o), fma(z1, (double)w, (double)o), act, g0, g1, d0, d1);
+    bound_slope(::fma(z0, (double)w, (double)o), ::fma(z1, (double)w, (double)o), act, g0, g1, d0, d1);
     dw = d0 * z0 + d1 * z1;
     db = d0 + d1;
     q0 = e.cut0 ? 0.0 : (turned ? d1 : d0) * (double)w;
@@ -323,8 +355,8 @@ __device__ __forceinline__ void sum_back(const Raw<float, V>& lv, const Raw<floa
         bound_dz(e, w[j], o[j], act, gl[j], gu[j], q0, q1, dw, db);
         by[j].x += (float)db;
         by[j].y += (float)dw;
-        s[j].a = fma(q0, e.s0, s[j].a);
-        s[j].b = fma(q1, e.s1, s[j].b);
+        s[j].a = ::fma(q0, e.s0, s[j].a);
+        s[j].b = ::fma(q1, e.s1, s[j].b);
         const double t0 = q0 * e.n0, t1 = q1 * e.n1;
         s[j].c += (e.n0 >= 0.0 ? t0 : 0.0) + (e.n1 >= 0.0 ? 0.0 : t1);
         s[j].d += (e.n0 >= 0.0 ? 0.0 : t0) + (e.n1 >= 0.0 ? t1 : 0.0);
@@ -528,7 +560,7 @@ int forward(const float* lower, const float* upper, const NormGiven& given, cons
                            out_u, sums);
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     Sum4* part = static_cast<Sum4*>(ws);
-    const size_t one = bound_space<V>(p, 0).box, two = sizeof(Box) * p.groups;
+    const size_t ring = norm_ring_bytes<float, V, 2, kBoundRing>(), one = ring + bound_space<V>(p, 0).box, two = ring + sizeof(Ends32) * p.groups;
     if (!allow_shared(bound_sums_kernel<V>, one) || !allow_shared(bound_apply_kernel<V>, two)) return LINF_ERR_LAUNCH;
     bound_sums_kernel<V><<<grid, kNormThreads, one, st>>>(lower, upper, d, p, part);
     bound_apply_kernel<V><<<grid, kNormThreads, two, st>>>(lower, upper, given.gamma, given.beta, part, d, p, eps, act, out_l, out_u, sums);

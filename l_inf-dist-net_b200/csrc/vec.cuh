@@ -106,34 +106,69 @@ __device__ __forceinline__ void store_param(void* p, int c, int type, float v) {
     else static_cast<__nv_bfloat16*>(p)[c] = __float2bfloat16_rn(v);
 }
 
-// ---- V values at a time, two to an instruction ------------------------------------------------------------------
-template <int V> __device__ __forceinline__ void add_all(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
-    if (V == 1) { r[0] = a[0] + b[0]; return; }
+// ---- V fp32 values at a time, two to a register pair and an instruction ------------------------------------------
+template <int V> struct Lanes {
+    unsigned long long p[V / 2];
+    __device__ __forceinline__ void get(float (&f)[V]) const {
 #pragma unroll
-    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(add_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), r[j], r[j + 1]);
-}
-template <int V> __device__ __forceinline__ void sub_all(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
-    if (V == 1) { r[0] = a[0] - b[0]; return; }
+        for (int j = 0; j < V / 2; ++j) unpack_f32x2(p[j], f[2 * j], f[2 * j + 1]);
+    }
+    __device__ __forceinline__ void set(const float (&f)[V]) {
 #pragma unroll
-    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(sub_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), r[j], r[j + 1]);
-}
-template <int V> __device__ __forceinline__ void mul_all(float (&r)[V], const float (&a)[V], const float (&b)[V]) {
-    if (V == 1) { r[0] = a[0] * b[0]; return; }
+        for (int j = 0; j < V / 2; ++j) p[j] = pack_f32x2(f[2 * j], f[2 * j + 1]);
+    }
+    __device__ __forceinline__ void fill(float f) {
 #pragma unroll
-    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(mul_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1])), r[j], r[j + 1]);
-}
-template <int V> __device__ __forceinline__ void mul_all(float (&r)[V], const float (&a)[V], float b) {
-    if (V == 1) { r[0] = a[0] * b; return; }
-    const unsigned long long two = pack_f32x2(b, b);
+        for (int j = 0; j < V / 2; ++j) p[j] = pack_f32x2(f, f);
+    }
+};
+template <> struct Lanes<1> {
+    float p[1];
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = p[0]; }
+    __device__ __forceinline__ void set(const float (&f)[1]) { p[0] = f[0]; }
+    __device__ __forceinline__ void fill(float f) { p[0] = f; }
+};
+#define LINF_LANES(name, scalar, packed)                                                                   \
+    template <int V> __device__ __forceinline__ Lanes<V> name(const Lanes<V>& a, const Lanes<V>& b) {      \
+        Lanes<V> r;                                                                                        \
+        _Pragma("unroll") for (int j = 0; j < V / 2; ++j) r.p[j] = packed(a.p[j], b.p[j]);                 \
+        return r;                                                                                          \
+    }                                                                                                      \
+    __device__ __forceinline__ Lanes<1> name(const Lanes<1>& a, const Lanes<1>& b) {                       \
+        Lanes<1> r;                                                                                        \
+        r.p[0] = a.p[0] scalar b.p[0];                                                                     \
+        return r;                                                                                          \
+    }
+// (no difference: the packed addition takes no sign, and turning the signs of a pair costs two operations)
+LINF_LANES(add, +, add_f32x2)
+LINF_LANES(mul, *, mul_f32x2)
+#undef LINF_LANES
+template <int V> __device__ __forceinline__ Lanes<V> fma(const Lanes<V>& a, const Lanes<V>& b, const Lanes<V>& c) {
+    Lanes<V> r;
 #pragma unroll
-    for (int j = 0; j + 1 < V; j += 2) unpack_f32x2(mul_f32x2(pack_f32x2(a[j], a[j + 1]), two), r[j], r[j + 1]);
+    for (int j = 0; j < V / 2; ++j) r.p[j] = fma_f32x2(a.p[j], b.p[j], c.p[j]);
+    return r;
 }
-template <int V> __device__ __forceinline__ void fma_all(float (&r)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
-    if (V == 1) { r[0] = fmaf(a[0], b[0], c[0]); return; }
-#pragma unroll
-    for (int j = 0; j + 1 < V; j += 2)
-        unpack_f32x2(fma_f32x2(pack_f32x2(a[j], a[j + 1]), pack_f32x2(b[j], b[j + 1]), pack_f32x2(c[j], c[j + 1])), r[j], r[j + 1]);
+__device__ __forceinline__ Lanes<1> fma(const Lanes<1>& a, const Lanes<1>& b, const Lanes<1>& c) {
+    Lanes<1> r;
+    r.p[0] = fmaf(a.p[0], b.p[0], c.p[0]);
+    return r;
 }
+template <int V> __device__ __forceinline__ Lanes<V> filled(float f) { Lanes<V> r; r.fill(f); return r; }
+template <int V> __device__ __forceinline__ Lanes<V> lanes(const float (&f)[V]) { Lanes<V> r; r.set(f); return r; }
+template <typename T, int V>
+__device__ __forceinline__ Lanes<V> lanes_of(const Raw<T, V>& raw) {
+    float f[V];
+    unpack<T, V>(raw, f);
+    return lanes<V>(f);
+}
+template <typename T, int V>
+__device__ __forceinline__ Raw<T, V> raw_of(const Lanes<V>& v) {
+    float f[V];
+    v.get(f);
+    return pack<T, V>(f);
+}
+template <typename T, int V> __device__ __forceinline__ Lanes<V> load_lanes(const T* p) { return lanes_of<T, V>(load_raw<T, V>(p)); }
 
 // ---- activations: the value, and the value's derivative ---------------------------------------------------------
 // silu(u) = u / (1 + e^-u) has one minimum, at u = kSiluArg; it falls before and rises behind it
@@ -155,56 +190,54 @@ __device__ __forceinline__ float tanh16(float u) {
 template <bool WIDE> __device__ __forceinline__ float tanh_of(float u) { return WIDE ? tanhf(u) : tanh16(u); }
 
 // 1 / (1 + e^-u): both ends come out as 1 and 0
-template <int V> __device__ __forceinline__ void sigmoid_all(float (&q)[V], const float (&u)[V]) {
-    float one[V];
+template <int V> __device__ __forceinline__ Lanes<V> sigmoid(const Lanes<V>& u) {
+    float f[V];
+    mul(u, filled<V>(-kLog2E)).get(f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) one[j] = 1.f;
-    mul_all<V>(q, u, -kLog2E);
+    for (int j = 0; j < V; ++j) f[j] = exp2_unit(f[j]);
+    add(lanes<V>(f), filled<V>(1.f)).get(f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) q[j] = exp2_unit(q[j]);
-    add_all<V>(q, q, one);
-#pragma unroll
-    for (int j = 0; j < V; ++j) q[j] = rcp_unit(q[j]);
+    for (int j = 0; j < V; ++j) f[j] = rcp_unit(f[j]);
+    return lanes<V>(f);
 }
 
 // WIDE: the results stay fp32.
 template <bool WIDE, int V>
-__device__ __forceinline__ void activate_all(float (&f)[V], int act) {
+__device__ __forceinline__ Lanes<V> activate(const Lanes<V>& u, int act) {
+    if (act == LINF_ACT_IDENTITY) return u;
+    if (act == LINF_ACT_SILU) return mul(u, sigmoid<V>(u));
+    float f[V];
+    u.get(f);
     if (act == LINF_ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = f[j] < 0.f ? 0.f : f[j];          // keeps a NaN
-    } else if (act == LINF_ACT_TANH) {
+    } else {
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = tanh_of<WIDE>(f[j]);
-    } else if (act == LINF_ACT_SILU) {
-        float q[V];
-        sigmoid_all<V>(q, f);
-        mul_all<V>(f, f, q);
     }
+    return lanes<V>(f);
 }
 template <bool WIDE, int V>
-__device__ __forceinline__ void slope_all(float (&f)[V], int act) {
+__device__ __forceinline__ Lanes<V> slope(const Lanes<V>& u, int act) {
+    const Lanes<V> one = filled<V>(1.f);
+    if (act == LINF_ACT_IDENTITY) return one;
+    if (act == LINF_ACT_SILU) {
+        const Lanes<V> q = sigmoid<V>(u);
+        return mul(fma(u, fma(q, filled<V>(-1.f), one), one), q);
+    }
+    float f[V];
+    u.get(f);
     if (act == LINF_ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < V; ++j) f[j] = f[j] > 0.f ? 1.f : 0.f;
-    } else if (act == LINF_ACT_TANH) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) { const float t = tanh_of<WIDE>(f[j]); f[j] = fmaf(-t, t, 1.f); }
-    } else if (act == LINF_ACT_SILU) {
-        float q[V], one[V], rest[V];
-        sigmoid_all<V>(q, f);
-#pragma unroll
-        for (int j = 0; j < V; ++j) one[j] = 1.f;
-        sub_all<V>(rest, one, q);
-        fma_all<V>(f, f, rest, one);
-        mul_all<V>(f, f, q);
     } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = 1.f;
+        for (int j = 0; j < V; ++j) { const float t = tanh_of<WIDE>(f[j]); f[j] = fmaf(-t, t, 1.f); }
     }
+    return lanes<V>(f);
 }
-__device__ __forceinline__ float activate(float u, int act) { float f[1] = {u}; activate_all<true, 1>(f, act); return f[0]; }
-__device__ __forceinline__ float slope(float u, int act) { float f[1] = {u}; slope_all<true, 1>(f, act); return f[0]; }
+__device__ __forceinline__ float activate(float u, int act) { return activate<true, 1>(filled<1>(u), act).p[0]; }
+__device__ __forceinline__ float slope(float u, int act) { return slope<true, 1>(filled<1>(u), act).p[0]; }
 
 // ---- counter-based dropout --------------------------------------------------------------------------------------
 // Philox4x32 with 7 rounds (Salmon, Moraes, Dror, Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011; 7 is the least
@@ -257,9 +290,12 @@ __device__ __forceinline__ unsigned drop_mask(const Drop& d, const DropKey& k, u
     return mask;
 }
 template <int V>
-__device__ __forceinline__ void drop_masked(const Drop& d, unsigned mask, float (&f)[V]) {
+__device__ __forceinline__ void drop_masked(const Drop& d, unsigned mask, Lanes<V>& v) {
+    float f[V];
+    v.get(f);
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = (mask >> j & 1u) ? f[j] * d.scale : 0.f;
+    v.set(f);
 }
 // scaled where the piece keeps it, 0 where not (whatever the value was, a NaN included)
 __device__ __forceinline__ float drop_one(const Drop& d, unsigned piece, float f) { return piece >= d.threshold ? f * d.scale : 0.f; }

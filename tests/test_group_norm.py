@@ -397,17 +397,33 @@ def make_box(shape, seed, radius, level=3.0):
 
 
 def bound_reference(lo, up, w, b, groups, act, g0, g1):
-    """Values and gradients in 64 bits, and what they may be off by: all is computed in 64 bits but for v rounded to fp32, the
-    activation and its slope (norm_reference.error_of_act, error_of_slope of that rounding), their product with the gradient, and one
-    rounding of each result; what a gradient's terms may be off by passes through the linear steps behind them by the terms' sizes."""
+    """Values and gradients in 64 bits, and what they may be off by.
+
+    Values: the sums and what a group shares are 64-bit, rounded to fp32 (E; the means in two parts, as good as exact).  n = (l - mean) + own with
+    own = (u - l) / M: a rounding of the first difference and one of its second part (2 E |l - mean|, which is at most |n| + |own|), three of
+    own, one of the sum: below 4 E (|n| + 2 |own|).  z = n s: that times s, and 2 E |z|.  v = w z + b: |w| times that and E |v|, twice for
+    the squares left out.  Then the activation's own error.  Gradients: computed in 64 bits but for v rounded to fp32, the slope
+    (norm_reference.error_of_slope of that rounding), its product with the gradient, and one rounding of each result; what a gradient's
+    terms may be off by passes through the linear steps behind them by the terms' sizes."""
     leaves = [t.double().requires_grad_() for t in (lo, up, w, b)]
     ys = R.group_norm_bound(*leaves[:2], groups, *leaves[2:], EPS, act)
     grads = torch.autograd.grad(ys, leaves, [g0.double(), g1.double()])
     with torch.no_grad():
         v = R.bound_parts(*[t.double() for t in (lo, up)], groups, w.double(), b.double(), EPS)
+        N, C = lo.shape[:2]
+        l, u = (t.double().reshape(N, groups, -1) for t in (lo, up))
+        M = l.size(2)
+        ctr, rad = (l + u) / 2, (u - l) / 2
+        sd = ((ctr - ctr.mean(2, keepdim=True)) ** 2).mean(2, keepdim=True).sqrt()
+        tight = ((sd - (rad ** 2).mean(2, keepdim=True).sqrt()).clamp(min=0) ** 2 + EPS) ** -0.5
+        wide = [(l - u.mean(2, keepdim=True)).abs(), (u - l.mean(2, keepdim=True)).abs()]
+        cut = torch.tensor(math.sqrt(M - 1), dtype=torch.float64)
+        ez = [4 * E * (n + 3 * rad * 2 / M) * tight + 2 * E * torch.minimum(n * tight, cut) for n in wide]
+        ez = torch.maximum(*ez).reshape(lo.shape) * w.double().abs().view([1, C] + [1] * (lo.dim() - 2))
+        off = [2 * (ez + E * t.abs()) for t in v]
         most = []
-        for y, e in zip(ys, v):
-            worst = torch.maximum(*[R.error_of_act(t, E * t.abs(), act) for t in v]) if act == "silu" else R.error_of_act(e, E * e.abs(), act)
+        for y, e, o in zip(ys, v, off):
+            worst = torch.maximum(*[R.error_of_act(t, f, act) for t, f in zip(v, off)]) if act == "silu" else R.error_of_act(e, o, act)
             most.append(worst + R.rounded(y, torch.float32))
     # one gradient at a time, its size in the place of its value: d / dv is scaled by what the slope may be off by
     def spread(which, g):
