@@ -51,14 +51,12 @@ dropout_kernel(Tensors t, long long n, Drop d) {
                 for (int j = 0; j < 8; ++j)
                     if (b * 8 + j < n) f[k][j] = to_float<T>(static_cast<const T*>(t.in[k])[b * 8 + j]);
         }
-        const uint4 w = drop_words(key, (unsigned long long)b);
-        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+        unsigned piece[8];
+        drop_pieces<8>(key, (unsigned long long)b * 8, piece);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const unsigned piece = (j & 1) ? u[j >> 1] >> 16 : u[j >> 1] & 0xffffu;
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int k = 0; k < TENSORS; ++k) f[k][j] = drop_one(d, piece, f[k][j]);
-        }
+            for (int k = 0; k < TENSORS; ++k) f[k][j] = piece[j] > d.limit ? f[k][j] * d.scale : 0.f;
         if (whole) {
 #pragma unroll
             for (int k = 0; k < TENSORS; ++k) Eight<T>::store(static_cast<T*>(t.out[k]) + b * 8, f[k]);

@@ -40,11 +40,9 @@ __device__ __forceinline__ void load_column(Column<V>& k, const float2* stat, co
 }
 template <typename T, int V>
 __device__ __forceinline__ void write_vector(const Raw<T, V>& v, const Column<V>& col, int act, const Drop& drop, const DropKey& key, size_t i, T* y) {
-    const Lanes<V> u = activate<sizeof(T) == 4, V>(fma(add(lanes_of<T, V>(v), col.m), col.a, col.o), act);
-    float f[V];
-    u.get(f);
-    if (drop.on) drop_apply<V>(drop, key, i, f);
-    store_once<T, V>(y + i, pack<T, V>(f));
+    Lanes<V> u = activate<sizeof(T) == 4, V>(fma(add(lanes_of<T, V>(v), col.m), col.a, col.o), act);
+    if (drop.on) u = linf::drop<V>(drop, key, i, u);
+    store_once<T, V>(y + i, raw_of<T, V>(u));
 }
 __device__ __forceinline__ float2 finish_stat(double mean, double var, double eps) {
     return make_float2((float)mean, 1.f / sqrtf((float)(var + eps)));
@@ -209,9 +207,10 @@ norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __res
     const int r0 = split * p.rows, rows = min(p.rows, d.L - r0);
     if (rt < p.rt && cv < b.nvec) {
         const T* const at[1] = {x + ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V};
+        NormStream<T, V, 1, kRing> stream(space, at, rt, rows, p.rt, d.C);
         Moments<V> t;
         if (rt < rows) t.start(load_lanes<T, V>(at[0] + (size_t)rt * d.C));
-        norm_stream<T, V, 1, kRing>(space, at, rt, rows, p.rt, d.C, [&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); });
+        stream.template run<true>([&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); });
         t.put(red, p, rt, cv, rows_of(rows, rt, p));
     }
     const double count = (double)rows * (p.pieces == 1 ? d.Cg : b.nvec * V);
@@ -240,6 +239,11 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
     float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 1, kRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, r0 = split * p.rows;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const T* const from[1] = {x + at};
+    NormStream<T, V, 1, kRing> stream(space, from, rt, in ? min(p.rows, d.L - r0) : 0, p.rt, d.C);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const double2 v = add_parts(part, d, p, n, b.g0 + g);
         const double var = v.y - v.x * v.x;
@@ -253,17 +257,11 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
         }
     }
     __syncthreads();
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
-    if (rt >= p.rt || cv >= b.nvec) return;
+    if (!in) return;
     Column<V> col;
     load_column<V>(col, stat, gamma, beta, d, p, b, cv);
     const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-    const int r0 = split * p.rows;
-    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
-    const T* const from[1] = {x + at};
-    norm_stream<T, V, 1, kRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<T, V>(&v)[1]) {
-        write_vector<T, V>(v[0], col, act, drop, key, at + (size_t)r * d.C, y);
-    });
+    stream.template run<false>([&](int r, const Raw<T, V>(&v)[1]) { write_vector<T, V>(v[0], col, act, drop, key, at + (size_t)r * d.C, y); });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
@@ -304,12 +302,7 @@ template <typename T, int V>
 __device__ __forceinline__ void back_du(const Raw<T, V>& xv, const Raw<T, V>& gv, const BackColumn<V>& k, int act, const Drop& drop, const DropKey& key,
                                         size_t i, Lanes<V>& du, Lanes<V>& e) {
     du = lanes_of<T, V>(gv);
-    if (drop.on) {
-        float f[V];
-        du.get(f);
-        drop_apply<V>(drop, key, i, f);
-        du.set(f);
-    }
+    if (drop.on) du = linf::drop<V>(drop, key, i, du);
     back_du<T, V>(xv, k, act, du, e);
 }
 
@@ -406,7 +399,7 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
             if (drop.on) {
                 const unsigned mask = drop_mask<V>(drop, key, at + (size_t)r * d.C);
                 if (sizeof(T) == 2) kept[r * p.tx + cv] = (unsigned char)mask;
-                drop_masked<V>(drop, mask, du);
+                du = drop_masked<V>(drop, mask, du);
             }
             back_du<T, V>(load_raw<T, V>(own + r * pitch), col, act, du, e);
             sum_a = add(sum_a, du);
@@ -446,7 +439,7 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
                 if (sizeof(T) == 4) {
                     e = add(load_lanes<T, V>(own + r * pitch), col.m);
                 } else {
-                    if (drop.on) drop_masked<V>(drop, kept[r * p.tx + cv], du);
+                    if (drop.on) du = drop_masked<V>(drop, kept[r * p.tx + cv], du);
                     back_du<T, V>(load_raw<T, V>(own + r * pitch), col, act, du, e);
                 }
                 write_dx<T, V>(du, e, col, means, dx + at + (size_t)r * d.C);
@@ -479,12 +472,13 @@ norm_back_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
         Lanes<V> sum_a = filled<V>(0.f), sum_b = sum_a;
         BackColumn<V> col;
         if (cv < b.nvec) {
-            load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
-            const DropKey key = drop.on ? drop_key(drop) : DropKey{};
             const int r0 = split * p.rows;
             const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
             const T* const from[2] = {x + at, dy + at};
-            norm_stream<T, V, 2, kBackRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<T, V>(&v)[2]) {
+            NormStream<T, V, 2, kBackRing> stream(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C);
+            load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
+            const DropKey key = drop.on ? drop_key(drop) : DropKey{};
+            stream.template run<false>([&](int r, const Raw<T, V>(&v)[2]) {
                 Lanes<V> du, e;
                 back_du<T, V>(v[0], v[1], col, act, drop, key, at + (size_t)r * d.C, du, e);
                 sum_a = add(sum_a, du);
@@ -518,22 +512,23 @@ norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
     float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 2, kBackRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, r0 = split * p.rows;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const T* const from[2] = {x + at, dy + at};
+    NormStream<T, V, 2, kBackRing> stream(space, from, rt, in ? min(p.rows, d.L - r0) : 0, p.rt, d.C);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const double2 v = add_parts(by_group, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) stat[g] = make_float2((float)v.x, (float)v.y);
     }
     __syncthreads();
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
-    if (rt >= p.rt || cv >= b.nvec) return;
+    if (!in) return;
     BackColumn<V> col;
     load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
     Means<V> means;
     load_means<V>(stat, d, p, cv, col, means);
     const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-    const int r0 = split * p.rows;
-    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
-    const T* const from[2] = {x + at, dy + at};
-    norm_stream<T, V, 2, kBackRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<T, V>(&v)[2]) {
+    stream.template run<false>([&](int r, const Raw<T, V>(&v)[2]) {
         const size_t i = at + (size_t)r * d.C;
         Lanes<V> du, e;
         back_du<T, V>(v[0], v[1], col, act, drop, key, i, du, e);

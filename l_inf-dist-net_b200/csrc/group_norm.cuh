@@ -281,65 +281,85 @@ __device__ __forceinline__ Raw<T, V> load_shared(unsigned at) {
     return v;
 }
 
-// The rows r, r + step, ... below r1 of a thread's column in each of N tensors (at[k] points at row 0): body(row, vectors).  S rows are on their way
+// The rows first, first + every, ... below `end` of a thread's column in each of N tensors (at[k] points at row 0): body(row, vectors).  S rows are on their way
 // to shared memory at a time, each thread's to places of its own (`ring`: norm_ring_bytes), so that neither registers nor barriers
 // limit how much is read ahead.  Elements of two bytes that no wider copy reaches come through registers.
 template <typename T, int V, int N, int S>
 __host__ __device__ constexpr size_t norm_ring_bytes() { return sizeof(T) * V >= 4 ? (size_t)kNormThreads * sizeof(T) * V * N * S : 0; }
 
-template <typename T, int V, int N, int S, typename Body>
-__device__ __forceinline__ void norm_stream(void* ring, const T* const (&at)[N], int r, int r1, int step, size_t C, Body body) {
-    if constexpr (sizeof(T) * V >= 4) {
-        constexpr int bytes = sizeof(T) * V, place = kNormThreads * bytes;      // [S][N][threads]
-        const unsigned own = (unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * bytes;
-        const T* next[N];
+template <typename T, int V, int N, int S>
+struct NormStream {
+    static constexpr int bytes = sizeof(T) * V, place = kNormThreads * bytes;      // ring: [S][N][threads]
+    unsigned own;
+    const T* next[N];
+    size_t stride;
+    int r, r1, step, ahead;
+
+    // starts with the first rows on their way: what the CTA does before run() overlaps with them
+    __device__ __forceinline__ NormStream(void* ring, const T* const (&at)[N], int first, int end, int every, size_t C) {
+        r = ahead = first;
+        r1 = end;
+        step = every;
+        stride = (size_t)every * C;
 #pragma unroll
-        for (int k = 0; k < N; ++k) next[k] = at[k] + (size_t)r * C;
-        const size_t stride = (size_t)step * C;
-        int ahead = r;
-        auto issue = [&](int s) {
-            if (ahead < r1) {
+        for (int k = 0; k < N; ++k) next[k] = at[k] + (size_t)first * C;
+        if constexpr (bytes >= 4) {
+            own = (unsigned)__cvta_generic_to_shared(ring) + threadIdx.x * bytes;
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    copy_shared<bytes>(own + (s * N + k) * place, next[k]);
-                    next[k] += stride;
-                }
-            }
-            ahead += step;
-            cp_async_commit();
-        };
-#pragma unroll
-        for (int s = 0; s < S; ++s) issue(s);
-        auto row = [&](int s) {
-            cp_async_wait<S - 1>();
-            Raw<T, V> v[N];
-#pragma unroll
-            for (int k = 0; k < N; ++k) v[k] = load_shared<T, V>(own + (s * N + k) * place);
-            body(r, v);
-            issue(s);                                           // behind body, which has used what it overwrites
-            r += step;
-        };
-        for (int turns = r < r1 ? ((r1 - r - 1) / step + 1) / S : 0; turns > 0; --turns) {
-#pragma unroll
-            for (int s = 0; s < S; ++s) row(s);
-        }
-#pragma unroll 1
-        for (int s = 0; r < r1; ++s) row(s);
-    } else {
-        constexpr int K = 8 / N;
-        for (; r < r1; r += K * step) {
-            Raw<T, V> v[K][N];
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-#pragma unroll
-                for (int k = 0; k < N; ++k)
-                    if (r + j * step < r1) v[j][k] = load_raw<T, V>(at[k] + (size_t)(r + j * step) * C);
-#pragma unroll
-            for (int j = 0; j < K; ++j)
-                if (r + j * step < r1) body(r + j * step, v[j]);
+            for (int s = 0; s < S; ++s) issue(s);
         }
     }
-}
+    __device__ __forceinline__ void issue(int s) {
+        if (ahead < r1) {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                copy_shared<bytes>(own + (s * N + k) * place, next[k]);
+                next[k] += stride;
+            }
+        }
+        ahead += step;
+        cp_async_commit();
+    }
+    template <typename Body> __device__ __forceinline__ void row(int s, Body& body) {
+        cp_async_wait<S - 1>();
+        Raw<T, V> v[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = load_shared<T, V>(own + (s * N + k) * place);
+        body(r, v);
+        issue(s);                                               // behind body, which has used what it overwrites
+        r += step;
+    }
+    // LIGHT bodies are written out for a whole turn of the ring: half the instructions (sums of bf16 maps: 52 -> 34 a vector, 24 -> 21 us);
+    // heavy ones are not, their code would be too long (38 -> 40 us).
+    template <bool LIGHT, typename Body> __device__ __forceinline__ void run(Body body) {
+        if constexpr (bytes >= 4) {
+            if constexpr (LIGHT) {
+                for (int turns = r < r1 ? ((r1 - r - 1) / step + 1) / S : 0; turns > 0; --turns) {
+#pragma unroll
+                    for (int s = 0; s < S; ++s) row(s, body);
+                }
+            }
+#pragma unroll 1
+            for (int s = 0; r < r1; s = s + 1 == S ? 0 : s + 1) row(s, body);
+        } else {
+            constexpr int K = 8 / N;
+            for (; r < r1; r += K * step) {
+                Raw<T, V> v[K][N];
+#pragma unroll
+                for (int j = 0; j < K; ++j) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        if (r + j * step < r1) v[j][k] = load_raw<T, V>(next[k]);
+                        next[k] += stride;
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < K; ++j)
+                    if (r + j * step < r1) body(r + j * step, v[j]);
+            }
+        }
+    }
+};
 
 template <typename F>
 bool allow_shared(F kernel, size_t bytes) {

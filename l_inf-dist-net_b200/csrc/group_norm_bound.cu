@@ -269,14 +269,14 @@ bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upp
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     if (rt < p.rt && cv < b.nvec) {
-        Sum4 s[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
         const int r0 = split * p.rows;
         const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
         const float* const from[2] = {lower + at, upper + at};
-        norm_stream<float, V, 2, kBoundRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C,
-                                             [&](int, const Raw<float, V>(&v)[2]) { sum_vector<V>(v[0], v[1], s); });
+        NormStream<float, V, 2, kBoundRing> stream(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C);
+        Sum4 s[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
+        stream.template run<true>([&](int, const Raw<float, V>(&v)[2]) { sum_vector<V>(v[0], v[1], s); });
         put_sums<V>(red4, p, rt, cv, s);
     }
     __syncthreads();
@@ -301,6 +301,11 @@ bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ up
     Ends32* ends = space_at<Ends32>(space, norm_ring_bytes<float, V, 2, kBoundRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, r0 = split * p.rows;
+    const bool in = rt < p.rt && cv < b.nvec;
+    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const float* const from[2] = {lower + at, upper + at};
+    NormStream<float, V, 2, kBoundRing> stream(space, from, rt, in ? min(p.rows, d.L - r0) : 0, p.rt, d.C);
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(part, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
@@ -309,14 +314,10 @@ bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ up
         }
     }
     __syncthreads();
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
-    if (rt >= p.rt || cv >= b.nvec) return;
+    if (!in) return;
     BoundColumn<V> col;
     load_column<V>(col, ends, gamma, beta, d, p, b, cv * V);
-    const int r0 = split * p.rows;
-    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
-    const float* const from[2] = {lower + at, upper + at};
-    norm_stream<float, V, 2, kBoundRing>(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C, [&](int r, const Raw<float, V>(&v)[2]) {
+    stream.template run<false>([&](int r, const Raw<float, V>(&v)[2]) {
         write_bounds<V>(v[0], v[1], col, at + (size_t)r * d.C, act, out_l, out_u);
     });
 }

@@ -112,11 +112,9 @@ dense_norm_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, 
         for (int k = 0; k < K; ++k)
             if (s.t + k * p.tpr < vecs) {
                 const size_t at = row + (s.t + k * p.tpr) * V;
-                const Lanes<V> u = activate<sizeof(T) == 4, V>(fma(mul(add(f[k], left), scale), w[k], o[k]), act);
-                float e[V];
-                u.get(e);
-                if (drop.on) drop_apply<V>(drop, key, at, e);
-                store_once<T, V>(y + at, pack<T, V>(e));
+                Lanes<V> u = activate<sizeof(T) == 4, V>(fma(mul(add(f[k], left), scale), w[k], o[k]), act);
+                if (drop.on) u = linf::drop<V>(drop, key, at, u);
+                store_once<T, V>(y + at, raw_of<T, V>(u));
             }
     }
 }
@@ -158,12 +156,7 @@ dense_norm_back_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
             if (in && s.t + k * p.tpr < vecs) {
                 h[k] = mul(add(lanes_of<T, V>(v[k]), shift), scale);
                 du[k] = lanes_of<T, V>(g[k]);
-                if (drop.on) {
-                    float f[V];
-                    du[k].get(f);
-                    drop_apply<V>(drop, key, row + (s.t + k * p.tpr) * V, f);
-                    du[k].set(f);
-                }
+                if (drop.on) du[k] = linf::drop<V>(drop, key, row + (s.t + k * p.tpr) * V, du[k]);
                 if (act != LINF_ACT_IDENTITY) du[k] = mul(du[k], slope<sizeof(T) == 4, V>(fma(h[k], w[k], o[k]), act));
                 sum_a[k] = add(sum_a[k], du[k]);
                 sum_b[k] = fma(du[k], h[k], sum_b[k]);

@@ -250,7 +250,7 @@ __device__ __forceinline__ float slope(float u, int act) { return slope<true, 1>
 struct Drop {
     const long long* rng;       // {seed, offset} on the device
     int on;                     // 0: no dropout
-    unsigned threshold;         // 0 .. 65536
+    unsigned limit;             // threshold * 2^16 - 1: a piece in the upper half of a word, lower half whatever it is, is kept iff word > limit
     float scale;
 };
 struct DropKey { unsigned k0, k1, o0, o1; };
@@ -271,59 +271,68 @@ __device__ __forceinline__ uint4 drop_words(const DropKey& k, unsigned long long
     }
     return c;
 }
-// Bit j: element i0 + j (i0 a multiple of V) is kept.
+// The words that hold the pieces of elements i0 .. i0 + V - 1 (i0 a multiple of V) in their upper halves.
+template <int V>
+__device__ __forceinline__ void drop_pieces(const DropKey& k, unsigned long long i0, unsigned (&piece)[V]) {
+    const uint4 w = drop_words(k, i0 >> 3);
+    if constexpr (V == 8) {
+        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) piece[j] = (j & 1) ? u[j >> 1] : u[j >> 1] << 16;
+    } else {
+        const bool second = (i0 & 4) != 0;                          // of the block's two halves
+        const unsigned u[2] = {second ? w.z : w.x, second ? w.w : w.y};
+        if constexpr (V == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) piece[j] = (j & 1) ? u[j >> 1] : u[j >> 1] << 16;
+        } else {
+            const unsigned word = (i0 & 2) != 0 ? u[1] : u[0];
+            if constexpr (V == 2) {
+                piece[0] = word << 16;
+                piece[1] = word;
+            } else {
+                piece[0] = (i0 & 1) != 0 ? word : word << 16;
+            }
+        }
+    }
+}
+// Bit j: element i0 + j is kept.
 template <int V>
 __device__ __forceinline__ unsigned drop_mask(const Drop& d, const DropKey& k, unsigned long long i0) {
-    const uint4 w = drop_words(k, i0 >> 3);
-    unsigned mask = 0;
-    if (V == 8) {
-        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+    unsigned piece[V], mask = 0;
+    drop_pieces<V>(k, i0, piece);
 #pragma unroll
-        for (int j = 0; j < V; ++j) mask |= (((j & 1) ? u[(j >> 1) & 3] >> 16 : u[(j >> 1) & 3] & 0xffffu) >= d.threshold ? 1u : 0u) << j;
-    } else {
-        const bool second = (i0 & 4) != 0;
-        unsigned long long bits = second ? ((unsigned long long)w.w << 32 | w.z) : ((unsigned long long)w.y << 32 | w.x);
-        if (V < 4) bits >>= 16 * (unsigned)(i0 & 3);
-#pragma unroll
-        for (int j = 0; j < V; ++j) mask |= ((unsigned)((bits >> (16 * (j & 3))) & 0xffffu) >= d.threshold ? 1u : 0u) << j;
-    }
+    for (int j = 0; j < V; ++j) mask |= (piece[j] > d.limit ? 1u : 0u) << j;
     return mask;
 }
+// Scaled where it is kept, 0 where not (whatever the value was, a NaN included).
 template <int V>
-__device__ __forceinline__ void drop_masked(const Drop& d, unsigned mask, Lanes<V>& v) {
+__device__ __forceinline__ Lanes<V> drop_masked(const Drop& d, unsigned mask, const Lanes<V>& v) {
     float f[V];
-    v.get(f);
+    mul(v, filled<V>(d.scale)).get(f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = (mask >> j & 1u) ? f[j] * d.scale : 0.f;
-    v.set(f);
+    for (int j = 0; j < V; ++j) f[j] = (mask >> j & 1u) ? f[j] : 0.f;
+    return lanes<V>(f);
 }
-// scaled where the piece keeps it, 0 where not (whatever the value was, a NaN included)
-__device__ __forceinline__ float drop_one(const Drop& d, unsigned piece, float f) { return piece >= d.threshold ? f * d.scale : 0.f; }
-// f[j] of element i0 + j (i0 a multiple of V)
 template <int V>
-__device__ __forceinline__ void drop_apply(const Drop& d, const DropKey& k, unsigned long long i0, float (&f)[V]) {
-    const uint4 w = drop_words(k, i0 >> 3);
-    if (V == 8) {
-        const unsigned u[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ Lanes<V> drop(const Drop& d, const DropKey& k, unsigned long long i0, const Lanes<V>& v) {
+    unsigned piece[V];
+    drop_pieces<V>(k, i0, piece);
+    float f[V];
+    mul(v, filled<V>(d.scale)).get(f);
 #pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = drop_one(d, (j & 1) ? u[(j >> 1) & 3] >> 16 : u[(j >> 1) & 3] & 0xffffu, f[j]);
-    } else {
-        // the 64 bits that hold the pieces of this element's half of the block, shifted to its first piece
-        const bool second = (i0 & 4) != 0;
-        unsigned long long bits = second ? ((unsigned long long)w.w << 32 | w.z) : ((unsigned long long)w.y << 32 | w.x);
-        if (V < 4) bits >>= 16 * (unsigned)(i0 & 3);
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[j] = drop_one(d, (unsigned)((bits >> (16 * (j & 3))) & 0xffffu), f[j]);
-    }
+    for (int j = 0; j < V; ++j) f[j] = piece[j] > d.limit ? f[j] : 0.f;
+    return lanes<V>(f);
 }
 
 // threshold and scale of a rate in [0, 1]; false outside (a NaN included).  Rate 1 keeps nothing.
 inline bool make_drop(double rate, const long long* rng, Drop* d) {
     if (!(rate >= 0.0 && rate <= 1.0)) return false;
-    d->threshold = (unsigned)(rate * 65536.0 + 0.5);
-    d->scale = d->threshold < 65536u ? (float)(65536.0 / (65536.0 - (double)d->threshold)) : 0.f;
+    const unsigned threshold = (unsigned)(rate * 65536.0 + 0.5);
+    d->limit = threshold * 65536u - 1u;             // 65536 * 65536 wraps around to 0: no word is above the limit
+    d->scale = threshold < 65536u ? (float)(65536.0 / (65536.0 - (double)threshold)) : 0.f;
     d->rng = rng;
-    d->on = d->threshold > 0;                       // a threshold of 0 keeps every element as it is
+    d->on = threshold > 0;                          // a threshold of 0 keeps every element as it is
     return true;
 }
 

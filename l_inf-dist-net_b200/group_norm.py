@@ -19,7 +19,8 @@ ACTIVATIONS = {"identity": 0, "relu": 1, "tanh": 2, "silu": 3}        # LINF_ACT
 
 def _rows(t):
     """[N, C, ...] -> the tensor itself where its channels lie last in memory, or a copy for which they do."""
-    if t.is_contiguous() if t.dim() == 2 else t.movedim(1, -1).is_contiguous():
+    dims = t.dim()
+    if t.is_contiguous() if dims == 2 else t.is_contiguous(memory_format=torch.channels_last) if dims == 4 else t.movedim(1, -1).is_contiguous():
         return t
     return t.movedim(1, -1).contiguous().movedim(-1, 1)
 
