@@ -85,26 +85,25 @@ template <int V> struct Moments {
     }
 };
 
-// (mean, M2) of each group of the block over `rows` rows from what the threads put into red; done(g, mean, M2) in one lane.
+// (mean, M2) of each group of the block over the CTA's rows from what the threads put into red; done(g, mean, M2) in one lane.
 template <int V, typename Done>
-__device__ __forceinline__ void join_moments(float2* red, const NormDims& d, const NormPlan& p, const NormBlock& b, int rows, Done done) {
+__device__ __forceinline__ void join_moments(float2* red, const NormDims& d, const NormPlan& p, const NormBlock& b, const NormRows& share, Done done) {
     const int each = p.same ? V : 1, width = p.same ? p.tx : p.tx * V, lane = threadIdx.x & 31;
     const int per = (p.pieces == 1 ? d.Cg : b.nvec * V) / each;         // columns of red of a group
     __syncthreads();
     if (p.rt > 1) {
         // columns along the rows, about the first row's mean
-        const int base = rows / p.rt, more = rows - base * p.rt;     // rows of a thread: one more in the first `more` of them
         by_columns(width, p.rt, [&](int c, int first, int step, auto join) {
             const float k0 = c < width ? red[c].x : 0.f, one = 1.f / (float)each;
             float s = 0.f, q = 0.f;
             for (int r = first; r < p.rt; r += step) {
                 const float2 v = red[r * width + c];
-                const float count = (float)(base + (r < more)), e = v.x - k0;
+                const float count = (float)rows_of(share, r), e = v.x - k0;
                 s = fmaf(count, e, s);
                 q = fmaf(count * e, e, fmaf(v.y, one, q));
             }
             if (join(s, q)) {
-                const float inv = 1.f / (float)rows;
+                const float inv = 1.f / (float)share.all;
                 red[c] = make_float2(fmaf(s, inv, k0), fmaf(-s * inv, s, q) * (float)each);
             }
         });
@@ -113,7 +112,7 @@ __device__ __forceinline__ void join_moments(float2* red, const NormDims& d, con
     // groups along their columns, about the first column's mean: as many lanes to a group as the group has columns, up to a warp
     int wide = 1;
     while (wide < per && wide < 32) wide *= 2;
-    const float weight = 1.f / (float)(rows * each), share = 1.f / (float)per;
+    const float weight = 1.f / ((float)share.all * (float)each), by = 1.f / (float)per;
     for (int g0 = (threadIdx.x >> 5) * (32 / wide); g0 < b.ng; g0 += (blockDim.x >> 5) * (32 / wide)) {
         const int g = g0 + lane / wide;
         float s = 0.f, q = 0.f, k0 = 0.f;
@@ -130,7 +129,7 @@ __device__ __forceinline__ void join_moments(float2* red, const NormDims& d, con
             s += __shfl_xor_sync(0xffffffffu, s, o);
             q += __shfl_xor_sync(0xffffffffu, q, o);
         }
-        if (g < b.ng && (lane & (wide - 1)) == 0) done(g, fmaf(s, share, k0), fmaf(-s * share, s, q) * (float)rows * (float)each);
+        if (g < b.ng && (lane & (wide - 1)) == 0) done(g, fmaf(s, by, k0), fmaf(-s * by, s, q) * (float)share.all * (float)each);
     }
 }
 
@@ -160,7 +159,8 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const bool in = rt < p.rt && cv < b.nvec;
-    const int rows = d.L, r1 = in ? rows : 0;
+    const int r1 = in ? d.L : 0;
+    const NormRows share = norm_rows(d, p, 0);
     const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
     T* own = data + cv * V;
     const int pitch = p.tx * V;
@@ -171,9 +171,9 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
         if (rt < r1) t.start(load_lanes<T, V>(own + rt * pitch));
 #pragma unroll 4
         for (int r = rt + p.rt; r < r1; r += p.rt) t.add(load_lanes<T, V>(own + r * pitch));
-        t.put(red, p, rt, cv, rows_of(rows, rt, p));
+        t.put(red, p, rt, cv, rows_of(share, rt));
     }
-    join_moments<V>(red, d, p, b, rows, [&](int g, float mu, float m2) {
+    join_moments<V>(red, d, p, b, share, [&](int g, float mu, float m2) {
         const float2 s = finish_stat(mu, (double)m2 * d.inv_m, eps);
         stat[g] = s;
         if (mean != nullptr) {
@@ -204,17 +204,19 @@ norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __res
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
-    const int r0 = split * p.rows, rows = min(p.rows, d.L - r0);
+    const NormRows share = norm_rows(d, p, split);
     if (rt < p.rt && cv < b.nvec) {
-        const T* const at[1] = {x + ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V};
-        NormStream<T, V, 1, kRing> stream(space, at, rt, rows, p.rt, d.C);
+        const int first = split * p.rt + rt;
+        const T* const at[1] = {x + ((size_t)n * d.L) * d.C + b.c0 + cv * V};
+        NormStream<T, V, 1, kRing> stream(space, at, first, d.L, p.splits * p.rt, d.C);
+        grid_let_go();
         Moments<V> t;
-        if (rt < rows) t.start(load_lanes<T, V>(at[0] + (size_t)rt * d.C));
+        t.start(load_lanes<T, V>(at[0] + (size_t)first * d.C));
         stream.template run<true>([&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); });
-        t.put(red, p, rt, cv, rows_of(rows, rt, p));
+        t.put(red, p, rt, cv, rows_of(share, rt));
     }
-    const double count = (double)rows * (p.pieces == 1 ? d.Cg : b.nvec * V);
-    join_moments<V>(red, d, p, b, rows, [&](int g, float mu, float m2) {
+    const double count = (double)share.all * (p.pieces == 1 ? d.Cg : b.nvec * V);
+    join_moments<V>(red, d, p, b, share, [&](int g, float mu, float m2) {
         part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_double2(count * mu, m2 + count * mu * mu);
     });
 }
@@ -239,11 +241,12 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
     float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 1, kRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, r0 = split * p.rows;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const bool in = rt < p.rt && cv < b.nvec;
-    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
     const T* const from[1] = {x + at};
-    NormStream<T, V, 1, kRing> stream(space, from, rt, in ? min(p.rows, d.L - r0) : 0, p.rt, d.C);
+    NormStream<T, V, 1, kRing> stream(space, from, split * p.rt + rt, in ? d.L : 0, p.splits * p.rt, d.C);
+    grid_wait();
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const double2 v = add_parts(part, d, p, n, b.g0 + g);
         const double var = v.y - v.x * v.x;
@@ -472,10 +475,10 @@ norm_back_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
         Lanes<V> sum_a = filled<V>(0.f), sum_b = sum_a;
         BackColumn<V> col;
         if (cv < b.nvec) {
-            const int r0 = split * p.rows;
-            const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+            const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
             const T* const from[2] = {x + at, dy + at};
-            NormStream<T, V, 2, kBackRing> stream(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C);
+            NormStream<T, V, 2, kBackRing> stream(space, from, split * p.rt + rt, d.L, p.splits * p.rt, d.C);
+            grid_let_go();
             load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
             const DropKey key = drop.on ? drop_key(drop) : DropKey{};
             stream.template run<false>([&](int r, const Raw<T, V>(&v)[2]) {
@@ -512,11 +515,12 @@ norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
     float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 2, kBackRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, r0 = split * p.rows;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const bool in = rt < p.rt && cv < b.nvec;
-    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
     const T* const from[2] = {x + at, dy + at};
-    NormStream<T, V, 2, kBackRing> stream(space, from, rt, in ? min(p.rows, d.L - r0) : 0, p.rt, d.C);
+    NormStream<T, V, 2, kBackRing> stream(space, from, split * p.rt + rt, in ? d.L : 0, p.splits * p.rt, d.C);
+    grid_wait();
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const double2 v = add_parts(by_group, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) stat[g] = make_float2((float)v.x, (float)v.y);
@@ -542,6 +546,7 @@ norm_params_kernel(const float2* __restrict__ by_channel, long long count, int C
     __shared__ double2 red[32][8];
     const int col = threadIdx.x & 7, lane = threadIdx.x >> 3, c = blockIdx.x * 8 + col;
     double a = 0.0, e = 0.0;
+    grid_wait();
     if (c < C) {
 #pragma unroll 4
         for (long long k = lane; k < count; k += 32) {
@@ -585,8 +590,8 @@ int forward(const T* x, const NormGiven& given, const NormDims& d, const NormPla
     const size_t one = ring + sizeof(float2) * p.rt * p.tx * (p.same ? 1 : V), two = ring + sizeof(float2) * p.groups;
     if (!allow_shared(norm_sums_kernel<T, V>, one) || !allow_shared(norm_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
     norm_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(x, d, p, part);
-    norm_apply_kernel<T, V><<<grid, kNormThreads, two, st>>>(x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
-    return launch_status(2);
+    if (launch_status()) return LINF_ERR_LAUNCH;
+    return launch_behind(norm_apply_kernel<T, V>, grid, kNormThreads, two, st, x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
 }
 
 template <typename T, int V>
@@ -605,9 +610,12 @@ int backward(const T* dy, const T* x, const NormGiven& given, int ptype, const f
         const size_t one = ring + sizeof(float2) * p.rt * p.tx * V, two = ring + sizeof(float2) * p.groups;
         if (!allow_shared(norm_back_sums_kernel<T, V>, one) || !allow_shared(norm_back_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
         norm_back_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_channel, by_group);
-        if (dx != nullptr)
-            norm_back_apply_kernel<T, V><<<grid, kNormThreads, two, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_group, dx);
-        if (launch_status(dx != nullptr ? 2 : 1)) return LINF_ERR_LAUNCH;
+        if (launch_status()) return LINF_ERR_LAUNCH;
+        if (dx != nullptr) {
+            const int rc = launch_behind(norm_back_apply_kernel<T, V>, grid, kNormThreads, two, st, dy, x, given.gamma, given.beta, mean, rstd, d, p, act,
+                                         drop, by_group, dx);
+            if (rc) return rc;
+        }
     }
     return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, channel_rows(p), d.C, dgamma, dbeta, ptype, st) : LINF_OK;
 }
@@ -635,8 +643,7 @@ bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g) {
 }
 
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st) {
-    norm_params_kernel<<<(C + 7) / 8, 256, 0, st>>>(by_channel, count, C, dgamma, dbeta, ptype);
-    return launch_status();
+    return launch_behind(norm_params_kernel, dim3((C + 7) / 8), 256, 0, st, by_channel, count, C, dgamma, dbeta, ptype);
 }
 
 size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back) {

@@ -5,8 +5,8 @@
 // Vectors are as wide as C, the groups and the pointers' alignment allow: a block of whole groups starts and ends on a vector.
 //
 // Where a CTA's shared memory holds a sample's column block, the CTA keeps it there ("kept"): every tensor is read once, reduced and
-// written.  What is larger takes two passes over memory: sums of row ranges, then, in a second launch whose CTAs add those up first and
-// which takes the ranges in the opposite order, the results: what was read last is still in L2.
+// written.  What is larger takes two passes over memory: sums of parts of the rows, then, in a second launch whose CTAs add those up first and
+// which takes the samples in the opposite order, the results: what was read last is still in L2.
 #pragma once
 
 #include "vec.cuh"
@@ -40,7 +40,7 @@ struct NormPlan {
     int same;                   // 1: all channels of a vector belong to one group
     int threads;                // of a CTA
     int kept;                   // 1: a CTA keeps a column block of a sample in shared memory, 0: two passes
-    int splits, rows;           // row ranges of a column block (kept: 1), rows of a range
+    int splits, rows;           // CTAs that share a column block's rows (kept: 1), rows that a kept block has
     int per_cta, chunks;        // samples that a CTA takes one after the other (kept), CTAs along the samples
     Divider by_tx, by_blocks, by_cg;
 };
@@ -184,8 +184,8 @@ inline void norm_two_passes(const NormDims& d, const NormKind& kind, bool aligne
         const double full = (double)(ctas * k) / (double)(norm_ceil(ctas * k, places) * places);
         if (full > best) { best = full; s = k; }
     }
-    p->rows = norm_ceil(d.L, s);
-    p->splits = norm_ceil(d.L, p->rows);
+    p->rows = 0;
+    p->splits = (int)s;                                         // splits * rt <= L: every thread has a row
     p->per_cta = 1;
     p->chunks = d.N;
 }
@@ -236,8 +236,18 @@ __device__ __forceinline__ double warp_sum(double v) {
     return v;
 }
 
-// rows rt, rt + p.rt, ... of [0, rows): how many
-__device__ __forceinline__ int rows_of(int rows, int rt, const NormPlan& p) { return rt < rows ? (rows - rt - 1) / p.rt + 1 : 0; }
+// The rows of a CTA: the threads of all row ranges take the sample's rows in turn, so that CTAs that run side by side read side by side.  A thread
+// has `base` rows, or one more in the first `more` of the CTA's rows of threads.
+struct NormRows { int base, more, all; };
+__device__ __forceinline__ NormRows norm_rows(const NormDims& d, const NormPlan& p, int split) {
+    const int threads = p.splits * p.rt;
+    NormRows r;
+    r.base = d.L / threads;
+    r.more = min(max(d.L - r.base * threads - split * p.rt, 0), p.rt);
+    r.all = r.base * p.rt + r.more;
+    return r;
+}
+__device__ __forceinline__ int rows_of(const NormRows& r, int rt) { return r.base + (rt < r.more ? 1 : 0); }
 
 // Columns c of [0, width), each with as many neighbouring lanes as the CTA has to spare, up to a warp: body(c, first row, step, join) adds the
 // rows first, first + step, ... up and calls join(s, t), which adds both over the lanes and is true in the one that keeps them.  c >= width
@@ -364,6 +374,31 @@ struct NormStream {
 template <typename F>
 bool allow_shared(F kernel, size_t bytes) {
     return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+}
+
+// ---- launches that begin before the kernel in front has ended ---------------------------------------------------------
+// The kernel in front lets the next one's CTAs in where its own have left (all of its CTAs are running by then); what it wrote is read
+// behind grid_wait(), which returns when it has ended.  What the CTAs do before that overlaps with its end and with the launch itself.
+__device__ __forceinline__ void grid_let_go() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename... A, typename... B>
+int launch_behind(void (*kernel)(A...), dim3 grid, int threads, size_t shared, cudaStream_t st, B... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = shared;
+    c.stream = st;
+    cudaLaunchAttribute a = {};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &a;
+    c.numAttrs = 1;
+    if (cudaLaunchKernelEx(&c, kernel, A(args)...) != cudaSuccess) {
+        cudaGetLastError();
+        return LINF_ERR_LAUNCH;
+    }
+    return launch_status();
 }
 
 // A kept call.

@@ -269,10 +269,10 @@ bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upp
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     if (rt < p.rt && cv < b.nvec) {
-        const int r0 = split * p.rows;
-        const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
         const float* const from[2] = {lower + at, upper + at};
-        NormStream<float, V, 2, kBoundRing> stream(space, from, rt, min(p.rows, d.L - r0), p.rt, d.C);
+        NormStream<float, V, 2, kBoundRing> stream(space, from, split * p.rt + rt, d.L, p.splits * p.rt, d.C);
+        grid_let_go();
         Sum4 s[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
@@ -301,11 +301,12 @@ bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ up
     Ends32* ends = space_at<Ends32>(space, norm_ring_bytes<float, V, 2, kBoundRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
-    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, r0 = split * p.rows;
+    const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const bool in = rt < p.rt && cv < b.nvec;
-    const size_t at = ((size_t)n * d.L + r0) * d.C + b.c0 + cv * V;
+    const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
     const float* const from[2] = {lower + at, upper + at};
-    NormStream<float, V, 2, kBoundRing> stream(space, from, rt, in ? min(p.rows, d.L - r0) : 0, p.rt, d.C);
+    NormStream<float, V, 2, kBoundRing> stream(space, from, split * p.rt + rt, in ? d.L : 0, p.splits * p.rt, d.C);
+    grid_wait();
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(part, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
@@ -496,9 +497,8 @@ bound_back_sums_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
         float w[V], o[V];
         load_params<V>(gamma, b.c0 + c, w);
         load_params<V>(beta, b.c0 + c, o);
-        const int r1 = min(d.L, (split + 1) * p.rows);
         const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
-        for (int r = split * p.rows + rt; r < r1; r += p.rt) {
+        for (int r = split * p.rt + rt; r < d.L; r += p.splits * p.rt) {
             const size_t i = at + (size_t)r * d.C;
             sum_back<V>(load_raw<float, V>(in4.lower + i), load_raw<float, V>(in4.upper + i), load_raw<float, V>(in4.g_l + i),
                         load_raw<float, V>(in4.g_u + i), box, w, o, d, p, c, act, s, by);
@@ -520,6 +520,7 @@ bound_back_apply_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict
     Back* back = reinterpret_cast<Back*>(reinterpret_cast<char*>(space) + at_.back);
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
+    grid_wait();
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(by_group, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
@@ -534,9 +535,8 @@ bound_back_apply_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict
     float w[V], o[V];
     load_params<V>(gamma, b.c0 + c, w);
     load_params<V>(beta, b.c0 + c, o);
-    const int r1 = min(d.L, (split + 1) * p.rows);
     const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
-    for (int r = split * p.rows + rt; r < r1; r += p.rt) {
+    for (int r = split * p.rt + rt; r < d.L; r += p.splits * p.rt) {
         const size_t i = at + (size_t)r * d.C;
         write_back<V>(load_raw<float, V>(in4.lower + i), load_raw<float, V>(in4.upper + i), load_raw<float, V>(in4.g_l + i),
                       load_raw<float, V>(in4.g_u + i), box, back, w, o, d, p, c, i, act, d_l, d_u);
@@ -564,8 +564,9 @@ int forward(const float* lower, const float* upper, const NormGiven& given, cons
     const size_t ring = norm_ring_bytes<float, V, 2, kBoundRing>(), one = ring + bound_space<V>(p, 0).box, two = ring + sizeof(Ends32) * p.groups;
     if (!allow_shared(bound_sums_kernel<V>, one) || !allow_shared(bound_apply_kernel<V>, two)) return LINF_ERR_LAUNCH;
     bound_sums_kernel<V><<<grid, kNormThreads, one, st>>>(lower, upper, d, p, part);
-    bound_apply_kernel<V><<<grid, kNormThreads, two, st>>>(lower, upper, given.gamma, given.beta, part, d, p, eps, act, out_l, out_u, sums);
-    return launch_status(2);
+    if (launch_status()) return LINF_ERR_LAUNCH;
+    return launch_behind(bound_apply_kernel<V>, grid, kNormThreads, two, st, lower, upper, given.gamma, given.beta, part, d, p, eps, act, out_l, out_u,
+                         sums);
 }
 
 template <int V>
@@ -582,9 +583,12 @@ int backward(const In4& in4, const NormGiven& given, const Sum4* sums, const Nor
         const size_t shared = bound_space<V>(p, 0).bytes;
         if (!allow_shared(bound_back_sums_kernel<V>, shared) || !allow_shared(bound_back_apply_kernel<V>, shared)) return LINF_ERR_LAUNCH;
         bound_back_sums_kernel<V><<<grid, kNormThreads, shared, st>>>(in4, given.gamma, given.beta, sums, d, p, eps, act, by_channel, by_group);
-        if (d_l != nullptr)
-            bound_back_apply_kernel<V><<<grid, kNormThreads, shared, st>>>(in4, given.gamma, given.beta, sums, by_group, d, p, eps, act, d_l, d_u);
-        if (launch_status(d_l != nullptr ? 2 : 1)) return LINF_ERR_LAUNCH;
+        if (launch_status()) return LINF_ERR_LAUNCH;
+        if (d_l != nullptr) {
+            const int rc = launch_behind(bound_back_apply_kernel<V>, grid, kNormThreads, shared, st, in4, given.gamma, given.beta, sums, by_group, d, p, eps,
+                                         act, d_l, d_u);
+            if (rc) return rc;
+        }
     }
     return dgamma != nullptr || dbeta != nullptr ? norm_params(by_channel, channel_rows(p), d.C, dgamma, dbeta, LINF_F32, st) : LINF_OK;
 }
