@@ -48,7 +48,7 @@ extern "C" {
 #define LINF_ERR_TOO_LARGE  7   /* size beyond a documented fixed maximum               */
 #define LINF_ERR_TYPE       8   /* unknown element type, or parameters of another one   */
 #define LINF_ERR_RATE       9   /* dropout rate outside [0, 1], or > 0 without a state  */
-#define LINF_ERR_EPS       10   /* eps is NaN, infinite or <= 0                         */
+#define LINF_ERR_EPS       10   /* eps is no positive normal fp32 number                */
 #define LINF_ERR_ACT       11   /* unknown activation                                   */
 
 /* Element types of the operators between two layers. */
@@ -386,8 +386,8 @@ int linf_dropout_next(long long* state, long long* used, void* stream);
  *   h = (x - mean) / sqrt(var + eps),   u = gamma[c] h + beta[c],   y = dropout(activation(u))
  * gamma, beta: [C] of param_type (fp32 or the type of x), each may be NULL (1 and 0).  rate > 0 drops elements of y under rng as
  * linf_dropout does, numbered as they lie in memory.  mean, rstd [N, G] (fp32) are kept for the backward pass, or both NULL.
- * fp32 inside whatever the type; one rounding at the end.  The workspace (16-byte aligned) has
- * linf_group_norm_workspace_bytes(...) bytes.  N * L * C may exceed 2^31.
+ * fp32 inside whatever the type; one rounding at the end.  The workspace (16-byte aligned; NULL where it is 0 bytes) has
+ * linf_group_norm_workspace_bytes(...) bytes.  N and L are 2^30 at most; N * L * C may exceed 2^31.
  */
 size_t linf_group_norm_workspace_bytes(int N, int C, int G, int L, int type, int backward);
 int linf_group_norm_forward(const void* x, const void* gamma, const void* beta, int N, int C, int G, int L, int type, int param_type,
@@ -403,7 +403,8 @@ int linf_group_norm_backward(const void* grad_output, const void* x, const void*
  * Bounds of a group norm with its activation over the box lower <= x <= upper, fp32, same layout: for every x in the box
  * output_lower <= activation(u) <= output_upper up to the rounding of the results.  The exact range of x_i - mean(x) is divided by
  * the range of the deviation, [max(0, std(c) - rho), std(c) + rho] with c the box's centre and rho the root mean square of
- * its radii.  sums [N, G, 4] (64 bits) is kept for the backward pass, or NULL.  Computed in 64 bits, rounded once.
+ * its radii.  sums [N, G, 4] (64 bits) is kept for the backward pass, or NULL.  Sums, and the whole backward pass, are computed in 64
+ * bits; the bounds themselves in fp32, off by no more than a few roundings of their own terms.
  */
 size_t linf_group_norm_bound_workspace_bytes(int N, int C, int G, int L, int backward);
 int linf_group_norm_bound_forward(const float* lower, const float* upper, const float* gamma, const float* beta, int N, int C, int G,

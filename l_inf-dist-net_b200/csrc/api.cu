@@ -99,7 +99,7 @@ namespace {
 inline bool bad_p(float p) { return !(p > 1.f) || isinf(p); }
 inline bool bad_type(int t) { return t != LINF_F32 && t != LINF_F16 && t != LINF_BF16; }
 inline bool bad_act(int a) { return a < LINF_ACT_IDENTITY || a > LINF_ACT_SILU; }
-inline bool bad_eps(double e) { return !(e > 0.f) || isinf(e); }
+inline bool bad_eps(double e) { return !(e >= 1.1754943508222875e-38 && e <= 3.4028234663852886e38); }     // a normal fp32 number
 inline bool bad_rate(double r, const long long* rng) { return !(r >= 0.0 && r <= 1.0) || (r > 0.0 && rng == nullptr); }
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 }  // namespace
@@ -122,7 +122,7 @@ const char* linf_error_string(int code) {
         case LINF_ERR_TOO_LARGE: return "size exceeds a fixed maximum of this entry point";
         case LINF_ERR_TYPE: return "element type is none of LINF_F32, LINF_F16, LINF_BF16, or parameters are neither fp32 nor of that type";
         case LINF_ERR_RATE: return "dropout rate must lie in [0, 1], and a rate above 0 needs a generator state";
-        case LINF_ERR_EPS: return "eps must be finite and greater than 0";
+        case LINF_ERR_EPS: return "eps must be a positive normal fp32 number";
         case LINF_ERR_ACT: return "unknown activation";
         default: return "unknown error code";
     }

@@ -194,7 +194,7 @@ inline void norm_two_passes(const NormDims& d, const NormKind& kind, bool aligne
 inline int norm_make(int N, int C, int G, int L, const NormKind& kind, bool aligned, NormDims* d, NormPlan* p) {
     if (N <= 0 || C <= 0 || G <= 0 || L <= 0) return LINF_ERR_DIMS;
     if (C % G != 0) return LINF_ERR_GROUP;
-    if (L > (1 << 30)) return LINF_ERR_TOO_LARGE;
+    if (N > (1 << 30) || L > (1 << 30)) return LINF_ERR_TOO_LARGE;
     d->N = N; d->C = C; d->G = G; d->L = L; d->Cg = C / G;
     d->inv_m = 1.0 / ((double)L * d->Cg);
     *p = NormPlan{};
@@ -276,7 +276,7 @@ __device__ __forceinline__ void keep_vector(T* to, const T* from) {
     else if (sizeof(T) * V == 4) cp_async4(to, from, 4);
     else *to = *from;
 }
-__device__ __forceinline__ void keep_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ void keep_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }      // a thread reads only what it copied itself
 
 template <int BYTES>
 __device__ __forceinline__ void copy_shared(unsigned to, const void* from) {

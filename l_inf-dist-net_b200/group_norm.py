@@ -153,12 +153,12 @@ def _check_sizes(shape, name, groups, eps, activation):
     groups, C, positions = int(groups), shape[1], math.prod(shape[2:])
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("the channel count must be a multiple of the group count")
-    if max(shape[0], C, positions) >= 2 ** 31:
-        raise RuntimeError(f"each size of {name} must be below 2^31")
+    if max(shape[0], positions) > 2 ** 30 or C >= 2 ** 31:
+        raise RuntimeError(f"{name} may have 2^30 samples, 2^30 positions and 2^31 - 1 channels at most")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {', '.join(ACTIVATIONS)}")
-    if not (math.isfinite(eps) and eps > 0):
-        raise ValueError("eps must be finite and greater than 0")
+    if not 1.1754943508222875e-38 <= eps <= 3.4028234663852886e38:
+        raise ValueError("eps must be a positive normal fp32 number")
     if len(_checked) >= 4096:
         _checked.clear()
     found = _checked[key] = ((shape[0], C, groups, positions), ACTIVATIONS[activation], float(eps))
@@ -218,7 +218,7 @@ def group_norm_bound(lower, upper, groups, weight=None, bias=None, eps=1e-5, act
 
     The exact range of x_i - mean(x) over the box is divided by a range of the deviation that the triangle inequality gives, so the
     bounds hold for the box as a whole and collapse to the value where lower = upper; nothing normalised exceeds sqrt(M - 1) in a
-    group of M.  Computed in 64 bits and rounded once, to nearest (as the bounds of the other layers are)."""
+    group of M.  The sums are 64-bit, the bounds fp32, rounded to nearest (as the bounds of the other layers are)."""
     if upper.shape != lower.shape or upper.dtype != lower.dtype or upper.device != lower.device:
         raise RuntimeError("upper must have the shape, dtype and device of lower")
     if lower.dtype != torch.float32:

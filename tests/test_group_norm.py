@@ -18,7 +18,9 @@ EPS = 1e-5
 # odd channel counts; groups of more vectors than a CTA has threads; one position; many positions; many samples
 SHAPES = [(1, 1, 1, (1,)), (2, 4, 4, ()), (3, 6, 3, ()), (5, 30, 3, (5, 7)), (2, 64, 8, (16, 16)), (3, 75, 5, (37,)), (2, 40, 4, (9, 9)),
           (2, 320, 32, (8, 8)), (1, 2048, 2048, (3,)), (7, 512, 16, ()), (3, 5120, 1, ()), (2, 8200, 1, (2,)), (2, 2666, 2, (3,)),
-          (1, 6144, 2, (5,)), (1, 16, 2, (150, 150)), (1, 3, 1, (101, 103)), (3000, 8, 2, ())]
+          (1, 6144, 2, (5,)), (1, 16, 2, (150, 150)), (1, 3, 1, (101, 103)), (3000, 8, 2, ()),
+          # rows too wide for a CTA's threads; small samples of which a CTA takes several; parts of the rows of several samples; one channel
+          (2, 20000, 1, ()), (5000, 32, 4, (3,)), (3, 48, 6, (60, 61)), (2, 1, 1, (200, 90))]
 
 
 def ids(s):
@@ -150,9 +152,9 @@ def _refused(fn, base, cases):
 def test_library_refuses(lib):
     p = ctypes.c_void_p(4096)          # never followed: each call is refused before a launch
     inf, nan = float("inf"), float("nan")
-    sizes = [(dict(N=0), 2), (dict(C=-4), 2), (dict(G=0), 2), (dict(L=0), 2), (dict(G=3), 3), (dict(L=(1 << 30) + 1), 7)]
+    sizes = [(dict(N=0), 2), (dict(C=-4), 2), (dict(G=0), 2), (dict(L=0), 2), (dict(G=3), 3), (dict(L=(1 << 30) + 1), 7), (dict(N=(1 << 30) + 1), 7)]
     common = sizes + [(dict(act=4), 11), (dict(act=-1), 11), (dict(L=1 << 20, ws=None), 6), (dict(L=1 << 20, ws=ctypes.c_void_p(4097)), 6), (dict(L=1 << 20, ws_bytes=8), 6)]
-    eps = [(dict(eps=0.0), 10), (dict(eps=-1.0), 10), (dict(eps=inf), 10), (dict(eps=nan), 10)]
+    eps = [(dict(eps=0.0), 10), (dict(eps=-1.0), 10), (dict(eps=1e-40), 10), (dict(eps=inf), 10), (dict(eps=nan), 10)]
     kinds = [(dict(type=3), 8), (dict(type=-1), 8), (dict(ptype=2), 8), (dict(rate=-1.0), 9), (dict(rate=nan), 9), (dict(rate=0.5), 9), (dict(rate=2.0), 9)]
     fwd = dict(x=p, w=p, b=p, N=2, C=8, G=2, L=4, type=0, ptype=0, eps=1e-5, act=0, rate=0.0, rng=None, y=p, mean=p, rstd=p, ws=p, ws_bytes=1 << 20, st=None)
     _refused(lib.linf_group_norm_forward, fwd, common + eps + kinds + [(dict(x=None), 1), (dict(y=None), 1), (dict(mean=None), 1)])
@@ -315,6 +317,43 @@ def test_same_bits_each_time(cuda, lib):
     runs = [check((4, 64, 8, (40, 40)), torch.bfloat16, "silu", 9) for _ in range(3)]
     for other in runs[1:]:
         assert all(torch.equal(a, e) for a, e in zip(runs[0], other))
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(7, 512, 16, ()), (3, 24, 4, (6, 5)), (1, 16, 2, (150, 150))], ids=ids)
+def test_parameters_off_a_boundary_and_twice_backward(cuda, lib, shape):
+    """A weight and a bias that lie off a 16-byte boundary; a graph that is gone through twice; a call without gradients."""
+    x, w, b, g = make(shape, torch.float32, 12)
+    xd = last(x).requires_grad_()
+    off = torch.zeros(2, shape[1] + 1, device="cuda")
+    off[0, 1:], off[1, 1:] = w.cuda(), b.cuda()
+    wo, bo = (off[k, 1:].detach().requires_grad_() for k in range(2))
+    wd, bd = w.cuda().requires_grad_(), b.cuda().requires_grad_()
+    assert wo.data_ptr() % 16 != 0 or bo.data_ptr() % 16 != 0
+    y, want = (L.group_norm(xd, shape[2], *p, activation="silu") for p in ((wo, bo), (wd, bd)))
+    first = torch.autograd.grad(y, (xd, wo, bo), last(g), retain_graph=True)
+    again = torch.autograd.grad(y, (xd, wo, bo), last(g))
+    assert torch.equal(y, want)
+    for a, e, f in zip(first, again, torch.autograd.grad(want, (xd, wd, bd), last(g))):
+        assert torch.equal(a, e) and torch.equal(a, f)
+    with torch.no_grad():
+        assert torch.equal(L.group_norm(xd, shape[2], wo, bo, activation="silu"), y)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(7, 64, 4, ()), (3, 24, 4, (6, 5)), (1, 16, 2, (150, 150))], ids=ids)
+def test_dropped_values_are_zero_whatever_they_were(cuda, lib, shape):
+    """Infinities make their group's values NaN; dropped ones among them are 0, in the value and in the gradient that reaches dy."""
+    x, w, b, g = make(shape, torch.float32, 13)
+    x[0, 0] = float("inf")
+    rng = torch.tensor([9, 1], dtype=torch.int64, device="cuda")
+    y = L.group_norm(last(x), shape[2], w.cuda(), b.cuda(), rate=0.5, rng=rng).cpu()
+    kept = numbered(x.shape, 9, 1, 0.5) != 0
+    group = torch.zeros(x.shape, dtype=torch.bool)
+    group[0, :shape[1] // shape[2]] = True
+    assert not y[~kept].any() and torch.isnan(y[kept & group]).all() and torch.isfinite(y[~group]).all()
+    none = L.group_norm(last(x), shape[2], rate=1.0, rng=rng)
+    assert not none.any()
 
 
 @gpu
