@@ -665,13 +665,16 @@ size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back) {
     switch (type) {                                                                                                \
         case LINF_F32:                                                                                             \
             if (p.V == 4) return CALL32(float, 4);                                                                 \
+            if (p.V == 2) return CALL32(float, 2);                                                                 \
             return CALL32(float, 1);                                                                               \
         case LINF_F16:                                                                                             \
             if (p.V == 8) return CALL16(__half, 8);                                                                \
+            if (p.V == 4) return CALL16(__half, 4);                                                                \
             if (p.V == 2) return CALL16(__half, 2);                                                                \
             return CALL16(__half, 1);                                                                              \
         default:                                                                                                   \
             if (p.V == 8) return CALL16(__nv_bfloat16, 8);                                                         \
+            if (p.V == 4) return CALL16(__nv_bfloat16, 4);                                                         \
             if (p.V == 2) return CALL16(__nv_bfloat16, 2);                                                         \
             return CALL16(__nv_bfloat16, 1);                                                                       \
     }

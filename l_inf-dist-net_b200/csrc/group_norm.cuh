@@ -93,11 +93,11 @@ constexpr int kNormPlaces = 4;            // CTAs of the two passes that an SM h
 
 inline int norm_ceil(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// widest vector of {16 bytes, 4 bytes, one element} that the call allows, and the least number of groups whose channels make whole
+// widest vector of {16, 8, 4 bytes, one element} that the call allows, and the least number of groups whose channels make whole
 // vectors; `cap`: vectors along the channels of a CTA.  One group may be wider than `cap`: *kmin = 0 then (it has to be cut).
 inline int norm_vector(const NormDims& d, int elem_bytes, bool aligned, int cap, int* kmin) {
-    const int widths[3] = {16 / elem_bytes, 4 / elem_bytes, 1};
-    for (int k = 0; k < 3; ++k) {
+    const int widths[4] = {16 / elem_bytes, 8 / elem_bytes, 4 / elem_bytes, 1};
+    for (int k = 0; k < 4; ++k) {
         const int V = widths[k];
         if (V > 1 && (!aligned || d.C % V != 0)) continue;
         int a = d.Cg, b = V;
@@ -269,25 +269,27 @@ __device__ __forceinline__ void by_columns(int width, int rows, Body body) {
     }
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_shared(unsigned to, const void* from) {
+    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else if (BYTES == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
 // One vector of a kept row from global to shared memory, asynchronously where its size allows.
 template <typename T, int V>
 __device__ __forceinline__ void keep_vector(T* to, const T* from) {
-    if (sizeof(T) * V == 16) cp_async16(to, from, 16);
-    else if (sizeof(T) * V == 4) cp_async4(to, from, 4);
+    constexpr int bytes = sizeof(T) * V;
+    if constexpr (bytes >= 4) copy_shared<bytes>((unsigned)__cvta_generic_to_shared(to), from);
     else *to = *from;
 }
 __device__ __forceinline__ void keep_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }      // a thread reads only what it copied itself
 
-template <int BYTES>
-__device__ __forceinline__ void copy_shared(unsigned to, const void* from) {
-    if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
-    else asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
-}
 template <typename T, int V>
 __device__ __forceinline__ Raw<T, V> load_shared(unsigned at) {
     Raw<T, V> v;
     if constexpr (sizeof(T) * V == 16) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+    else if constexpr (sizeof(T) * V == 8) asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    else asm volatile("ld.shared.b32 %0, [%1];" : "=r"(*reinterpret_cast<unsigned*>(&v)) : "r"(at) : "memory");
     return v;
 }
 

@@ -619,7 +619,8 @@ int group_norm_bound_forward(const float* lower, const float* upper, const float
     if (!norm_given(gamma, beta, LINF_F32, &given)) return LINF_ERR_LAUNCH;
     Sum4* s = reinterpret_cast<Sum4*>(sums);
     return p.V == 4 ? forward<4>(lower, upper, given, d, p, eps, act, out_l, out_u, s, ws, st)
-                    : forward<1>(lower, upper, given, d, p, eps, act, out_l, out_u, s, ws, st);
+           : p.V == 2 ? forward<2>(lower, upper, given, d, p, eps, act, out_l, out_u, s, ws, st)
+                      : forward<1>(lower, upper, given, d, p, eps, act, out_l, out_u, s, ws, st);
 }
 
 int group_norm_bound_backward(const float* g_l, const float* g_u, const float* lower, const float* upper, const float* gamma, const float* beta,
@@ -637,7 +638,8 @@ int group_norm_bound_backward(const float* g_l, const float* g_u, const float* l
     const Sum4* s = reinterpret_cast<const Sum4*>(sums);
     const In4 in4 = {g_l, g_u, lower, upper};
     return p.V == 4 ? backward<4>(in4, given, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st)
-                    : backward<1>(in4, given, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st);
+           : p.V == 2 ? backward<2>(in4, given, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st)
+                      : backward<1>(in4, given, s, d, p, eps, act, d_l, d_u, dgamma, dbeta, ws, st);
 }
 
 }  // namespace linf

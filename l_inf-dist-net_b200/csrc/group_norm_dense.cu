@@ -198,8 +198,8 @@ template <int V> struct DenseK { static constexpr int value = V == 8 ? 2 : 4; };
 // Whether a slot can hold a row; its plan.  ctas: CTAs that the call should have at least, as far as there are samples.
 bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, DensePlan* p) {
     if (d.L != 1) return false;
-    const int widths[3] = {16 / elem_bytes, 4 / elem_bytes, 1};
-    for (int k = 0; k < 3; ++k) {
+    const int widths[4] = {16 / elem_bytes, 8 / elem_bytes, 4 / elem_bytes, 1};
+    for (int k = 0; k < 4; ++k) {
         const int V = widths[k];
         if (V > 1 && (!aligned || d.Cg % V != 0)) continue;
         p->V = V;
@@ -226,13 +226,16 @@ bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, Dense
     switch (type) {                                                                   \
         case LINF_F32:                                                                \
             if (p.V == 4) return CALL(float, 4);                                      \
+            if (p.V == 2) return CALL(float, 2);                                      \
             return CALL(float, 1);                                                    \
         case LINF_F16:                                                                \
             if (p.V == 8) return CALL(__half, 8);                                     \
+            if (p.V == 4) return CALL(__half, 4);                                     \
             if (p.V == 2) return CALL(__half, 2);                                     \
             return CALL(__half, 1);                                                   \
         default:                                                                      \
             if (p.V == 8) return CALL(__nv_bfloat16, 8);                              \
+            if (p.V == 4) return CALL(__nv_bfloat16, 4);                              \
             if (p.V == 2) return CALL(__nv_bfloat16, 2);                              \
             return CALL(__nv_bfloat16, 1);                                            \
     }

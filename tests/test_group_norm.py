@@ -20,7 +20,9 @@ SHAPES = [(1, 1, 1, (1,)), (2, 4, 4, ()), (3, 6, 3, ()), (5, 30, 3, (5, 7)), (2,
           (2, 320, 32, (8, 8)), (1, 2048, 2048, (3,)), (7, 512, 16, ()), (3, 5120, 1, ()), (2, 8200, 1, (2,)), (2, 2666, 2, (3,)),
           (1, 6144, 2, (5,)), (1, 16, 2, (150, 150)), (1, 3, 1, (101, 103)), (3000, 8, 2, ()),
           # rows too wide for a CTA's threads; small samples of which a CTA takes several; parts of the rows of several samples; one channel
-          (2, 20000, 1, ()), (5000, 32, 4, (3,)), (3, 48, 6, (60, 61)), (2, 1, 1, (200, 90))]
+          (2, 20000, 1, ()), (5000, 32, 4, (3,)), (3, 48, 6, (60, 61)), (2, 1, 1, (200, 90)),
+          # vectors of 8 and 4 bytes
+          (2, 36, 3, (9, 5)), (1, 20, 2, (70, 90)), (6, 44, 2, ()), (1, 18, 1, (80, 90)), (2, 22, 11, (7,))]
 
 
 def ids(s):
