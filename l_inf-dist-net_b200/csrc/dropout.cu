@@ -2,7 +2,8 @@
 // element number) and never stored.  The backward pass of dropout is dropout of the gradient under the same (seed, offset).
 //
 // Bound by HBM: each value is read once and written once.  A thread takes the 8 elements of one generator block, so the
-// generator's seven rounds are paid once for 8 elements (and once for the 24 of a triple).
+// generator's seven rounds are paid once for 8 elements (and once for the 24 of a triple).  Measured on one B200: 64 x 256 x 64 x 64 bf16, value and
+// gradient, 98 us, 5.5 TB/s (135 us with a multiplication by a kept scale or 0 for each tensor instead of one selection).
 #include "vec.cuh"
 
 namespace linf {

@@ -4,11 +4,18 @@
 //   dbeta = sum du, dgamma = sum du h (over samples and positions),
 //   dx = (gamma du - mean(gamma du) - h mean(gamma du h)) / sqrt(var + eps)
 //
-// Bound by HBM: every tensor once in or out (16-bit types come near the issue limit as well).  The sums of the kept form are a mean and a
+// What bounds it: kept and dense slabs the latency of load, reduction and store; two passes the instructions (a bf16 value with silu takes 12 to
+// 15, with dropout 25; 2.0 to 2.4 a clock are issued) before HBM, which sees x once or twice.  Measured on one B200, us: 32 x 320 x 64 x 64 bf16,
+// 32 groups, silu: 58 (sums 23, results 38 with what is left in L2; 26 if x and y crossed HBM once); 16 x 128 x 160 x 160 bf16, silu and dropout:
+// forward 83, backward 138; 64 x 128 x 16 x 16 fp32, tanh, kept: forward 11, backward 18.  Clusters of up to 8 CTAs that held larger slabs in
+// their shared memory read x once, but loaded, reduced and stored in turn: 65 for the first, and 528 instead of 221 for the second, whose rows
+// they had to cut into pieces of 32 bytes.
+//
+// The sums of the kept form are a mean and a
 // sum of squared deviations (of a thread's values, of a column's, of a group's), joined by
 //   mean = sum n_i mean_i / n,  M2 = sum M2_i + sum n_i (mean_i - mean)^2;
-// row ranges of the two passes are joined as sums of x and x^2 in 64 bits: so data far from 0 against their spread (activations of distance layers are all
-// positive) lose nothing of their variance.  The order of every addition is fixed by the shape alone.
+// the CTAs of the two passes join theirs as sums of x and x^2 in 64 bits.  So data far from 0 against their spread (activations of distance
+// layers are all positive) lose nothing of their variance.  The order of every addition is fixed by the shape alone.
 #include "group_norm.cuh"
 
 namespace linf {
@@ -221,12 +228,12 @@ norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __res
     });
 }
 
-// The two sums of a group over its row ranges and pieces, in all lanes.
+// The two sums of a group over the CTAs that share its rows and over its pieces, in all lanes.
 __device__ __forceinline__ double2 add_parts(const double2* part, const NormDims& d, const NormPlan& p, int n, int g) {
     double a = 0.0, e = 0.0;
     for (int k = threadIdx.x & 31; k < p.splits * p.pieces; k += 32) {
         const int s = k / p.pieces, piece = k - s * p.pieces;
-        const double2 v = part[(((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece];
+        const double2 v = __ldcg(part + (((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece);
         a += v.x;
         e += v.y;
     }
@@ -373,7 +380,7 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
     T* data = reinterpret_cast<T*>(space);
     float2* red = space_at<float2>(space, sp.red);
     float2* stat = space_at<float2>(space, sp.stat);
-    unsigned char* kept = space_at<unsigned char>(space, sp.mask) ;
+    unsigned char* kept = space_at<unsigned char>(space, sp.mask);
     const int chunk = p.by_blocks(blockIdx.x);
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - chunk * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
@@ -550,7 +557,7 @@ norm_params_kernel(const float2* __restrict__ by_channel, long long count, int C
     if (c < C) {
 #pragma unroll 4
         for (long long k = lane; k < count; k += 32) {
-            const float2 v = __ldg(by_channel + k * C + c);
+            const float2 v = __ldcg(by_channel + k * C + c);
             a += v.x;
             e += v.y;
         }

@@ -9,7 +9,9 @@
 //
 // Sums, and all of the backward pass, are computed in 64 bits: which of two ends a bound takes, and with it a gradient, is decided next to
 // 0.  The elements of the forward pass, whose values do not jump there, are fp32, with the means in two parts, so that no bound is off by more
-// than a few roundings of its own terms.  Forward passes are bound by HBM, backward passes by the 64-bit units.
+// than a few roundings of its own terms.  Forward passes are bound by HBM, backward passes by
+// the 64-bit units.  Measured on one B200, us: 32 x 192 x 56 x 56, relu, forward 95 (elements in 64 bits: 119; 47 if all crossed HBM once); 16 x 192 x
+// 56 x 56, tanh, both directions 236; 512 x 512, 16 groups, tanh, both 27.
 #include "group_norm.cuh"
 
 namespace linf {
@@ -283,12 +285,14 @@ bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upp
     group_sums(red4, d, p, b, [&](int g, const Sum4& s) { part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = s; });
 }
 
-// The sums of a group over its row ranges and pieces, in all lanes.
+// The sums of a group over the CTAs that share its rows and over its pieces, in all lanes.
 __device__ __forceinline__ Sum4 all_parts(const Sum4* part, const NormDims& d, const NormPlan& p, int n, int g) {
     Sum4 t = {0.0, 0.0, 0.0, 0.0};
     for (int k = threadIdx.x & 31; k < p.splits * p.pieces; k += 32) {
         const int s = k / p.pieces, piece = k - s * p.pieces;
-        t = add4(t, part[(((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece]);
+        const double2* v = reinterpret_cast<const double2*>(part + (((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece);
+        const double2 a = __ldcg(v), e = __ldcg(v + 1);
+        t = add4(t, Sum4{a.x, a.y, e.x, e.y});
     }
     return warp_sum4(t);
 }
