@@ -547,25 +547,37 @@ norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
     });
 }
 
-// dgamma, dbeta: the rows of per-channel sums in 64 bits, 8 channels to a CTA (a row's piece is two sectors) and 32 rows at a time
-__global__ void __launch_bounds__(256)
+// dgamma, dbeta: the rows of per-channel sums in 64 bits, 8 channels to a CTA (a row's piece is two sectors).  A thread has 8 rows on their way
+// at a time: with few CTAs the time is the latency of its loads.
+constexpr int kParamThreads = 512, kParamRows = kParamThreads / 8, kParamLoads = 8;
+__global__ void __launch_bounds__(kParamThreads)
 norm_params_kernel(const float2* __restrict__ by_channel, long long count, int C, void* __restrict__ dgamma, void* __restrict__ dbeta, int ptype) {
-    __shared__ double2 red[32][8];
+    __shared__ double2 red[kParamThreads / 32][8];
     const int col = threadIdx.x & 7, lane = threadIdx.x >> 3, c = blockIdx.x * 8 + col;
     double a = 0.0, e = 0.0;
     grid_wait();
     if (c < C) {
-#pragma unroll 4
-        for (long long k = lane; k < count; k += 32) {
-            const float2 v = __ldcg(by_channel + k * C + c);
-            a += v.x;
-            e += v.y;
+        for (long long k0 = lane; k0 < count; k0 += kParamRows * kParamLoads) {
+            float2 v[kParamLoads];
+#pragma unroll
+            for (int u = 0; u < kParamLoads; ++u) {
+                const long long k = k0 + u * kParamRows;
+                v[u] = k < count ? __ldcg(by_channel + k * C + c) : make_float2(0.f, 0.f);
+            }
+#pragma unroll
+            for (int u = 0; u < kParamLoads; ++u) { a += v[u].x; e += v[u].y; }
         }
     }
-    red[lane][col] = make_double2(a, e);
+#pragma unroll
+    for (int o = 8; o < 32; o *= 2) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        e += __shfl_xor_sync(0xffffffffu, e, o);
+    }
+    if ((threadIdx.x & 31) < 8) red[threadIdx.x >> 5][col] = make_double2(a, e);
     __syncthreads();
     if (threadIdx.x >= 8 || c >= C) return;
-    for (int k = 1; k < 32; ++k) { a += red[k][col].x; e += red[k][col].y; }
+#pragma unroll
+    for (int k = 1; k < kParamThreads / 32; ++k) { a += red[k][col].x; e += red[k][col].y; }
     if (dbeta != nullptr) store_param(dbeta, c, ptype, (float)a);
     if (dgamma != nullptr) store_param(dgamma, c, ptype, (float)e);
 }
@@ -650,7 +662,7 @@ bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g) {
 }
 
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st) {
-    return launch_behind(norm_params_kernel, dim3((C + 7) / 8), 256, 0, st, by_channel, count, C, dgamma, dbeta, ptype);
+    return launch_behind(norm_params_kernel, dim3((C + 7) / 8), kParamThreads, 0, st, by_channel, count, C, dgamma, dbeta, ptype);
 }
 
 size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back) {
