@@ -6,6 +6,7 @@ place is the head behind the distance layers, and a certificate takes its bounds
 zbh2047/L_inf-dist-net has no counterpart.  Kernels: csrc/group_norm.cu, csrc/group_norm_bound.cu.
 """
 import math
+import operator
 
 import torch
 import torch.nn as nn
@@ -144,13 +145,14 @@ _checked = {}
 
 def _check_sizes(shape, name, groups, eps, activation):
     """(sizes, activation's number, eps) of a call; what was found once for a shape is kept."""
+    groups, eps = operator.index(groups), float(eps)
     key = (shape, groups, eps, activation)
     found = _checked.get(key)
     if found is not None:
         return found
     if len(shape) < 2:
         raise RuntimeError(f"{name} must be [N, C, ...]")
-    groups, C, positions = int(groups), shape[1], math.prod(shape[2:])
+    C, positions = shape[1], math.prod(shape[2:])
     if groups < 1 or C < 1 or C % groups != 0:
         raise ValueError("the channel count must be a multiple of the group count")
     if max(shape[0], positions) > 2 ** 30 or C >= 2 ** 31:
@@ -161,7 +163,7 @@ def _check_sizes(shape, name, groups, eps, activation):
         raise ValueError("eps must be a positive normal fp32 number")
     if len(_checked) >= 4096:
         _checked.clear()
-    found = _checked[key] = ((shape[0], C, groups, positions), ACTIVATIONS[activation], float(eps))
+    found = _checked[key] = ((shape[0], C, groups, positions), ACTIVATIONS[activation], eps)
     return found
 
 
@@ -235,6 +237,7 @@ class BoundGroupNorm(_Masks):
 
     def __init__(self, groups, channels, eps=1e-5, affine=True, activation="identity", dropout=0.0, seed=None):
         super().__init__()
+        groups = operator.index(groups)
         if groups < 1 or channels % groups != 0:
             raise ValueError("the channel count must be a multiple of the group count")
         if activation not in ACTIVATIONS:

@@ -180,6 +180,10 @@ def test_python_refuses_on_the_host():
                dict(rate=0.5, rng=torch.zeros(2)), dict(weight=w.half())):
         with pytest.raises(RuntimeError, match="weight|bias|rng"):
             L.group_norm(x, 2, **kw)
+    with pytest.raises(TypeError):
+        L.group_norm(torch.zeros(2, 5), 2.5)
+    with pytest.raises(TypeError):
+        L.BoundGroupNorm(2.5, 5)
     with pytest.raises(RuntimeError, match="N, C"):
         L.group_norm(torch.zeros(4), 2)
     with pytest.raises(RuntimeError, match="CUDA"):
