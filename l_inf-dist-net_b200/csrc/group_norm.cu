@@ -7,8 +7,8 @@
 // What bounds it: kept and dense slabs the latency of load, reduction and store; two passes the instructions (a bf16 value with silu takes 12 to
 // 15, with dropout 25; 2.0 to 2.4 a clock are issued) before HBM, which sees x once or twice.  Measured on one B200, us: 32 x 320 x 64 x 64 bf16,
 // 32 groups, silu: 58 (sums 23, results 38 with what is left in L2; 26 if x and y crossed HBM once); 16 x 128 x 160 x 160 bf16, silu and dropout:
-// forward 83, backward 138; 64 x 128 x 16 x 16 fp32, tanh, kept: forward 11, backward 18.  Clusters of up to 8 CTAs that held larger slabs in
-// their shared memory read x once, but loaded, reduced and stored in turn: 65 for the first, and 528 instead of 221 for the second, whose rows
+// forward 83, backward 133; 64 x 128 x 16 x 16 fp32, tanh, kept: forward 11, backward 18.  Clusters of up to 8 CTAs that held larger slabs in
+// their shared memory read x once, but loaded, reduced and stored in turn: 65 for the first, and 528 instead of 216 for the second, whose rows
 // they had to cut into pieces of 32 bytes.
 //
 // The sums of the kept form are a mean and a

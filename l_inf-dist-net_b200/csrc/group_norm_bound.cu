@@ -11,7 +11,7 @@
 // 0.  The elements of the forward pass, whose values do not jump there, are fp32, with the means in two parts, so that no bound is off by more
 // than a few roundings of its own terms.  Forward passes are bound by HBM, backward passes by
 // the 64-bit units.  Measured on one B200, us: 32 x 192 x 56 x 56, relu, forward 95 (elements in 64 bits: 119; 47 if all crossed HBM once); 16 x 192 x
-// 56 x 56, tanh, both directions 236; 512 x 512, 16 groups, tanh, both 27.
+// 56 x 56, tanh, both directions 231; 512 x 512, 16 groups, tanh, both 24.
 #include "group_norm.cuh"
 
 namespace linf {
