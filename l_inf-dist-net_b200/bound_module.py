@@ -126,7 +126,7 @@ class Predictor(nn.Module):
         self.fc1 = BoundLinear(in_features, hidden, bias=True)
         if groups is None:
             self.tanh = BoundTanh()
-            self.drop = BoundDropout(dropout) if dropout > 0 else None
+            self.drop = BoundDropout(dropout) if dropout != 0 else None
         else:
             self.norm = BoundGroupNorm(groups, hidden, activation="tanh", dropout=dropout)
         self.groups = groups

@@ -159,7 +159,7 @@ __device__ __forceinline__ Ends32 make_ends32(const Sum4& s, const NormDims& d, 
     return e;
 }
 // ... and of the channels of a thread's column
-template <int V> struct BoundColumn { Ends32 e[V]; float w[V], o[V], inv_m, cut; };
+template <int V> struct BoundColumn { Ends32 e[V]; float w[V], o[V], inv_m2, cut; };
 template <int V>
 __device__ __forceinline__ void load_column(BoundColumn<V>& k, const Ends32* ends, const Param& gamma, const Param& beta, const NormDims& d,
                                             const NormPlan& p, const NormBlock& b, int c) {
@@ -169,7 +169,7 @@ __device__ __forceinline__ void load_column(BoundColumn<V>& k, const Ends32* end
     load_params<V>(beta, b.c0 + c, k.o);
 #pragma unroll
     for (int j = 0; j < V; ++j) k.e[j] = ends[g[j]];
-    k.inv_m = (float)d.inv_m;
+    k.inv_m2 = 2.f * (float)d.inv_m;
     k.cut = sqrtf((float)((double)d.L * d.Cg - 1.0));
 }
 
@@ -182,7 +182,7 @@ __device__ __forceinline__ void write_bounds(const Raw<float, V>& lv, const Raw<
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const Ends32& e = k.e[j];
-        const float own = (u[j] - l[j]) * k.inv_m;
+        const float own = fmaf(u[j], 0.5f, -0.5f * l[j]) * k.inv_m2;      // the width halved: it may be beyond fp32
         const float n0 = ((l[j] - e.mu) - e.mu2) + own, n1 = ((u[j] - e.ml) - e.ml2) - own;
         float z0 = n0 * (n0 >= 0.f ? e.s_lo : e.s_hi), z1 = n1 * (n1 >= 0.f ? e.s_hi : e.s_lo);
         z0 = z0 <= -k.cut ? -k.cut : z0;                        // a NaN stays

@@ -248,6 +248,8 @@ class BoundGroupNorm(_Masks):
         self._make_masks(dropout, seed)
 
     def forward(self, x, lower=None, upper=None):
+        if x.size(1) != self.channels:
+            raise RuntimeError(f"the input must have {self.channels} channels")
         args = (self.groups, self.weight, self.bias, self.eps, self.activation)
         rate = self.rate if self.training else 0.0
         used = dropout_next(self.rng) if rate > 0 else None

@@ -197,6 +197,12 @@ def test_python_refuses_on_the_host():
     for bad in (dict(groups=3, channels=8), dict(groups=2, channels=8, activation="gelu"), dict(groups=2, channels=8, dropout=2.0)):
         with pytest.raises(ValueError):
             L.BoundGroupNorm(**bad)
+    for rate in (-0.1, float("nan"), 1.5):
+        for groups in (None, 2):
+            with pytest.raises(ValueError):
+                L.Predictor(6, 8, 3, groups=groups, dropout=rate)
+    with pytest.raises(RuntimeError, match="16 channels"):
+        L.BoundGroupNorm(2, 16, affine=False)(x)
 
 
 def test_modules_state_on_the_host():
@@ -579,6 +585,18 @@ def test_bounds_off_a_boundary_and_not_finite(cuda, lib):
 
 
 # ---- as a user has them together ------------------------------------------------------------------------------------------
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(7, 64, 4, ()), (3, 24, 4, (6, 5)), (1, 16, 2, (150, 150))], ids=ids)
+def test_boxes_wider_than_their_type(cuda, lib, shape):
+    """Boxes whose width leaves fp32: every normalised value is possible, so the bounds are -+sqrt(M - 1), where they are cut."""
+    n, c, groups, space = shape
+    l = last(torch.full((n, c, *space), -3e38))
+    lo, up = L.group_norm_bound(l, -l, groups)
+    m = c // groups * math.prod(space)
+    # the root is rounded once, from M - 1 < 2^24
+    assert torch.allclose(up, torch.full_like(up, math.sqrt(m - 1)), rtol=2.0 ** -23, atol=0) and torch.equal(lo, -up)
 
 
 @gpu
