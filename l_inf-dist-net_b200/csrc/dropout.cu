@@ -95,7 +95,7 @@ int launch(const Tensors& t, int tensors, long long n, const Drop& d, cudaStream
 
 int dropout(const void* const* in, void* const* out, int tensors, long long n, int type, double rate, const long long* rng, cudaStream_t st) {
     Drop d;
-    if (!make_drop(rate, rng, &d)) return LINF_ERR_RATE;
+    if (!make_drop(rate, rng, nullptr, &d)) return LINF_ERR_RATE;
     if (!d.on) {                                     // nothing is dropped: every element as it is, a NaN's bits included
         for (int k = 0; k < tensors; ++k)
             if (out[k] != in[k] &&

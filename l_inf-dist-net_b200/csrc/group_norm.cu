@@ -21,9 +21,9 @@
 namespace linf {
 namespace {
 
-// The values that stand for a gamma or beta that was not given.
-struct Own { float one, zero; };
-__device__ Own g_own = {1.f, 0.f};
+// The values that stand for a gamma or beta that was not given, and for the state of a generator that nothing is drawn from.
+struct Own { float one, zero; long long rng[2]; };
+__device__ Own g_own = {1.f, 0.f, {0, 0}};
 
 // What a thread's column needs for u = (x + m) a + o: m is the mean with its sign turned.
 template <int V> struct Column { Lanes<V> m, a, o; };
@@ -658,6 +658,7 @@ bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g) {
     };
     g->gamma = given(gamma, &own->one);
     g->beta = given(beta, &own->zero);
+    g->idle = own->rng;
     return true;
 }
 
@@ -702,8 +703,6 @@ int group_norm_forward(const void* x, const void* gamma, const void* beta, int N
                        double rate, const long long* rng, void* y, float* mean, float* rstd, void* ws, size_t ws_bytes, cudaStream_t st) {
     NormDims d;
     NormPlan p;
-    Drop drop;
-    if (!make_drop(rate, rng, &drop)) return LINF_ERR_RATE;
     const int rc = norm_make(N, C, G, L, forward_kind(type), aligned16(x) && aligned16(y), &d, &p);
     if (rc) return rc;
     DensePlan dp;
@@ -712,6 +711,8 @@ int group_norm_forward(const void* x, const void* gamma, const void* beta, int N
     if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need)) return LINF_ERR_WORKSPACE;
     NormGiven given;
     if (!norm_given(gamma, beta, ptype, &given)) return LINF_ERR_LAUNCH;
+    Drop drop;
+    if (!make_drop(rate, rng, given.idle, &drop)) return LINF_ERR_RATE;
     if (dense) return dense_norm_forward(x, given, d, dp, type, eps, act, drop, y, mean, rstd, st);
 #define LINF_CALL(T, V) forward<T, V>(static_cast<const T*>(x), given, d, p, eps, act, drop, static_cast<T*>(y), mean, rstd, ws, st)
     LINF_BY_VECTOR(LINF_CALL, LINF_CALL)
@@ -723,8 +724,6 @@ int group_norm_backward(const void* dy, const void* x, const void* gamma, const 
                         void* ws, size_t ws_bytes, cudaStream_t st) {
     NormDims d;
     NormPlan p;
-    Drop drop;
-    if (!make_drop(rate, rng, &drop)) return LINF_ERR_RATE;
     const int rc = norm_make(N, C, G, L, backward_kind(type), aligned16(x) && aligned16(dy) && aligned16(dx), &d, &p);
     if (rc) return rc;
     DensePlan dp;
@@ -732,6 +731,8 @@ int group_norm_backward(const void* dy, const void* x, const void* gamma, const 
     if (ws == nullptr || !aligned16(ws) || ws_bytes < (dense ? dense_workspace(d, dp) : workspace(d, p, true))) return LINF_ERR_WORKSPACE;
     NormGiven given;
     if (!norm_given(gamma, beta, ptype, &given)) return LINF_ERR_LAUNCH;
+    Drop drop;
+    if (!make_drop(rate, rng, given.idle, &drop)) return LINF_ERR_RATE;
     if (dense) {
         float2* by_channel = static_cast<float2*>(ws);
         const int done = dense_norm_backward(dy, x, given, mean, rstd, d, dp, type, act, drop, dx, by_channel, st);

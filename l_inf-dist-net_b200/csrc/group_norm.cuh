@@ -224,8 +224,9 @@ int dense_norm_backward(const void* dy, const void* x, const NormGiven& given, c
 // dgamma and dbeta from `count` rows of per-channel sums (du, du h); either may be null (group_norm.cu)
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st);
 
-// gamma and beta, or what stands for them where they are null, on the current device; false if CUDA refused (group_norm.cu)
-struct NormGiven { Param gamma, beta; };
+// gamma and beta, or what stands for them where they are null, and a generator state that stands for one that is not needed, on the
+// current device; false if CUDA refused (group_norm.cu)
+struct NormGiven { Param gamma, beta; const long long* idle; };
 bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g);
 
 template <typename X> __device__ __forceinline__ X* space_at(uint4* space, size_t at) { return reinterpret_cast<X*>(reinterpret_cast<char*>(space) + at); }

@@ -248,7 +248,7 @@ __device__ __forceinline__ float slope(float u, int act) { return slope<true, 1>
 // makes up for the rounded rate, so that the expectation is exact.  With 32 bits and 10 rounds a pass over 64 Mi bf16 values took 72 us
 // for the integer multiplications alone, with 16 bits 49 us, without a generator 44 us.
 struct Drop {
-    const long long* rng;       // {seed, offset} on the device
+    const long long* rng;       // {seed, offset} on the device; never null, dropout or none
     int on;                     // 0: no dropout
     unsigned limit;             // threshold * 2^16 - 1: a piece in the upper half of a word, lower half whatever it is, is kept iff word > limit
     float scale;
@@ -325,14 +325,16 @@ __device__ __forceinline__ Lanes<V> drop(const Drop& d, const DropKey& k, unsign
     return lanes<V>(f);
 }
 
-// threshold and scale of a rate in [0, 1]; false outside (a NaN included).  Rate 1 keeps nothing.
-inline bool make_drop(double rate, const long long* rng, Drop* d) {
+// threshold and scale of a rate in [0, 1]; false outside (a NaN included).  Rate 1 keeps nothing.  Where nothing is dropped the kernels hold
+// `idle` (two words on the device) in the place of rng, which may be null then: as with PARAM_ONE, no kernel holds a pointer that it must not
+// follow, wherever the compiler moves the load to.
+inline bool make_drop(double rate, const long long* rng, const long long* idle, Drop* d) {
     if (!(rate >= 0.0 && rate <= 1.0)) return false;
     const unsigned threshold = (unsigned)(rate * 65536.0 + 0.5);
     d->limit = threshold * 65536u - 1u;             // 65536 * 65536 wraps around to 0: no word is above the limit
     d->scale = threshold < 65536u ? (float)(65536.0 / (65536.0 - (double)threshold)) : 0.f;
-    d->rng = rng;
     d->on = threshold > 0;                          // a threshold of 0 keeps every element as it is
+    d->rng = d->on ? rng : idle;
     return true;
 }
 

@@ -1,0 +1,45 @@
+"""Host-side decisions of the group-norm and dropout kernels, called as they are from a small program: no GPU needed."""
+import os
+import subprocess
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "l_inf-dist-net_b200", "csrc")
+
+PROGRAM = r"""
+#include <cstdio>
+#include <cstdlib>
+#include <cstring>
+#include "group_norm.cuh"
+namespace linf { int sm_count() { return 148; } std::atomic<unsigned long long> g_launches{0}; }
+using namespace linf;
+int main(int argc, char** argv) {
+    if (!strcmp(argv[1], "drop")) {                 // rate, whether a state is given -> on, which pointer
+        static const long long idle[2] = {0, 0}, rng[2] = {1, 2};
+        Drop d;
+        if (!make_drop(atof(argv[2]), atoi(argv[3]) ? rng : nullptr, idle, &d)) return printf("refused"), 0;
+        printf("%d %s", d.on, d.rng == rng ? "rng" : d.rng == idle ? "idle" : "null");
+    }
+    return 0;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def ask(tmp_path_factory):
+    """ask("what", ...) -> what the program prints."""
+    at = tmp_path_factory.mktemp("plans")
+    source, program = at / "plans.cu", at / "plans"
+    source.write_text(PROGRAM)
+    subprocess.check_call(["nvcc", "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-I", CSRC, "-o", str(program), str(source)])
+
+    def call(*words):
+        return subprocess.run([str(program), *map(str, words)], capture_output=True, text=True, timeout=20, check=True).stdout.split()
+    return call
+
+
+@pytest.mark.parametrize("rate, given, want", [(0.0, 0, ["0", "idle"]), (0.0, 1, ["0", "idle"]), (2.0 ** -18, 1, ["0", "idle"]),
+                                               (0.5, 1, ["1", "rng"]), (1.0, 1, ["1", "rng"]), (1.5, 1, ["refused"])])
+def test_no_kernel_holds_a_null_generator_state(ask, rate, given, want):
+    """Where nothing is dropped a valid address stands for the state, so that a load moved in front of its condition reads nothing it must not."""
+    assert ask("drop", rate, given) == want
