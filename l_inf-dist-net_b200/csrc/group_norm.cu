@@ -11,11 +11,9 @@
 // their shared memory read x once, but loaded, reduced and stored in turn: 65 for the first, and 528 instead of 216 for the second, whose rows
 // they had to cut into pieces of 32 bytes.
 //
-// The sums of the kept form are a mean and a
-// sum of squared deviations (of a thread's values, of a column's, of a group's), joined by
-//   mean = sum n_i mean_i / n,  M2 = sum M2_i + sum n_i (mean_i - mean)^2;
-// the CTAs of the two passes join theirs as sums of x and x^2 in 64 bits.  So data far from 0 against their spread (activations of distance
-// layers are all positive) lose nothing of their variance.  The order of every addition is fixed by the shape alone.
+// The forward sums are fp32 over a few dozen rows of a thread, about a shift near the data, joined as means and variances, and 64-bit over the
+// CTAs of a group (Moments).  So neither the number of rows, nor data far from 0 against their spread (activations of distance layers are all
+// positive), nor single rows far from the others cost more than a few roundings.  The order of every addition is fixed by the shape alone.
 #include "group_norm.cuh"
 
 namespace linf {
@@ -25,10 +23,12 @@ namespace {
 struct Own { float one, zero; long long rng[2]; };
 __device__ Own g_own = {1.f, 0.f, {0, 0}};
 
+// Mean and 1 / deviation of a group.
+struct Stat { float mean, r; };
 // What a thread's column needs for u = (x + m) a + o: m is the mean with its sign turned.
 template <int V> struct Column { Lanes<V> m, a, o; };
 template <int V>
-__device__ __forceinline__ void load_column(Column<V>& k, const float2* stat, const Param& gamma, const Param& beta, const NormDims& d,
+__device__ __forceinline__ void load_column(Column<V>& k, const Stat* stat, const Param& gamma, const Param& beta, const NormDims& d,
                                             const NormPlan& p, const NormBlock& b, int cv) {
     int g[V];
     groups_of<V>(d, p, cv * V, g);
@@ -37,9 +37,9 @@ __device__ __forceinline__ void load_column(Column<V>& k, const float2* stat, co
     load_params<V>(beta, b.c0 + cv * V, o);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const float2 s = stat[g[j]];
-        m[j] = -s.x;
-        a[j] *= s.y;
+        const Stat s = stat[g[j]];
+        m[j] = -s.mean;
+        a[j] *= s.r;
     }
     k.m.set(m);
     k.a.set(a);
@@ -51,92 +51,170 @@ __device__ __forceinline__ void write_vector(const Raw<T, V>& v, const Column<V>
     if (drop.on) u = linf::drop<V>(drop, key, i, u);
     store_once<T, V>(y + i, raw_of<T, V>(u));
 }
-__device__ __forceinline__ float2 finish_stat(double mean, double var, double eps) {
-    return make_float2((float)mean, 1.f / sqrtf((float)(var + eps)));
+__device__ __forceinline__ Stat finish_stat(double mean, double var, double eps) {
+    Stat s;
+    s.mean = (float)mean;
+    s.r = 1.f / sqrtf((float)((var > 0.0 || var != var ? var : 0.0) + eps));
+    return s;
 }
 
-// A thread's sums of its column about its first row: s = sum (x + k), q = sum (x + k)^2, k the first row with its sign turned.
-template <int V> struct Moments {
-    Lanes<V> k, s, q;
-    __device__ __forceinline__ Moments() { k = s = q = filled<V>(0.f); }
-    __device__ __forceinline__ void start(const Lanes<V>& v) { k = mul(v, filled<V>(-1.f)); }
+// A thread's sums for the mean and the variance of what it reads.  They are taken in runs of at most 39 rows (8 the first time) about a shift near
+// the data -- the first row, then the mean so far --, and the runs are added up: so a column's length costs few roundings, and a first row
+// apart from the rest (a border, a special position) is as good as forgotten from the second run on.  A new shift: sums S, Q of n values,
+// moved by e, become S + n e and Q + e (2 S + n e).  What a thread hands on is a shift, the mean less that shift, and the variance: data far
+// from 0 against their spread lose nothing by the mean's rounding.
+//   SAME (a vector lies in one group): one shift and one pair of sums for the vector; else one for each channel, the runs' in shared memory.
+constexpr int kRunTurns = 4;               // turns of 8 rows between two flushes
+struct Part { float shift, mean, var; };   // of some values; the mean is shift + mean
+template <int V, bool SAME> struct Moments {
+    static_assert(SAME || V > 1, "a vector of one channel lies in one group");
+    Lanes<V> k, s, q;                           // the shift with its sign turned, sum (x + k), sum (x + k)^2 of the run
+    float S, Q;                                 // SAME: of the runs before
+    float2* runs;                               // else: S, Q of each channel
+    int rows;                                   // up to the last flush
+    // place: where the thread's parts will be; its runs are there before
+    __device__ __forceinline__ explicit Moments(Part* place) : S(0.f), Q(0.f), runs(reinterpret_cast<float2*>(place)), rows(0) {
+        k = s = q = filled<V>(0.f);
+    }
+    __device__ __forceinline__ void start(const Lanes<V>& v) {
+        if constexpr (SAME) {
+            float f[V];
+            mul(v, filled<V>(-1.f / V)).get(f);
+            k = filled<V>(tree(f));
+        } else {
+            k = mul(v, filled<V>(-1.f));
+        }
+    }
     __device__ __forceinline__ void add(const Lanes<V>& v) {
         const Lanes<V> e = linf::add(v, k);
         s = linf::add(s, e);
         q = fma(e, e, q);
     }
-    // (mean, M2) of `count` rows into red: one pair for each channel, or for the vector where it lies in one group
-    __device__ __forceinline__ void put(float2* red, const NormPlan& p, int rt, int cv, int count) const {
-        const float inv = count > 0 ? 1.f / (float)count : 0.f;
-        float m[V], m2[V], first[V];
-        s.get(m);
-        q.get(m2);
-        k.get(first);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            m2[j] = fmaf(-m[j] * inv, m[j], m2[j]);
-            m[j] = fmaf(m[j], inv, -first[j]);
-        }
-        if (p.same) {
-            float all = m[0], t = m2[0];
-#pragma unroll
-            for (int j = 1; j < V; ++j) { all += m[j]; t += m2[j]; }
-            all *= 1.f / V;
-#pragma unroll
-            for (int j = 0; j < V; ++j) t = fmaf((float)count * (m[j] - all), m[j] - all, t);
-            red[rt * p.tx + cv] = make_float2(all, t);
+    // what came since the last flush; upto: rows so far
+    __device__ __forceinline__ void flush(int upto) {
+        if constexpr (SAME) {
+            float a, b;
+            all_runs(a, b);
+            rows = upto;
+            const float n = (float)(rows * V), from = shift(), to = fmaf(a, -1.f / n, from), e = to - from;
+            S = fmaf(n, e, a);
+            Q = fmaf(e, a + S, b);
+            k = filled<V>(to);
         } else {
+            Lanes<V> a, b;
+            all_runs(a, b);
+            rows = upto;
+            const Lanes<V> to = fma(a, filled<V>(-1.f / (float)rows), k), e = fma(k, filled<V>(-1.f), to);
+            const Lanes<V> moved = fma(e, filled<V>((float)rows), a);
+            float f[V], h[V];
+            moved.get(f);
+            fma(e, linf::add(a, moved), b).get(h);
 #pragma unroll
-            for (int j = 0; j < V; ++j) red[(rt * p.tx + cv) * V + j] = make_float2(m[j], m2[j]);
+            for (int j = 0; j < V; ++j) runs[j] = make_float2(f[j], h[j]);
+            k = to;
+        }
+        s = q = filled<V>(0.f);
+    }
+    // mean and variance of `all` rows, for each channel or for the vector
+    __device__ __forceinline__ void put(Part* to, int all) const {
+        if constexpr (SAME) {
+            float a, b;
+            all_runs(a, b);
+            const float inv = 1.f / (float)(all * V), m = a * inv;
+            *to = Part{-shift(), m, fmaf(-m, m, b * inv)};
+        } else {
+            Lanes<V> a, b;
+            all_runs(a, b);
+            const Lanes<V> inv = filled<V>(1.f / (float)all);
+            float m[V], v[V], h[V];
+            mul(a, inv).get(m);
+            mul(b, inv).get(v);
+            k.get(h);
+#pragma unroll
+            for (int j = 0; j < V; ++j) to[j] = Part{-h[j], m[j], fmaf(-m[j], m[j], v[j])};
         }
     }
+private:
+    static __device__ __forceinline__ float tree(float (&f)[V]) {
+#pragma unroll
+        for (int n = V / 2; n > 0; n /= 2)
+#pragma unroll
+            for (int j = 0; j < n; ++j) f[j] += f[j + n];
+        return f[0];
+    }
+    __device__ __forceinline__ float shift() const { float f[V]; k.get(f); return f[0]; }
+    // the sums of all rows so far about the shift
+    __device__ __forceinline__ void all_runs(float& a, float& b) const {
+        float f[V], h[V];
+        s.get(f);
+        q.get(h);
+        a = S + tree(f);
+        b = Q + tree(h);
+    }
+    __device__ __forceinline__ void all_runs(Lanes<V>& a, Lanes<V>& b) const {
+        a = s;
+        b = q;
+        if (rows == 0) return;
+        float f[V], h[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float2 v = runs[j];
+            f[j] = v.x;
+            h[j] = v.y;
+        }
+        a = linf::add(lanes<V>(f), s);
+        b = linf::add(lanes<V>(h), q);
+    }
 };
+// A thread's place among the CTA's parts.
+template <int V, bool SAME> __device__ __forceinline__ Part* moments_at(Part* red, const NormPlan& p, int rt, int cv) {
+    return red + (rt * p.tx + cv) * (SAME ? 1 : V);
+}
 
-// (mean, M2) of each group of the block over the CTA's rows from what the threads put into red; done(g, mean, M2) in one lane.
-template <int V, typename Done>
-__device__ __forceinline__ void join_moments(float2* red, const NormDims& d, const NormPlan& p, const NormBlock& b, const NormRows& share, Done done) {
-    const int each = p.same ? V : 1, width = p.same ? p.tx : p.tx * V, lane = threadIdx.x & 31;
-    const int per = (p.pieces == 1 ? d.Cg : b.nvec * V) / each;         // columns of red of a group
+// Mean and variance of each group of the block over the CTA's rows from what the threads put into red; done(g, mean, variance) in one lane.
+// Parts of weights w_i join as mean = sum w_i mean_i, variance = sum w_i (variance_i + mean_i^2) - mean^2, about one part's shift.
+template <int V, bool SAME, typename Done>
+__device__ __forceinline__ void join_moments(Part* red, const NormDims& d, const NormPlan& p, const NormBlock& b, const NormRows& share, Done done) {
+    const int width = SAME ? p.tx : p.tx * V, lane = threadIdx.x & 31;
+    const int per = (p.pieces == 1 ? d.Cg : b.nvec * V) / (SAME ? V : 1);         // columns of red of a group
     __syncthreads();
     if (p.rt > 1) {
-        // columns along the rows, about the first row's mean
+        // columns along the rows
         by_columns(width, p.rt, [&](int c, int first, int step, auto join) {
-            const float k0 = c < width ? red[c].x : 0.f, one = 1.f / (float)each;
+            const float k0 = c < width ? red[c].shift : 0.f, inv = 1.f / (float)share.all;
             float s = 0.f, q = 0.f;
             for (int r = first; r < p.rt; r += step) {
-                const float2 v = red[r * width + c];
-                const float count = (float)rows_of(share, r), e = v.x - k0;
-                s = fmaf(count, e, s);
-                q = fmaf(count * e, e, fmaf(v.y, one, q));
+                const Part v = red[r * width + c];
+                const float weight = (float)rows_of(share, r) * inv, e = (v.shift - k0) + v.mean;
+                s = fmaf(weight, e, s);
+                q = fmaf(weight, fmaf(e, e, v.var), q);
             }
-            if (join(s, q)) {
-                const float inv = 1.f / (float)share.all;
-                red[c] = make_float2(fmaf(s, inv, k0), fmaf(-s * inv, s, q) * (float)each);
-            }
+            if (join(s, q)) red[c] = Part{k0, s, fmaf(-s, s, q)};
         });
         __syncthreads();
     }
-    // groups along their columns, about the first column's mean: as many lanes to a group as the group has columns, up to a warp
+    // groups along their columns: as many lanes to a group as the group has columns, up to a warp
     int wide = 1;
     while (wide < per && wide < 32) wide *= 2;
-    const float weight = 1.f / ((float)share.all * (float)each), by = 1.f / (float)per;
+    const float by = 1.f / (float)per;
     for (int g0 = (threadIdx.x >> 5) * (32 / wide); g0 < b.ng; g0 += (blockDim.x >> 5) * (32 / wide)) {
         const int g = g0 + lane / wide;
         float s = 0.f, q = 0.f, k0 = 0.f;
         if (g < b.ng) {
-            k0 = red[g * per].x;
+            k0 = red[g * per].shift;
             for (int c = lane & (wide - 1); c < per; c += wide) {
-                const float2 v = red[g * per + c];
-                const float e = v.x - k0;
+                const Part v = red[g * per + c];
+                const float e = (v.shift - k0) + v.mean;
                 s += e;
-                q = fmaf(e, e, fmaf(v.y, weight, q));
+                q += fmaf(e, e, v.var);
             }
         }
         for (int o = 1; o < wide; o *= 2) {
             s += __shfl_xor_sync(0xffffffffu, s, o);
             q += __shfl_xor_sync(0xffffffffu, q, o);
         }
-        if (g < b.ng && (lane & (wide - 1)) == 0) done(g, fmaf(s, by, k0), fmaf(-s * by, s, q) * (float)share.all * (float)each);
+        s *= by;
+        if (g < b.ng && (lane & (wide - 1)) == 0) done(g, (double)k0 + (double)s, fmaf(-s, s, q * by));
     }
 }
 
@@ -145,23 +223,23 @@ __device__ __forceinline__ void join_moments(float2* red, const NormDims& d, con
 // Shared memory: the rows of all tensors, a pair for each thread and channel (or vector), the statistics of each group, and where elements are
 // dropped in a backward pass a byte for each vector: which of its elements are kept.  Offsets in bytes.
 struct KeptSpace { int red, stat, mask, bytes; };
-KeptSpace kept_space(const NormPlan& p, int elem_bytes, int tensors, bool by_vector, bool masks) {
+KeptSpace kept_space(const NormPlan& p, int elem_bytes, int tensors, size_t of_thread, bool by_vector, size_t of_group, bool masks) {
     KeptSpace s;
     s.red = (p.rows * p.tx * p.V * elem_bytes * tensors + 15) / 16 * 16;
-    s.stat = s.red + (int)sizeof(float2) * p.rt * p.tx * (by_vector ? 1 : p.V);
-    s.mask = s.stat + (int)sizeof(float2) * p.groups;
+    s.stat = (s.red + (int)of_thread * p.rt * p.tx * (by_vector ? 1 : p.V) + 15) / 16 * 16;
+    s.mask = s.stat + (int)of_group * p.groups;
     s.bytes = s.mask + (masks ? p.rows * p.tx : 0);
     return s;
 }
 
-template <typename T, int V>
+template <typename T, int V, bool SAME>
 __global__ void __launch_bounds__(kNormThreads, 3)
 norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, NormPlan p, KeptSpace sp, double eps, int act, Drop drop,
                  T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
     extern __shared__ uint4 space[];
     T* data = reinterpret_cast<T*>(space);
-    float2* red = space_at<float2>(space, sp.red);
-    float2* stat = space_at<float2>(space, sp.stat);
+    Part* red = space_at<Part>(space, sp.red);
+    Stat* stat = space_at<Stat>(space, sp.stat);
     const int n = p.by_blocks(blockIdx.x);
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
@@ -174,18 +252,25 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
     for (int r = rt; r < r1; r += p.rt) keep_vector<T, V>(own + r * pitch, x + at + (size_t)r * d.C);
     keep_wait();
     if (in) {
-        Moments<V> t;
-        if (rt < r1) t.start(load_lanes<T, V>(own + rt * pitch));
+        Part* place = moments_at<V, SAME>(red, p, rt, cv);
+        Moments<V, SAME> t(place);
+        t.start(load_lanes<T, V>(own + rt * pitch));
+        const int rows = rows_of(share, rt);
+        const T* at_r = own + rt * pitch;
+        for (int r = 0, run = 8; r < rows; run = 8 * kRunTurns) {
+            const int to = min(rows, r + run);
 #pragma unroll 4
-        for (int r = rt + p.rt; r < r1; r += p.rt) t.add(load_lanes<T, V>(own + r * pitch));
-        t.put(red, p, rt, cv, rows_of(share, rt));
+            for (; r < to; ++r, at_r += p.rt * pitch) t.add(load_lanes<T, V>(at_r));
+            if (to < rows) t.flush(to);
+        }
+        t.put(place, rows);
     }
-    join_moments<V>(red, d, p, b, share, [&](int g, float mu, float m2) {
-        const float2 s = finish_stat(mu, (double)m2 * d.inv_m, eps);
+    join_moments<V, SAME>(red, d, p, b, share, [&](int g, double mu, float var) {
+        const Stat s = finish_stat(mu, var, eps);
         stat[g] = s;
         if (mean != nullptr) {
-            mean[(size_t)n * d.G + b.g0 + g] = s.x;
-            rstd[(size_t)n * d.G + b.g0 + g] = s.y;
+            mean[(size_t)n * d.G + b.g0 + g] = s.mean;
+            rstd[(size_t)n * d.G + b.g0 + g] = s.r;
         }
     });
     __syncthreads();
@@ -203,41 +288,49 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
 
 constexpr int kRing = 8, kBackRing = 4;    // rows that are on their way at a time
 
-template <typename T, int V>
+template <typename T, int V, bool SAME>
 __global__ void __launch_bounds__(kNormThreads, 4)
 norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __restrict__ part) {
     extern __shared__ uint4 space[];                            // the ring, then [rt][tx] or [rt][tx * V]
-    float2* red = space_at<float2>(space, norm_ring_bytes<T, V, 1, kRing>());
+    Part* red = space_at<Part>(space, norm_ring_bytes<T, V, 1, kRing>());
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const NormRows share = norm_rows(d, p, split);
     if (rt < p.rt && cv < b.nvec) {
-        const int first = split * p.rt + rt;
+        const int first = split * p.rt + rt, rows = rows_of(share, rt);
         const T* const at[1] = {x + ((size_t)n * d.L) * d.C + b.c0 + cv * V};
         NormStream<T, V, 1, kRing> stream(space, at, first, d.L, p.splits * p.rt, d.C);
         grid_let_go();
-        Moments<V> t;
+        Part* place = moments_at<V, SAME>(red, p, rt, cv);
+        Moments<V, SAME> t(place);
         t.start(load_lanes<T, V>(at[0] + (size_t)first * d.C));
-        stream.template run<true>([&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); });
-        t.put(red, p, rt, cv, rows_of(share, rt));
+        int turns = 0;
+        stream.template run<true>([&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); },
+                                  [&]() { if ((turns++ & (kRunTurns - 1)) == 0) t.flush(min(rows, turns * kRing)); });
+        t.put(place, rows);
     }
-    const double count = (double)share.all * (p.pieces == 1 ? d.Cg : b.nvec * V);
-    join_moments<V>(red, d, p, b, share, [&](int g, float mu, float m2) {
-        part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_double2(count * mu, m2 + count * mu * mu);
+    join_moments<V, SAME>(red, d, p, b, share, [&](int g, double mu, float var) {
+        part[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = make_double2(mu, var);
     });
 }
 
-// The two sums of a group over the CTAs that share its rows and over its pieces, in all lanes.
-__device__ __forceinline__ double2 add_parts(const double2* part, const NormDims& d, const NormPlan& p, int n, int g) {
-    double a = 0.0, e = 0.0;
+// Mean and variance of a group from those of the CTAs that share its rows and of its pieces, about the first one's mean; in all lanes.
+__device__ __forceinline__ double2 join_parts(const double2* part, const NormDims& d, const NormPlan& p, int n, int g) {
+    const double ref = __ldcg(&part[((size_t)n * p.splits * d.G + g) * p.pieces].x);
+    const int threads = p.splits * p.rt, base = d.L / threads, more = d.L - base * threads;
+    double a = 0.0, q = 0.0;
     for (int k = threadIdx.x & 31; k < p.splits * p.pieces; k += 32) {
         const int s = k / p.pieces, piece = k - s * p.pieces;
         const double2 v = __ldcg(part + (((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece);
-        a += v.x;
-        e += v.y;
+        const int rows = base * p.rt + min(max(more - s * p.rt, 0), p.rt), width = p.pieces == 1 ? d.Cg : min(p.piece, d.Cg / p.V - piece * p.piece) * p.V;
+        const double weight = (double)rows * (double)width * d.inv_m, e = v.x - ref;
+        a += weight * e;
+        q += weight * (v.y + e * e);
     }
-    return make_double2(warp_sum(a) * d.inv_m, warp_sum(e) * d.inv_m);
+    a = warp_sum(a);
+    q = warp_sum(q);
+    return make_double2(ref + a, q - a * a);
 }
 
 template <typename T, int V>
@@ -245,7 +338,7 @@ __global__ void __launch_bounds__(kNormThreads, 4)
 norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double2* __restrict__ part, NormDims d, NormPlan p, double eps, int act,
                   Drop drop, T* __restrict__ y, float* __restrict__ mean, float* __restrict__ rstd) {
     extern __shared__ uint4 space[];                            // the ring, then the groups' mean and 1 / deviation
-    float2* stat = space_at<float2>(space, norm_ring_bytes<T, V, 1, kRing>());
+    Stat* stat = space_at<Stat>(space, norm_ring_bytes<T, V, 1, kRing>());
     const int last = gridDim.x - 1 - blockIdx.x, n = p.by_blocks(last), split = p.splits - 1 - blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, last - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
@@ -255,14 +348,13 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
     NormStream<T, V, 1, kRing> stream(space, from, split * p.rt + rt, in ? d.L : 0, p.splits * p.rt, d.C);
     grid_wait();
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
-        const double2 v = add_parts(part, d, p, n, b.g0 + g);
-        const double var = v.y - v.x * v.x;
+        const double2 v = join_parts(part, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
-            const float2 f = finish_stat(v.x, var > 0.0 || var != var ? var : 0.0, eps);
+            const Stat f = finish_stat(v.x, v.y, eps);
             stat[g] = f;
             if (split == 0 && b.piece == 0 && mean != nullptr) {
-                mean[(size_t)n * d.G + b.g0 + g] = f.x;
-                rstd[(size_t)n * d.G + b.g0 + g] = f.y;
+                mean[(size_t)n * d.G + b.g0 + g] = f.mean;
+                rstd[(size_t)n * d.G + b.g0 + g] = f.r;
             }
         }
     }
@@ -275,6 +367,18 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
+
+// The two sums of a group over the CTAs that share its rows and over its pieces, in all lanes.
+__device__ __forceinline__ double2 add_parts(const double2* part, const NormDims& d, const NormPlan& p, int n, int g) {
+    double a = 0.0, e = 0.0;
+    for (int k = threadIdx.x & 31; k < p.splits * p.pieces; k += 32) {
+        const int s = k / p.pieces, piece = k - s * p.pieces;
+        const double2 v = __ldcg(part + (((size_t)n * p.splits + s) * d.G + g) * p.pieces + piece);
+        a += v.x;
+        e += v.y;
+    }
+    return make_double2(warp_sum(a) * d.inv_m, warp_sum(e) * d.inv_m);
+}
 
 // What a thread's column needs for u = (x + m) a + o, and for dx = a du + ra + (x + m) rb; m as above.
 template <int V> struct BackColumn {
@@ -596,21 +700,28 @@ size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
     return parts_bytes(d, p) + (back ? sizeof(float2) * (size_t)channel_rows(p) * d.C : 0);
 }
 
-template <typename T, int V>
-int forward(const T* x, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, const Drop& drop, T* y, float* mean,
-            float* rstd, void* ws, cudaStream_t st) {
+template <typename T, int V, bool SAME>
+int forward_as(const T* x, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, const Drop& drop, T* y, float* mean,
+               float* rstd, void* ws, cudaStream_t st) {
     if (p.kept) {
-        const KeptSpace sp = kept_space(p, sizeof(T), 1, p.same, false);
-        return launch_kept(norm_kept_kernel<T, V>, p, sp.bytes, st, x, given.gamma, given.beta, d, p, sp, eps, act, drop, y, mean, rstd);
+        const KeptSpace sp = kept_space(p, sizeof(T), 1, sizeof(Part), SAME, sizeof(Stat), false);
+        return launch_kept(norm_kept_kernel<T, V, SAME>, p, sp.bytes, st, x, given.gamma, given.beta, d, p, sp, eps, act, drop, y, mean, rstd);
     }
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     double2* part = static_cast<double2*>(ws);
     const size_t ring = norm_ring_bytes<T, V, 1, kRing>();
-    const size_t one = ring + sizeof(float2) * p.rt * p.tx * (p.same ? 1 : V), two = ring + sizeof(float2) * p.groups;
-    if (!allow_shared(norm_sums_kernel<T, V>, one) || !allow_shared(norm_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
-    norm_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(x, d, p, part);
+    const size_t one = ring + sizeof(Part) * p.rt * p.tx * (SAME ? 1 : V), two = ring + sizeof(Stat) * p.groups;
+    if (!allow_shared(norm_sums_kernel<T, V, SAME>, one) || !allow_shared(norm_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
+    norm_sums_kernel<T, V, SAME><<<grid, kNormThreads, one, st>>>(x, d, p, part);
     if (launch_status()) return LINF_ERR_LAUNCH;
     return launch_behind(norm_apply_kernel<T, V>, grid, kNormThreads, two, st, x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
+}
+template <typename T, int V>
+int forward(const T* x, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, const Drop& drop, T* y, float* mean,
+            float* rstd, void* ws, cudaStream_t st) {
+    if constexpr (V > 1)
+        if (!p.same) return forward_as<T, V, false>(x, given, d, p, eps, act, drop, y, mean, rstd, ws, st);
+    return forward_as<T, V, true>(x, given, d, p, eps, act, drop, y, mean, rstd, ws, st);
 }
 
 template <typename T, int V>
@@ -619,7 +730,7 @@ int backward(const T* dy, const T* x, const NormGiven& given, int ptype, const f
     double2* by_group = static_cast<double2*>(ws);
     float2* by_channel = reinterpret_cast<float2*>(static_cast<char*>(ws) + parts_bytes(d, p));
     if (p.kept) {
-        const KeptSpace sp = kept_space(p, sizeof(T), 2, false, drop.on && sizeof(T) == 2);
+        const KeptSpace sp = kept_space(p, sizeof(T), 2, sizeof(float2), false, sizeof(float2), drop.on && sizeof(T) == 2);
         const int rc = launch_kept(norm_back_kept_kernel<T, V>, p, sp.bytes, st, dy, x, given.gamma, given.beta, mean, rstd, d, p, sp, act, drop,
                                    dx, by_channel);
         if (rc) return rc;

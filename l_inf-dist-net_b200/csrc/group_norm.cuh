@@ -301,6 +301,7 @@ __host__ __device__ constexpr size_t norm_ring_bytes() { return sizeof(T) * V >=
 // to shared memory at a time, each thread's to places of its own (`ring`: norm_ring_bytes), so that neither registers nor barriers limit
 // how much is read ahead (32 x 320 x 64 x 64 bf16, both passes: batches of 8 loads to registers 68 us, this 59 us).  Elements of two bytes that no wider copy
 // reaches come through registers.
+struct NoTurn { __device__ __forceinline__ void operator()() const {} };
 template <typename T, int V, int N, int S>
 struct NormStream {
     static constexpr int bytes = sizeof(T) * V, place = kNormThreads * bytes;      // ring: [S][N][threads]
@@ -344,19 +345,28 @@ struct NormStream {
         r += step;
     }
     // LIGHT bodies are written out for a whole turn of the ring: half the instructions (sums of bf16 maps: 52 -> 34 a vector, 24 -> 21 us);
-    // heavy ones are not, their code would be too long (38 -> 40 us).
-    template <bool LIGHT, typename Body> __device__ __forceinline__ void run(Body body) {
+    // heavy ones are not, their code would be too long (38 -> 40 us).  turn(): after each S rows, the last ones excepted.
+    template <bool LIGHT, typename Body, typename Turn = NoTurn> __device__ __forceinline__ void run(Body body, Turn turn = Turn()) {
         if constexpr (bytes >= 4) {
             if constexpr (LIGHT) {
                 for (int turns = r < r1 ? ((r1 - r - 1) / step + 1) / S : 0; turns > 0; --turns) {
 #pragma unroll
                     for (int s = 0; s < S; ++s) row(s, body);
+                    turn();
                 }
             }
+            if constexpr (LIGHT || std::is_same<Turn, NoTurn>::value) {
 #pragma unroll 1
-            for (int s = 0; r < r1; s = s + 1 == S ? 0 : s + 1) row(s, body);
+                for (int s = 0; r < r1; s = s + 1 == S ? 0 : s + 1) row(s, body);
+            } else {
+#pragma unroll 1
+                for (int s = 0; r < r1;) {
+                    row(s, body);
+                    if (++s == S) { s = 0; turn(); }
+                }
+            }
         } else {
-            constexpr int K = 8 / N;
+            constexpr int K = S;
             for (; r < r1; r += K * step) {
                 Raw<T, V> v[K][N];
 #pragma unroll
@@ -370,6 +380,7 @@ struct NormStream {
 #pragma unroll
                 for (int j = 0; j < K; ++j)
                     if (r + j * step < r1) body(r + j * step, v[j]);
+                turn();
             }
         }
     }

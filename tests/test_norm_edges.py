@@ -1,0 +1,59 @@
+"""Group norm, its interval form and their gradients where arithmetic runs out: long columns, values far from 0, values at the ends of
+their type.  Everything is compared with the formulas in 64 bits; the tolerances are worked out beside the tests."""
+import math
+
+import pytest
+import torch
+
+import linfdist_b200 as L
+import norm_reference as R
+from norm_reference import E
+
+gpu = pytest.mark.gpu
+EPS = 1e-5
+
+
+def stored(N, C, L_, dtype, seed, spread=0.5, level=3.0):
+    """[N, C, L_] on the GPU, the channels last in memory."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(N, L_, C, generator=gen, device="cuda").mul_(spread).add_(level)
+    return x.to(dtype).movedim(-1, 1)
+
+
+def parts(x, groups):
+    """(h, mean, 1 / deviation) of [N, C, L] in 64 bits on the device of x, h as [N, groups, C / groups, L]."""
+    t = x.detach().double().view(x.size(0), groups, x.size(1) // groups, -1)
+    mean = t.mean((2, 3), keepdim=True)
+    t = t - mean
+    r = (t.square().mean((2, 3), keepdim=True) + EPS).rsqrt()
+    return t.mul_(r), mean, r
+
+
+def assert_within(got, want, most, what):
+    bad = ~((got.double() - want).abs() <= most)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {((got.double() - want).abs() - most).max():.3g} over"
+
+
+# (N, C, groups, positions, rows of threads): the two passes with 2048 and 512 rows to a thread, vectors within one group and across several;
+# the kept form; elements one by one
+LONG = [(1, 1024, 32, 131072, 64), (1, 1024, 512, 131072, 64), (1, 255, 1, 32768, 64), (3, 8, 2, 2000, 128), (3, 12, 12, 1000, 85)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "C{}_G{}_L{}".format(*c[1:4]))
+def test_first_rows_apart_from_the_rest(cuda, lib, case, dtype):
+    """Every thread's first row lies 300 deviations off (a border, a special position).
+
+    A thread's first run has 8 rows, seven of them D off the shift.  Their sums are off by 7 E of 7 D and 7 D^2, so their sum of squares about
+    their mean by less than 135 E D^2; the runs behind it stand D / 8 off their shift at most and add less than 50 E D^2, the later ones 2.
+    The thread's own sum of squares is at least D^2 (1 - 1 / n), so the variance is off by less than 200 E of itself, 1 / deviation by
+    100 E.  The mean: 49 E D of the first run and 128 E D of the second, over n values, with D at most sqrt(n) deviations: below 177 E / sqrt(n)
+    deviations.  Then the roundings of the element itself."""
+    N, C, groups, n, first = case
+    x = stored(N, C, n, dtype, sum(case))
+    x[:, :, :first] += 150.0
+    y = L.group_norm(x, groups, eps=EPS)
+    h, mean, r = parts(x, groups)
+    most = 100 * E * h.abs() + 177 * E / math.sqrt(n / first) + 6 * E * (h.abs() + r * mean.abs()) + R.HALF_STEP[dtype] * h.abs() + 1e-30
+    assert_within(y.view(h.shape), h, most, "values")
