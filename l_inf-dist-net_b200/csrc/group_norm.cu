@@ -23,9 +23,9 @@ namespace {
 struct Own { float one, zero; long long rng[2]; };
 __device__ Own g_own = {1.f, 0.f, {0, 0}};
 
-// Mean and 1 / deviation of a group.
-struct Stat { float mean, r; };
-// What a thread's column needs for u = (x + m) a + o: m is the mean with its sign turned.
+// Mean (in two parts: values far from 0 against their spread would see the rounding of one) and 1 / deviation of a group.
+struct alignas(16) Stat { float mean, rest, r; };
+// What a thread's column needs for u = (x + m) a + o: m is the mean's first part with its sign turned, o takes the second.
 template <int V> struct Column { Lanes<V> m, a, o; };
 template <int V>
 __device__ __forceinline__ void load_column(Column<V>& k, const Stat* stat, const Param& gamma, const Param& beta, const NormDims& d,
@@ -40,6 +40,7 @@ __device__ __forceinline__ void load_column(Column<V>& k, const Stat* stat, cons
         const Stat s = stat[g[j]];
         m[j] = -s.mean;
         a[j] *= s.r;
+        o[j] = fmaf(-s.rest, a[j], o[j]);
     }
     k.m.set(m);
     k.a.set(a);
@@ -54,6 +55,7 @@ __device__ __forceinline__ void write_vector(const Raw<T, V>& v, const Column<V>
 __device__ __forceinline__ Stat finish_stat(double mean, double var, double eps) {
     Stat s;
     s.mean = (float)mean;
+    s.rest = (float)(mean - (double)s.mean);
     s.r = 1.f / sqrtf((float)((var > 0.0 || var != var ? var : 0.0) + eps));
     return s;
 }

@@ -57,3 +57,25 @@ def test_first_rows_apart_from_the_rest(cuda, lib, case, dtype):
     h, mean, r = parts(x, groups)
     most = 100 * E * h.abs() + 177 * E / math.sqrt(n / first) + 6 * E * (h.abs() + r * mean.abs()) + R.HALF_STEP[dtype] * h.abs() + 1e-30
     assert_within(y.view(h.shape), h, most, "values")
+
+
+# dense; kept, vectors within one group and across several; the two passes, both as well
+FAR = [(7, 512, 16, 1), (5, 64, 8, 9), (3, 24, 4, 30), (2, 2, 1, 50), (1, 64, 8, 40000), (1, 24, 4, 22500), (2, 3, 1, 9000)]
+
+
+@gpu
+@pytest.mark.parametrize("case", FAR, ids=lambda c: "N{}_C{}_G{}_L{}".format(*c))
+def test_values_very_far_from_zero(cuda, lib, case):
+    """A mean of 10^6 deviations: the mean is not rounded to fp32 anywhere, so the values are off by their own roundings alone and lie within the bounds
+    of a box of one point.
+
+    x less the mean's first part is exact (both are fp32 numbers less than a factor of two apart); the second part goes into the added
+    term, which is below 2^-24 * 10^6 / deviation and rounded once; 1 / deviation, its product with the difference, the sum: E each.  Parts of the sums
+    are joined about one shift, off by a few roundings of a deviation, as the variance is by a few of its own: 16 E in all."""
+    N, C, groups, n = case
+    x = stored(N, C, n, torch.float32, sum(case), level=5e5)
+    x = x if n > 1 else x.reshape(N, C)
+    h, mean, r = parts(x, groups)
+    most = 16 * E * (1 + h.abs()) + E * E * r * mean.abs()
+    y = L.group_norm(x, groups, eps=EPS)
+    assert_within(y.reshape(h.shape), h, most, "values")
