@@ -60,13 +60,13 @@ __device__ __forceinline__ Stat finish_stat(double mean, double var, double eps)
     return s;
 }
 
-// A thread's sums for the mean and the variance of what it reads.  They are taken in runs of at most 39 rows (8 the first time) about a shift near
+// A thread's sums for the mean and the variance of what it reads.  They are taken in runs of at most 32 rows (8 the first time) about a shift near
 // the data -- the first row, then the mean so far --, and the runs are added up: so a column's length costs few roundings, and a first row
 // apart from the rest (a border, a special position) is as good as forgotten from the second run on.  A new shift: sums S, Q of n values,
 // moved by e, become S + n e and Q + e (2 S + n e).  What a thread hands on is a shift, the mean less that shift, and the variance: data far
 // from 0 against their spread lose nothing by the mean's rounding.
 //   SAME (a vector lies in one group): one shift and one pair of sums for the vector; else one for each channel, the runs' in shared memory.
-constexpr int kRunTurns = 4;               // turns of 8 rows between two flushes
+constexpr int kFirstRun = 8, kRun = 32;    // multiples of kRing
 struct Part { float shift, mean, var; };   // of some values; the mean is shift + mean
 template <int V, bool SAME> struct Moments {
     static_assert(SAME || V > 1, "a vector of one channel lies in one group");
@@ -259,7 +259,7 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
         t.start(load_lanes<T, V>(own + rt * pitch));
         const int rows = rows_of(share, rt);
         const T* at_r = own + rt * pitch;
-        for (int r = 0, run = 8; r < rows; run = 8 * kRunTurns) {
+        for (int r = 0, run = kFirstRun; r < rows; run = kRun) {
             const int to = min(rows, r + run);
 #pragma unroll 4
             for (; r < to; ++r, at_r += p.rt * pitch) t.add(load_lanes<T, V>(at_r));
@@ -289,6 +289,7 @@ norm_kept_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, N
 // ---- forward, two passes ----------------------------------------------------------------------------------------------
 
 constexpr int kRing = 8, kBackRing = 4;    // rows that are on their way at a time
+constexpr int kBackRun = 64;               // rows that a thread adds up in fp32
 
 template <typename T, int V, bool SAME>
 __global__ void __launch_bounds__(kNormThreads, 4)
@@ -307,9 +308,12 @@ norm_sums_kernel(const T* __restrict__ x, NormDims d, NormPlan p, double2* __res
         Part* place = moments_at<V, SAME>(red, p, rt, cv);
         Moments<V, SAME> t(place);
         t.start(load_lanes<T, V>(at[0] + (size_t)first * d.C));
-        int turns = 0;
-        stream.template run<true>([&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); },
-                                  [&]() { if ((turns++ & (kRunTurns - 1)) == 0) t.flush(min(rows, turns * kRing)); });
+        for (int r = 0, run = kFirstRun; r < rows; run = kRun) {
+            const int to = min(rows, r + run);
+            stream.template run<true>(to - r, [&](int, const Raw<T, V>(&v)[1]) { t.add(lanes_of<T, V>(v[0])); });
+            if (to < rows) t.flush(to);
+            r = to;
+        }
         t.put(place, rows);
     }
     join_moments<V, SAME>(red, d, p, b, share, [&](int g, double mu, float var) {
@@ -365,7 +369,7 @@ norm_apply_kernel(const T* __restrict__ x, Param gamma, Param beta, const double
     Column<V> col;
     load_column<V>(col, stat, gamma, beta, d, p, b, cv);
     const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-    stream.template run<false>([&](int r, const Raw<T, V>(&v)[1]) { write_vector<T, V>(v[0], col, act, drop, key, at + (size_t)r * d.C, y); });
+    stream.run_all([&](int r, const Raw<T, V>(&v)[1]) { write_vector<T, V>(v[0], col, act, drop, key, at + (size_t)r * d.C, y); });
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------
@@ -423,8 +427,8 @@ __device__ __forceinline__ void back_du(const Raw<T, V>& xv, const Raw<T, V>& gv
 }
 
 // Sums of gamma du and gamma du h over each group of the block from its channels' sums (du, du h), which `sums` holds by channel.
-template <typename Done>
-__device__ __forceinline__ void group_sums(const float2* sums, const Param& gamma, const NormDims& d, const NormPlan& p, const NormBlock& b, Done done) {
+template <typename Pair, typename Done>
+__device__ __forceinline__ void group_sums(const Pair* sums, const Param& gamma, const NormDims& d, const NormPlan& p, const NormBlock& b, Done done) {
     const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int per = p.pieces == 1 ? d.Cg : b.nvec * p.V;
     int wide = 1;                                               // as many lanes to a group as it has channels, up to a warp
@@ -434,7 +438,7 @@ __device__ __forceinline__ void group_sums(const float2* sums, const Param& gamm
         double s = 0.0, t = 0.0;
         for (int c = first; c < per; c += wide) {
             const float w = load_param(gamma, b.c0 + g * per + c);
-            const float2 v = sums[g * per + c];
+            const Pair v = sums[g * per + c];
             s += (double)w * v.x;
             t += (double)w * v.y;
         }
@@ -447,11 +451,12 @@ __device__ __forceinline__ void group_sums(const float2* sums, const Param& gamm
 }
 
 // Adds the threads' channel sums up along the rows; they end in red's first row.
-__device__ __forceinline__ void fold_rows(float2* red, int width, int rt) {
+template <typename Pair> __device__ __forceinline__ void fold_rows(Pair* red, int width, int rt) {
     by_columns(width, rt, [&](int c, int first, int step, auto join) {
-        float s = 0.f, t = 0.f;
-        for (int r = first; r < rt; r += step) { const float2 v = red[r * width + c]; s += v.x; t += v.y; }
-        if (join(s, t)) red[c] = make_float2(s, t);
+        Pair t;
+        t.x = t.y = 0;
+        for (int r = first; r < rt; r += step) { const Pair v = red[r * width + c]; t.x += v.x; t.y += v.y; }
+        if (join(t.x, t.y)) red[c] = t;
     });
 }
 
@@ -509,8 +514,7 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
         if (in) load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
         Lanes<V> sum_a = filled<V>(0.f), sum_b = sum_a;
         keep_wait();
-#pragma unroll 2
-        for (int r = rt; r < r1; r += p.rt) {
+        auto sum_row = [&](int r) {
             Lanes<V> du = load_lanes<T, V>(own_g + r * pitch), e;
             if (drop.on) {
                 const unsigned mask = drop_mask<V>(drop, key, at + (size_t)r * d.C);
@@ -522,6 +526,19 @@ norm_back_kept_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
             sum_b = fma(du, e, sum_b);
             // fp32: du takes the place of dy; 16-bit types would round it, and work it out again
             if (sizeof(T) == 4) *reinterpret_cast<Raw<T, V>*>(own_g + r * pitch) = raw_of<T, V>(du);
+        };
+        if constexpr (V == 1 && sizeof(T) == 2) {               // up to 127 rows to a thread (else 63): in runs, which are added up
+            for (int r0 = rt; r0 < r1; r0 += 32 * p.rt) {
+                const Lanes<V> a = sum_a, b = sum_b;
+                sum_a = sum_b = filled<V>(0.f);
+#pragma unroll 2
+                for (int r = r0; r < min(r0 + 32 * p.rt, r1); r += p.rt) sum_row(r);
+                sum_a = add(a, sum_a);
+                sum_b = add(b, sum_b);
+            }
+        } else {
+#pragma unroll 2
+            for (int r = rt; r < r1; r += p.rt) sum_row(r);
         }
         float sa[V], sb[V];
         sum_a.get(sa);
@@ -579,44 +596,62 @@ norm_back_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param g
                       const float* __restrict__ rstd, NormDims d, NormPlan p, int act, Drop drop, float2* __restrict__ by_channel,
                       double2* __restrict__ by_group) {
     extern __shared__ uint4 space[];                            // the ring, then [rt][tx * V]
-    float2* redf = space_at<float2>(space, norm_ring_bytes<T, V, 2, kBackRing>());
+    double2* red = space_at<double2>(space, norm_ring_bytes<T, V, 2, kBackRing>());
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx;
     const int width = p.tx * V;
-    if (rt < p.rt) {
+    // fp32 over a run of rows, 64-bit over the runs where there is more than one (the sums kernel of 16 x 128 x 160 x 160 bf16: 68 us, with 64-bit
+    // pairs in any case 72)
+    const NormRows share = norm_rows(d, p, split);
+    const bool one = share.base + (share.more > 0 ? 1 : 0) <= kBackRun;
+    if (rt < p.rt && cv < b.nvec) {
         Lanes<V> sum_a = filled<V>(0.f), sum_b = sum_a;
         BackColumn<V> col;
-        if (cv < b.nvec) {
-            const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
-            const T* const from[2] = {x + at, dy + at};
-            NormStream<T, V, 2, kBackRing> stream(space, from, split * p.rt + rt, d.L, p.splits * p.rt, d.C);
-            grid_let_go();
-            load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
-            const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-            stream.template run<false>([&](int r, const Raw<T, V>(&v)[2]) {
+        const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
+        const T* const from[2] = {x + at, dy + at};
+        NormStream<T, V, 2, kBackRing> stream(space, from, split * p.rt + rt, d.L, p.splits * p.rt, d.C);
+        const int rows = rows_of(share, rt);
+        grid_let_go();
+        load_back_column<V>(col, mean, rstd, gamma, beta, d, p, b, n, cv);
+        const DropKey key = drop.on ? drop_key(drop) : DropKey{};
+        // into the thread's pairs: V sums of du and of du h
+        auto put = [&](auto* own, bool begun) {
+            float sa[V], sb[V];
+            sum_a.get(sa);
+            sum_b.get(sb);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                auto v = own[j];
+                v.x = (begun ? v.x : 0) + sa[j];
+                v.y = (begun ? v.y : 0) + sb[j] * col.r[j];
+                own[j] = v;
+            }
+        };
+        for (int left = rows, run = 0; left > 0; left -= kBackRun, ++run) {
+            stream.template run<false>(min(left, kBackRun), [&](int r, const Raw<T, V>(&v)[2]) {
                 Lanes<V> du, e;
                 back_du<T, V>(v[0], v[1], col, act, drop, key, at + (size_t)r * d.C, du, e);
                 sum_a = add(sum_a, du);
                 sum_b = fma(du, e, sum_b);
             });
+            if (one) break;
+            put(red + rt * width + cv * V, run > 0);
+            sum_a = sum_b = filled<V>(0.f);
         }
-        float sa[V], sb[V];
-        sum_a.get(sa);
-        sum_b.get(sb);
-        if (cv < b.nvec) {
-#pragma unroll
-            for (int j = 0; j < V; ++j) sb[j] *= col.r[j];
-        }
-#pragma unroll
-        for (int j = 0; j < V; ++j) redf[rt * width + cv * V + j] = make_float2(sa[j], sb[j]);
+        if (one) put(reinterpret_cast<float2*>(red) + rt * width + cv * V, false);
     }
-    __syncthreads();
-    fold_rows(redf, width, p.rt);
-    __syncthreads();
-    for (int c = threadIdx.x; c < b.nvec * V; c += kNormThreads) by_channel[((size_t)n * p.splits + split) * d.C + b.c0 + c] = redf[c];
-    group_sums(redf, gamma, d, p, b,
-               [&](int g, double2 v) { by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = v; });
+    auto finish = [&](auto* pairs) {
+        __syncthreads();
+        fold_rows(pairs, width, p.rt);
+        __syncthreads();
+        for (int c = threadIdx.x; c < b.nvec * V; c += kNormThreads)
+            by_channel[((size_t)n * p.splits + split) * d.C + b.c0 + c] = make_float2((float)pairs[c].x, (float)pairs[c].y);
+        group_sums(pairs, gamma, d, p, b,
+                   [&](int g, double2 v) { by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = v; });
+    };
+    if (one) finish(reinterpret_cast<float2*>(red));
+    else finish(red);
 }
 
 template <typename T, int V>
@@ -645,7 +680,7 @@ norm_back_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
     Means<V> means;
     load_means<V>(stat, d, p, cv, col, means);
     const DropKey key = drop.on ? drop_key(drop) : DropKey{};
-    stream.template run<false>([&](int r, const Raw<T, V>(&v)[2]) {
+    stream.run_all([&](int r, const Raw<T, V>(&v)[2]) {
         const size_t i = at + (size_t)r * d.C;
         Lanes<V> du, e;
         back_du<T, V>(v[0], v[1], col, act, drop, key, i, du, e);
@@ -739,7 +774,7 @@ int backward(const T* dy, const T* x, const NormGiven& given, int ptype, const f
     } else {
         const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
         const size_t ring = norm_ring_bytes<T, V, 2, kBackRing>();
-        const size_t one = ring + sizeof(float2) * p.rt * p.tx * V, two = ring + sizeof(float2) * p.groups;
+        const size_t one = ring + sizeof(double2) * p.rt * p.tx * V, two = ring + sizeof(float2) * p.groups;
         if (!allow_shared(norm_back_sums_kernel<T, V>, one) || !allow_shared(norm_back_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
         norm_back_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_channel, by_group);
         if (launch_status()) return LINF_ERR_LAUNCH;

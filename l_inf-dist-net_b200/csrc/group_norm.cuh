@@ -88,6 +88,7 @@ struct NormKind { int elem_bytes, tensors; bool sums; };
 constexpr int kNormThreads = 256;
 constexpr int kNormKeepBytes = 64 * 1024; // of a CTA, so that an SM has three
 constexpr int kNormSplits = 64;           // CTAs that share a block's rows in the two passes: one of the second adds up that many sums
+constexpr int kNormSamples = 32;          // samples whose sums a kept CTA adds up in fp32 at most
 constexpr int kNormPlaces = 4;            // CTAs of the two passes that an SM has at a time, about
 
 inline int norm_ceil(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -152,6 +153,7 @@ inline bool norm_keep(const NormDims& d, const NormKind& kind, bool aligned, Nor
     // with per-channel sums: as many CTAs as run at a time, twice over; a CTA adds its samples up in order
     const long long resident = (long long)sm_count() * (2048 / p->threads < 16 ? 2048 / p->threads : 16) * 2;
     p->per_cta = kind.sums ? norm_ceil((long long)d.N * p->blocks, resident) : 1;
+    if (p->per_cta > kNormSamples) p->per_cta = kNormSamples;
     p->chunks = norm_ceil(d.N, p->per_cta);
     return true;
 }
@@ -212,6 +214,7 @@ inline int norm_make(int N, int C, int G, int L, const NormKind& kind, bool alig
 
 // One position (group_norm_dense.cu): a row of C/G values belongs to a slot of `tpr` threads; a CTA has slots for `groups` groups times `subs`
 // samples, and takes `per` samples.
+constexpr int kDenseSamples = 64;
 struct DensePlan { int V, tpr, threads, groups, subs, blocks, per, chunks; };
 struct NormGiven;
 bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, DensePlan* p);
@@ -260,7 +263,7 @@ __device__ __forceinline__ void by_columns(int width, int rows, Body body) {
     const int at_a_time = blockDim.x / lanes, mine = threadIdx.x / lanes, part = threadIdx.x - mine * lanes;
     for (int c0 = 0; c0 < width; c0 += at_a_time) {
         const int c = c0 + mine;
-        body(c, c < width ? part : rows, lanes, [&](float& s, float& t) {
+        body(c, c < width ? part : rows, lanes, [&](auto& s, auto& t) {
             for (int o = 1; o < lanes; o *= 2) {
                 s += __shfl_xor_sync(0xffffffffu, s, o);
                 t += __shfl_xor_sync(0xffffffffu, t, o);
@@ -301,7 +304,6 @@ __host__ __device__ constexpr size_t norm_ring_bytes() { return sizeof(T) * V >=
 // to shared memory at a time, each thread's to places of its own (`ring`: norm_ring_bytes), so that neither registers nor barriers limit
 // how much is read ahead (32 x 320 x 64 x 64 bf16, both passes: batches of 8 loads to registers 68 us, this 59 us).  Elements of two bytes that no wider copy
 // reaches come through registers.
-struct NoTurn { __device__ __forceinline__ void operator()() const {} };
 template <typename T, int V, int N, int S>
 struct NormStream {
     static constexpr int bytes = sizeof(T) * V, place = kNormThreads * bytes;      // ring: [S][N][threads]
@@ -310,7 +312,7 @@ struct NormStream {
     size_t stride;
     int r, r1, step, ahead;
 
-    // starts with the first rows on their way: what the CTA does before run(body(row, vectors)) overlaps with them
+    // starts with the first rows on their way: what the CTA does before run(rows, body(row, vectors)) overlaps with them
     __device__ __forceinline__ NormStream(void* ring, const T* const (&at)[N], int first, int end, int every, size_t C) {
         r = ahead = first;
         r1 = end;
@@ -344,43 +346,39 @@ struct NormStream {
         issue(s);                                               // behind body, which has used what it overwrites
         r += step;
     }
+    // The next `rows` rows of the thread, a multiple of S but for the last ones.
     // LIGHT bodies are written out for a whole turn of the ring: half the instructions (sums of bf16 maps: 52 -> 34 a vector, 24 -> 21 us);
-    // heavy ones are not, their code would be too long (38 -> 40 us).  turn(): after each S rows, the last ones excepted.
-    template <bool LIGHT, typename Body, typename Turn = NoTurn> __device__ __forceinline__ void run(Body body, Turn turn = Turn()) {
-        if constexpr (bytes >= 4) {
-            if constexpr (LIGHT) {
-                for (int turns = r < r1 ? ((r1 - r - 1) / step + 1) / S : 0; turns > 0; --turns) {
+    // heavy ones are not, their code would be too long (38 -> 40 us).
+    template <bool LIGHT, typename Body> __device__ __forceinline__ void run(int rows, Body body) {
+        const int end = r + rows * step;                        // below L + step
+        if constexpr (LIGHT && bytes >= 4) {
+            for (int turns = rows / S; turns > 0; --turns) {
 #pragma unroll
-                    for (int s = 0; s < S; ++s) row(s, body);
-                    turn();
-                }
+                for (int s = 0; s < S; ++s) row(s, body);
             }
-            if constexpr (LIGHT || std::is_same<Turn, NoTurn>::value) {
+        }
+        run_to(end, body);
+    }
+    template <typename Body> __device__ __forceinline__ void run_all(Body body) { run_to(r1, body); }
+    template <typename Body> __device__ __forceinline__ void run_to(int end, Body& body) {
+        if constexpr (bytes >= 4) {
 #pragma unroll 1
-                for (int s = 0; r < r1; s = s + 1 == S ? 0 : s + 1) row(s, body);
-            } else {
-#pragma unroll 1
-                for (int s = 0; r < r1;) {
-                    row(s, body);
-                    if (++s == S) { s = 0; turn(); }
-                }
-            }
+            for (int s = 0; r < end; s = s + 1 == S ? 0 : s + 1) row(s, body);
         } else {
             constexpr int K = S;
-            for (; r < r1; r += K * step) {
+            for (; r < end; r += K * step) {
                 Raw<T, V> v[K][N];
 #pragma unroll
                 for (int j = 0; j < K; ++j) {
 #pragma unroll
                     for (int k = 0; k < N; ++k) {
-                        if (r + j * step < r1) v[j][k] = load_raw<T, V>(next[k]);
+                        if (r + j * step < end) v[j][k] = load_raw<T, V>(next[k]);
                         next[k] += stride;
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < K; ++j)
-                    if (r + j * step < r1) body(r + j * step, v[j]);
-                turn();
+                    if (r + j * step < end) body(r + j * step, v[j]);
             }
         }
     }

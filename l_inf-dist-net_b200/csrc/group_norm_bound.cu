@@ -278,7 +278,7 @@ bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upp
         Sum4 s[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
-        stream.template run<true>([&](int, const Raw<float, V>(&v)[2]) { sum_vector<V>(v[0], v[1], s); });
+        stream.template run<true>(rows_of(norm_rows(d, p, split), rt), [&](int, const Raw<float, V>(&v)[2]) { sum_vector<V>(v[0], v[1], s); });
         put_sums<V>(red4, p, rt, cv, s);
     }
     __syncthreads();
@@ -322,7 +322,7 @@ bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ up
     if (!in) return;
     BoundColumn<V> col;
     load_column<V>(col, ends, gamma, beta, d, p, b, cv * V);
-    stream.template run<false>([&](int r, const Raw<float, V>(&v)[2]) {
+    stream.run_all([&](int r, const Raw<float, V>(&v)[2]) {
         write_bounds<V>(v[0], v[1], col, at + (size_t)r * d.C, act, out_l, out_u);
     });
 }

@@ -34,9 +34,9 @@ __device__ __forceinline__ DenseSlot dense_slot(const NormDims& d, const DensePl
     DenseSlot s;
     const int slot = threadIdx.x / p.tpr, sub = slot / p.groups;
     s.t = threadIdx.x - slot * p.tpr;
-    s.g = blockIdx.x * p.groups + slot - sub * p.groups;
+    s.g = blockIdx.y * p.groups + slot - sub * p.groups;
     s.in = sub < p.subs && s.g < d.G;
-    s.n0 = blockIdx.y * p.per;
+    s.n0 = blockIdx.x * p.per;
     s.n1 = min(d.N, s.n0 + p.per);
     s.first = s.n0 + sub;
     s.iters = (s.n1 - s.n0 + p.subs - 1) / p.subs;              // the same for the whole CTA
@@ -181,7 +181,7 @@ dense_norm_back_kernel(const T* __restrict__ dy, const T* __restrict__ x, Param 
                 store_once<T, V>(dx + row + (s.t + k * p.tpr) * V, raw_of<T, V>(mul(fma(h[k], mb, add(du[k], ma)), scale)));
     }
     if (!s.in) return;
-    float2* to = by_channel + ((size_t)blockIdx.y * p.subs + (s.first - s.n0)) * d.C + s.g * d.Cg;
+    float2* to = by_channel + ((size_t)blockIdx.x * p.subs + (s.first - s.n0)) * d.C + s.g * d.Cg;
 #pragma unroll
     for (int k = 0; k < K; ++k)
         if (s.t + k * p.tpr < vecs) {
@@ -197,7 +197,8 @@ template <int V> struct DenseK { static constexpr int value = V == 8 ? 2 : 4; };
 
 }  // namespace
 
-// Whether a slot can hold a row; its plan.  ctas: CTAs that the call should have at least, as far as there are samples.
+// Whether a slot can hold a row; its plan.  ctas: CTAs that the call should have at least, as far as there are samples; a slot takes
+// kDenseSamples of them at most, whose sums for the parameters' gradients it adds up in fp32.
 bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, DensePlan* p) {
     if (d.L != 1) return false;
     const int widths[4] = {16 / elem_bytes, 8 / elem_bytes, 4 / elem_bytes, 1};
@@ -216,9 +217,10 @@ bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, Dense
     p->groups = d.G < slots ? d.G : slots;
     p->subs = slots / p->groups;
     p->blocks = norm_ceil(d.G, p->groups);
+    if (p->blocks > 65535) return false;
     long long chunks = norm_ceil(ctas, p->blocks);
     if (chunks > norm_ceil(d.N, p->subs)) chunks = norm_ceil(d.N, p->subs);
-    if (chunks > 65535) chunks = 65535;
+    if (chunks < norm_ceil(d.N, (long long)p->subs * kDenseSamples)) chunks = norm_ceil(d.N, (long long)p->subs * kDenseSamples);
     p->per = norm_ceil(d.N, chunks);
     p->chunks = norm_ceil(d.N, p->per);
     return true;
@@ -247,7 +249,7 @@ template <typename T, int V>
 int go_forward(const void* x, const NormGiven& given, const NormDims& d, const DensePlan& p, double eps, int act, const Drop& drop, void* y, float* mean,
                float* rstd, cudaStream_t st) {
     const auto kernel = dense_norm_kernel<T, V, DenseK<V>::value>;
-    const dim3 grid(p.blocks, p.chunks);
+    const dim3 grid(p.chunks, p.blocks);
     kernel<<<grid, p.threads, 0, st>>>(static_cast<const T*>(x), given.gamma, given.beta, d, p, eps, act, drop, static_cast<T*>(y), mean, rstd);
     return launch_status();
 }
@@ -255,7 +257,7 @@ template <typename T, int V>
 int go_backward(const void* dy, const void* x, const NormGiven& given, const float* mean, const float* rstd, const NormDims& d, const DensePlan& p, int act,
                 const Drop& drop, void* dx, float2* by_channel, cudaStream_t st) {
     const auto kernel = dense_norm_back_kernel<T, V, DenseK<V>::value>;
-    const dim3 grid(p.blocks, p.chunks);
+    const dim3 grid(p.chunks, p.blocks);
     kernel<<<grid, p.threads, 0, st>>>(static_cast<const T*>(dy), static_cast<const T*>(x), given.gamma, given.beta, mean, rstd, d, p, act, drop,
                                        static_cast<T*>(dx), by_channel);
     return launch_status();

@@ -79,3 +79,28 @@ def test_values_very_far_from_zero(cuda, lib, case):
     most = 16 * E * (1 + h.abs()) + E * E * r * mean.abs()
     y = L.group_norm(x, groups, eps=EPS)
     assert_within(y.reshape(h.shape), h, most, "values")
+
+
+# (N, C, groups, positions, additions in a row before: the gradient below is the one that many of them lose most with)
+CONSTANT = [(1, 1024, 32, 131072, 2048), (1, 255, 5, 300000, 2048), (444 * 256 * 512, 8, 1, 1, 512)]
+
+
+@gpu
+@pytest.mark.parametrize("case", CONSTANT, ids=lambda c: "N{}_C{}_G{}_L{}".format(*c[:4]))
+def test_constant_gradients_over_long_columns(cuda, lib, case):
+    """A gradient that is the same everywhere: every addition in a row rounds the same way, by up to half a step.
+
+    64 additions of equal terms in fp32 are off by at most E (64 + 1) / 2 of the sum; the partial sum is rounded once before 64-bit sums take over, and
+    so is the result: 36 E of the terms' sizes.  The weight's terms have h, off by 10 E (1 + |h|) of itself, besides."""
+    N, C, groups, n, adds = case
+    c = 1 + 0.499 * 2.0 ** (math.log2(adds) - 24)
+    x = stored(N, C, n, torch.float32, sum(case) % 1000)
+    x = (x if n > 1 else x.reshape(N, C)).requires_grad_()
+    w, b = torch.ones(C, device="cuda", requires_grad=True), torch.zeros(C, device="cuda", requires_grad=True)
+    y = L.group_norm(x, groups, w, b, EPS)
+    gx, gw, gb = torch.autograd.grad(y, (x, w, b), torch.full_like(y, c))
+    del y, gx
+    c = torch.tensor(c).double().item()          # as fp32 has it
+    assert_within(gb, torch.full((C,), N * n * c, dtype=torch.float64, device="cuda"), 36 * E * N * n * c, "grad_bias")
+    h = parts(x.view(N, C, n), groups)[0].view(N, C, n)
+    assert_within(gw, c * h.sum((0, 2)), c * ((36 + 10) * E * h.abs().sum((0, 2)) + 10 * E * N * n), "grad_weight")
