@@ -145,8 +145,10 @@ __device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<fl
     }
 }
 
-// What the forward pass needs of a box, in fp32; the means as a sum of two.
-struct Ends32 { float ml, ml2, mu, mu2, s_lo, s_hi; };
+// What the forward pass needs of a box, in fp32; the means as a sum of two.  far: differences from a mean may be beyond fp32, and s_lo and s_hi below its
+// normal numbers: differences are taken as kFar of themselves then, s_lo and s_hi as 1 / kFar times theirs (both exact).
+constexpr float kFar = 1.f / 16.f;
+struct Ends32 { float ml, ml2, mu, mu2, s_lo, s_hi; bool far; };
 __device__ __forceinline__ Ends32 make_ends32(const Sum4& s, const NormDims& d, double eps) {
     const Box b = make_box(s, d, eps);
     Ends32 e;
@@ -154,12 +156,14 @@ __device__ __forceinline__ Ends32 make_ends32(const Sum4& s, const NormDims& d, 
     e.ml2 = (float)(b.mean_l - e.ml);
     e.mu = (float)b.mean_u;
     e.mu2 = (float)(b.mean_u - e.mu);
-    e.s_lo = (float)b.s_lo;
-    e.s_hi = (float)b.s_hi;
+    // |x - mean| <= sqrt(M) (sd + rho) at both ends, whose means are 2 rho apart at most; not where they are no number
+    e.far = 3.0 * (b.cut + 1.0) * (b.sd + b.rho) >= 3e38;
+    e.s_lo = (float)(e.far ? b.s_lo / kFar : b.s_lo);
+    e.s_hi = (float)(e.far ? b.s_hi / kFar : b.s_hi);
     return e;
 }
-// ... and of the channels of a thread's column
-template <int V> struct BoundColumn { Ends32 e[V]; float w[V], o[V], inv_m2, cut; };
+// ... and of the channels of a thread's column; h: 1, or kFar where one of them has far ends
+template <int V> struct BoundColumn { Ends32 e[V]; float w[V], o[V], inv_m2, cut, h; };
 template <int V>
 __device__ __forceinline__ void load_column(BoundColumn<V>& k, const Ends32* ends, const Param& gamma, const Param& beta, const NormDims& d,
                                             const NormPlan& p, const NormBlock& b, int c) {
@@ -169,7 +173,21 @@ __device__ __forceinline__ void load_column(BoundColumn<V>& k, const Ends32* end
     load_params<V>(beta, b.c0 + c, k.o);
 #pragma unroll
     for (int j = 0; j < V; ++j) k.e[j] = ends[g[j]];
-    k.inv_m2 = 2.f * (float)d.inv_m;
+    bool far = false;
+#pragma unroll
+    for (int j = 0; j < V; ++j) far = far || k.e[j].far;
+    k.h = far ? kFar : 1.f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float up = far && !k.e[j].far ? 1.f / kFar : 1.f;
+        k.e[j].s_lo *= up;
+        k.e[j].s_hi *= up;
+        k.e[j].ml *= k.h;
+        k.e[j].ml2 *= k.h;
+        k.e[j].mu *= k.h;
+        k.e[j].mu2 *= k.h;
+    }
+    k.inv_m2 = 2.f * (float)d.inv_m * k.h;
     k.cut = sqrtf((float)((double)d.L * d.Cg - 1.0));
 }
 
@@ -183,7 +201,7 @@ __device__ __forceinline__ void write_bounds(const Raw<float, V>& lv, const Raw<
     for (int j = 0; j < V; ++j) {
         const Ends32& e = k.e[j];
         const float own = fmaf(u[j], 0.5f, -0.5f * l[j]) * k.inv_m2;      // the width halved: it may be beyond fp32
-        const float n0 = ((l[j] - e.mu) - e.mu2) + own, n1 = ((u[j] - e.ml) - e.ml2) - own;
+        const float n0 = (fmaf(l[j], k.h, -e.mu) - e.mu2) + own, n1 = (fmaf(u[j], k.h, -e.ml) - e.ml2) - own;
         float z0 = n0 * (n0 >= 0.f ? e.s_lo : e.s_hi), z1 = n1 * (n1 >= 0.f ? e.s_hi : e.s_lo);
         z0 = z0 <= -k.cut ? -k.cut : z0;                        // a NaN stays
         z1 = z1 >= k.cut ? k.cut : z1;

@@ -104,3 +104,31 @@ def test_constant_gradients_over_long_columns(cuda, lib, case):
     assert_within(gb, torch.full((C,), N * n * c, dtype=torch.float64, device="cuda"), 36 * E * N * n * c, "grad_bias")
     h = parts(x.view(N, C, n), groups)[0].view(N, C, n)
     assert_within(gw, c * h.sum((0, 2)), c * ((36 + 10) * E * h.abs().sum((0, 2)) + 10 * E * N * n), "grad_weight")
+
+
+# (N, C, groups, positions): dense, kept, kept with vectors across groups, the two passes
+EDGE = [(1, 4, 1, 1), (3, 64, 4, 1), (2, 24, 4, 30), (2, 24, 12, 30), (1, 16, 2, 22500)]
+
+
+@gpu
+@pytest.mark.parametrize("act", ["identity", "tanh"])
+@pytest.mark.parametrize("case", EDGE, ids=lambda c: "N{}_C{}_G{}_L{}".format(*c))
+def test_boxes_at_the_edge_of_fp32(cuda, lib, case, act):
+    """Values whose distance from their mean is beyond fp32: the bounds are ordered and those of the formulas.
+
+    The differences are taken in 64 bits, 1 / deviation is a normal number (2^64 times as large): each rounded once, their product once, then a
+    bound's own roundings: 8 E of it (weights 1, biases 0), and tanhf's 4 E."""
+    N, C, groups, n = case
+    gen = torch.Generator().manual_seed(sum(case))
+    x = 3e38 * torch.where(torch.rand(N, C, n, generator=gen) < 0.25, 1.0, -1.0)
+    x[:, ::C // groups, 0] = 3e38                    # one at least in each group, and one that is not
+    x[:, C // groups - 1::C // groups, n - 1] = -3e38
+    lo, up = x, (x.double() + 1e37 * torch.rand(x.shape, generator=gen).double()).float()
+    if n == 1:
+        lo, up = lo[..., 0], up[..., 0]
+    for low, high in ((lo, up), (lo, lo)):
+        want = R.group_norm_bound(low.double(), high.double(), groups, None, None, EPS, act)
+        got = [t.cpu() for t in L.group_norm_bound(low.cuda(), high.cuda(), groups, eps=EPS, activation=act)]
+        assert torch.isfinite(got[0]).all() and (got[0] <= got[1]).all()
+        for g, w, what in zip(got, want, ("lower", "upper")):
+            assert_within(g, w, 12 * E * w.abs() + 8 * E * (1 if act == "tanh" else 0), what)
