@@ -27,11 +27,18 @@ struct Box {
     double s_lo, s_hi, cut;             // range of 1 / sqrt(var + eps); sqrt(M - 1)
 };
 
-__device__ __forceinline__ Box make_box(const Sum4& s, const NormDims& d, double eps) {
+// One value of each group of sample n from group g0 on, each d.Cg apart (the first lower end of a row in the middle).  The squares of the centres are
+// taken about it: boxes far from 0 against their spread would lose the spread in the difference of two large sums.
+__device__ __forceinline__ const float* level_of(const float* lower, const NormDims& d, int n, int g0) {
+    return lower + ((size_t)n * d.L + d.L / 2) * d.C + (size_t)g0 * d.Cg;
+}
+
+// s: the sums of l, u, (l + u - 2 level)^2, (u - l)^2
+__device__ __forceinline__ Box make_box(const Sum4& s, double level, const NormDims& d, double eps) {
     Box b;
     b.mean_l = s.a * d.inv_m;
     b.mean_u = s.b * d.inv_m;
-    const double mc = (b.mean_l + b.mean_u) * 0.5, vc = 0.25 * s.c * d.inv_m - mc * mc, vr = 0.25 * s.d * d.inv_m;
+    const double mc = (b.mean_l + b.mean_u) * 0.5 - level, vc = 0.25 * s.c * d.inv_m - mc * mc, vr = 0.25 * s.d * d.inv_m;
     b.sd = sqrt(vc > 0.0 || vc != vc ? vc : 0.0);
     b.rho = sqrt(vr);
     const double far = b.sd + b.rho, near = fmax(b.sd - b.rho, 0.0) + (b.sd - b.rho) * 0.0;     // keeps a NaN
@@ -129,9 +136,24 @@ __device__ __forceinline__ Back make_back(const Box& x, const Sum4& t, const Nor
 
 __device__ __forceinline__ int group_of(const NormDims& d, const NormPlan& p, int c) { return p.pieces == 1 ? p.by_cg(c) : 0; }
 
-// Adds l, u, (l + u)^2, (u - l)^2 of a vector up.
-template <int V>
-__device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<float, V>& uv, Sum4 (&s)[V]) {
+// Twice the levels of a column's channels (SAME: of its one group).
+template <int V, bool SAME> struct Levels {
+    double twice[SAME ? 1 : V];
+    __device__ __forceinline__ Levels(const float* base, const NormDims& d, const NormPlan& p, int c) {
+        if constexpr (SAME) {
+            twice[0] = 2.0 * base[p.pieces == 1 ? p.by_cg(c) * d.Cg : 0];
+        } else {
+            int g[V];
+            groups_of<V>(d, p, c, g);
+#pragma unroll
+            for (int j = 0; j < V; ++j) twice[j] = 2.0 * base[g[j] * d.Cg];
+        }
+    }
+};
+
+// Adds l, u, (l + u - 2 level)^2, (u - l)^2 of a vector up.
+template <int V, bool SAME>
+__device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<float, V>& uv, const Levels<V, SAME>& level, Sum4 (&s)[V]) {
     float l[V], u[V];
     unpack<float, V>(lv, l);
     unpack<float, V>(uv, u);
@@ -140,7 +162,8 @@ __device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<fl
         const double a = l[j], e = u[j];
         s[j].a += a;
         s[j].b += e;
-        s[j].c = ::fma(a + e, a + e, s[j].c);
+        const double twice = a + e - level.twice[SAME ? 0 : j];
+        s[j].c = ::fma(twice, twice, s[j].c);
         s[j].d = ::fma(e - a, e - a, s[j].d);
     }
 }
@@ -149,8 +172,8 @@ __device__ __forceinline__ void sum_vector(const Raw<float, V>& lv, const Raw<fl
 // normal numbers: differences are taken as kFar of themselves then, s_lo and s_hi as 1 / kFar times theirs (both exact).
 constexpr float kFar = 1.f / 16.f;
 struct Ends32 { float ml, ml2, mu, mu2, s_lo, s_hi; bool far; };
-__device__ __forceinline__ Ends32 make_ends32(const Sum4& s, const NormDims& d, double eps) {
-    const Box b = make_box(s, d, eps);
+__device__ __forceinline__ Ends32 make_ends32(const Sum4& s, double level, const NormDims& d, double eps) {
+    const Box b = make_box(s, level, d, eps);
     Ends32 e;
     e.ml = (float)b.mean_l;
     e.ml2 = (float)(b.mean_l - e.ml);
@@ -233,8 +256,8 @@ __host__ __device__ inline BoundSpace bound_space(const NormPlan& p, int tensors
     return s;
 }
 
-template <int V>
-__global__ void __launch_bounds__(kNormThreads)
+template <int V, bool SAME>
+__global__ void __launch_bounds__(kNormThreads, 4)
 bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upper, Param gamma, Param beta, NormDims d, NormPlan p, double eps, int act,
                   float* __restrict__ out_l, float* __restrict__ out_u, Sum4* __restrict__ sums) {
     extern __shared__ uint4 space[];
@@ -250,6 +273,7 @@ bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upp
     const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
     float* own_l = data + c;
     float* own_u = own_l + (size_t)p.rows * pitch;
+    const Levels<V, SAME> level(level_of(lower, d, n, b.g0), d, p, in ? c : 0);
     for (int r = rt; r < r1; r += p.rt) {
         keep_vector<float, V>(own_l + r * pitch, lower + at + (size_t)r * d.C);
         keep_vector<float, V>(own_u + r * pitch, upper + at + (size_t)r * d.C);
@@ -260,12 +284,12 @@ bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upp
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
 #pragma unroll 2
-        for (int r = rt; r < r1; r += p.rt) sum_vector<V>(load_raw<float, V>(own_l + r * pitch), load_raw<float, V>(own_u + r * pitch), s);
+        for (int r = rt; r < r1; r += p.rt) sum_vector<V, SAME>(load_raw<float, V>(own_l + r * pitch), load_raw<float, V>(own_u + r * pitch), level, s);
         put_sums<V>(red, p, rt, cv, s);
     }
     __syncthreads();
     group_sums(red, d, p, b, [&](int g, const Sum4& s) {
-        ends[g] = make_ends32(s, d, eps);
+        ends[g] = make_ends32(s, data[(d.L / 2) * pitch + g * d.Cg], d, eps);       // the level, as it was kept
         if (sums != nullptr) sums[(size_t)n * d.G + b.g0 + g] = s;
     });
     __syncthreads();
@@ -280,7 +304,7 @@ bound_kept_kernel(const float* __restrict__ lower, const float* __restrict__ upp
 
 constexpr int kBoundRing = 4;              // rows that are on their way at a time
 
-template <int V>
+template <int V, bool SAME>
 __global__ void __launch_bounds__(kNormThreads, 3)
 bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upper, NormDims d, NormPlan p, Sum4* __restrict__ part) {
     extern __shared__ uint4 space[];                            // the ring, then [rt][tx] or [rt][tx * V]
@@ -293,10 +317,11 @@ bound_sums_kernel(const float* __restrict__ lower, const float* __restrict__ upp
         const float* const from[2] = {lower + at, upper + at};
         NormStream<float, V, 2, kBoundRing> stream(space, from, split * p.rt + rt, d.L, p.splits * p.rt, d.C);
         grid_let_go();
+        const Levels<V, SAME> level(level_of(lower, d, n, b.g0), d, p, cv * V);
         Sum4 s[V];
 #pragma unroll
         for (int j = 0; j < V; ++j) s[j] = Sum4{0.0, 0.0, 0.0, 0.0};
-        stream.template run<true>(rows_of(norm_rows(d, p, split), rt), [&](int, const Raw<float, V>(&v)[2]) { sum_vector<V>(v[0], v[1], s); });
+        stream.template run<true>(rows_of(norm_rows(d, p, split), rt), [&](int, const Raw<float, V>(&v)[2]) { sum_vector<V, SAME>(v[0], v[1], level, s); });
         put_sums<V>(red4, p, rt, cv, s);
     }
     __syncthreads();
@@ -328,11 +353,13 @@ bound_apply_kernel(const float* __restrict__ lower, const float* __restrict__ up
     const size_t at = ((size_t)n * d.L) * d.C + b.c0 + cv * V;
     const float* const from[2] = {lower + at, upper + at};
     NormStream<float, V, 2, kBoundRing> stream(space, from, split * p.rt + rt, in ? d.L : 0, p.splits * p.rt, d.C);
+    const float* base = level_of(lower, d, n, b.g0);
     grid_wait();
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
+        const float level = base[(size_t)g * d.Cg];
         const Sum4 t = all_parts(part, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
-            ends[g] = make_ends32(t, d, eps);
+            ends[g] = make_ends32(t, level, d, eps);
             if (split == 0 && b.piece == 0 && sums != nullptr) sums[(size_t)n * d.G + b.g0 + g] = t;
         }
     }
@@ -434,7 +461,7 @@ __device__ __forceinline__ void put_channels(float2* red, const NormPlan& p, con
 }
 
 template <int V>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, 2)
 bound_back_kept_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict__ sums, NormDims d, NormPlan p, double eps, int act,
                        float* __restrict__ d_l, float* __restrict__ d_u, float2* __restrict__ by_channel) {
     extern __shared__ uint4 space[];
@@ -468,7 +495,7 @@ bound_back_kept_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
             keep_vector<float, V>(own + 2 * tensor + r * pitch, in4.g_l + i);
             keep_vector<float, V>(own + 3 * tensor + r * pitch, in4.g_u + i);
         }
-        for (int g = threadIdx.x; g < b.ng; g += blockDim.x) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
+        for (int g = threadIdx.x; g < b.ng; g += blockDim.x) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], level_of(in4.lower, d, n, b.g0)[(size_t)g * d.Cg], d, eps);
         keep_wait();
         __syncthreads();
         if (in) {
@@ -498,7 +525,7 @@ bound_back_kept_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
 }
 
 template <int V>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, 2)
 bound_back_sums_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict__ sums, NormDims d, NormPlan p, double eps, int act,
                        float2* __restrict__ by_channel, Sum4* __restrict__ by_group) {
     extern __shared__ uint4 space[];
@@ -507,7 +534,7 @@ bound_back_sums_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
     Box* box = reinterpret_cast<Box*>(reinterpret_cast<char*>(space) + at_.box);
     const int n = p.by_blocks(blockIdx.x), split = blockIdx.y;
     const NormBlock b = norm_block<V>(d, p, blockIdx.x - n * p.blocks);
-    for (int g = threadIdx.x; g < b.ng; g += kNormThreads) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
+    for (int g = threadIdx.x; g < b.ng; g += kNormThreads) box[g] = make_box(sums[(size_t)n * d.G + b.g0 + g], level_of(in4.lower, d, n, b.g0)[(size_t)g * d.Cg], d, eps);
     __syncthreads();
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
     const bool in = rt < p.rt && cv < b.nvec;
@@ -546,7 +573,7 @@ bound_back_apply_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict
     for (int g = threadIdx.x >> 5; g < b.ng; g += kNormThreads / 32) {
         const Sum4 t = all_parts(by_group, d, p, n, b.g0 + g);
         if ((threadIdx.x & 31) == 0) {
-            const Box x = make_box(sums[(size_t)n * d.G + b.g0 + g], d, eps);
+            const Box x = make_box(sums[(size_t)n * d.G + b.g0 + g], level_of(in4.lower, d, n, b.g0)[(size_t)g * d.Cg], d, eps);
             box[g] = x;
             back[g] = make_back(x, t, d);
         }
@@ -575,20 +602,27 @@ size_t workspace(const NormDims& d, const NormPlan& p, bool back) {
     return parts_bytes(d, p) + (back ? sizeof(float2) * (size_t)channel_rows(p) * d.C : 0);
 }
 
-template <int V>
-int forward(const float* lower, const float* upper, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, float* out_l,
-            float* out_u, Sum4* sums, void* ws, cudaStream_t st) {
+template <int V, bool SAME>
+int forward_as(const float* lower, const float* upper, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, float* out_l,
+               float* out_u, Sum4* sums, void* ws, cudaStream_t st) {
     if (p.kept)
-        return launch_kept(bound_kept_kernel<V>, p, bound_space<V>(p, 2).bytes, st, lower, upper, given.gamma, given.beta, d, p, eps, act, out_l,
+        return launch_kept(bound_kept_kernel<V, SAME>, p, bound_space<V>(p, 2).bytes, st, lower, upper, given.gamma, given.beta, d, p, eps, act, out_l,
                            out_u, sums);
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     Sum4* part = static_cast<Sum4*>(ws);
     const size_t ring = norm_ring_bytes<float, V, 2, kBoundRing>(), one = ring + bound_space<V>(p, 0).box, two = ring + sizeof(Ends32) * p.groups;
-    if (!allow_shared(bound_sums_kernel<V>, one) || !allow_shared(bound_apply_kernel<V>, two)) return LINF_ERR_LAUNCH;
-    bound_sums_kernel<V><<<grid, kNormThreads, one, st>>>(lower, upper, d, p, part);
+    if (!allow_shared(bound_sums_kernel<V, SAME>, one) || !allow_shared(bound_apply_kernel<V>, two)) return LINF_ERR_LAUNCH;
+    bound_sums_kernel<V, SAME><<<grid, kNormThreads, one, st>>>(lower, upper, d, p, part);
     if (launch_status()) return LINF_ERR_LAUNCH;
     return launch_behind(bound_apply_kernel<V>, grid, kNormThreads, two, st, lower, upper, given.gamma, given.beta, part, d, p, eps, act, out_l, out_u,
                          sums);
+}
+template <int V>
+int forward(const float* lower, const float* upper, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, float* out_l,
+            float* out_u, Sum4* sums, void* ws, cudaStream_t st) {
+    if constexpr (V > 1)
+        if (!p.same) return forward_as<V, false>(lower, upper, given, d, p, eps, act, out_l, out_u, sums, ws, st);
+    return forward_as<V, true>(lower, upper, given, d, p, eps, act, out_l, out_u, sums, ws, st);
 }
 
 template <int V>

@@ -132,3 +132,28 @@ def test_boxes_at_the_edge_of_fp32(cuda, lib, case, act):
         assert torch.isfinite(got[0]).all() and (got[0] <= got[1]).all()
         for g, w, what in zip(got, want, ("lower", "upper")):
             assert_within(g, w, 12 * E * w.abs() + 8 * E * (1 if act == "tanh" else 0), what)
+
+
+@gpu
+@pytest.mark.parametrize("case", FAR, ids=lambda c: "N{}_C{}_G{}_L{}".format(*c))
+def test_boxes_very_far_from_zero(cuda, lib, case):
+    """Boxes around values of 10^6 deviations: the deviation is that of the formulas, the bounds are ordered, and a value is within the bounds of its own
+    box.
+
+    The 64-bit squares are taken about a value of the group, so 1 / deviation is as good as exact before it is rounded: E.  Differences from a
+    mean in two parts, twice rounded, own three times; the product: 12 E (1 + |bound|), with n below 2 |bound| + 1 deviations of the centres."""
+    N, C, groups, n = case
+    lo = stored(N, C, n, torch.float32, sum(case), level=5e5)
+    up = lo + 0.0625 * torch.randint(0, 3, lo.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    if n == 1:
+        lo, up = lo.reshape(N, C), up.reshape(N, C)
+    for low, high in ((lo, up), (lo, lo)):
+        one = torch.ones(C, dtype=torch.float64, device="cuda")
+        want = R.group_norm_bound(low.double(), high.double(), groups, one, 0 * one, EPS, "identity")
+        got = L.group_norm_bound(low, high, groups, eps=EPS)
+        assert (got[0] <= got[1]).all()
+        for g, w, what in zip(got, want, ("lower", "upper")):
+            assert_within(g, w, 12 * E * (1 + w.abs()), what)
+    value = L.group_norm(lo, groups, eps=EPS)
+    room = 28 * E * (1 + value.abs())                       # 16 of the value, 12 of the bound
+    assert (got[0] - room <= value).all() and (value <= got[1] + room).all()
