@@ -11,7 +11,8 @@
 // 0.  The elements of the forward pass, whose values do not jump there, are fp32, with the means in two parts, so that no bound is off by more
 // than a few roundings of its own terms.  Forward passes are bound by HBM, backward passes by
 // the 64-bit units.  Measured on one B200, us: 32 x 192 x 56 x 56, relu, forward 95 (elements in 64 bits: 119; 47 if all crossed HBM once); 16 x 192 x
-// 56 x 56, tanh, both directions 231; 512 x 512, 16 groups, tanh, both 24.
+// 56 x 56, tanh, both directions 231; 512 x 512, 16 groups, tanh, both 24.  Of the backward pass the activation's slope and its product with a
+// gradient are fp32, and so are the partial sums for gamma and beta that a CTA leaves behind.
 #include "group_norm.cuh"
 
 namespace linf {
@@ -248,7 +249,7 @@ struct BoundSpace { size_t red, box, back, bytes; };
 template <int V>
 __host__ __device__ inline BoundSpace bound_space(const NormPlan& p, int tensors) {
     BoundSpace s;
-    const size_t four = sizeof(Sum4) * p.rt * p.tx * (p.same ? 1 : V), two = sizeof(float2) * p.rt * p.tx * V;
+    const size_t four = sizeof(Sum4) * p.rt * p.tx * (p.same ? 1 : V), two = sizeof(double2) * p.rt * p.tx * V;
     s.red = tensors > 0 ? ((size_t)p.rows * p.tx * V * sizeof(float) * tensors + 15) / 16 * 16 : 0;
     s.box = s.red + ((four > two ? four : two) + 15) / 16 * 16;
     s.back = s.box + sizeof(Box) * p.groups;
@@ -393,7 +394,7 @@ struct In4 { const float *g_l, *g_u, *lower, *upper; };
 template <int V>
 __device__ __forceinline__ void sum_back(const Raw<float, V>& lv, const Raw<float, V>& uv, const Raw<float, V>& glv, const Raw<float, V>& guv,
                                          const Box* box, const float (&w)[V], const float (&o)[V], const NormDims& d, const NormPlan& p, int c, int act,
-                                         Sum4 (&s)[V], float2 (&by)[V]) {
+                                         Sum4 (&s)[V], double2 (&by)[V]) {
     float l[V], u[V], gl[V], gu[V];
     unpack<float, V>(lv, l);
     unpack<float, V>(uv, u);
@@ -404,8 +405,8 @@ __device__ __forceinline__ void sum_back(const Raw<float, V>& lv, const Raw<floa
         const Ends e = make_ends(box[group_of(d, p, c + j)], l[j], u[j], d.inv_m);
         double q0, q1, dw, db;
         bound_dz(e, w[j], o[j], act, gl[j], gu[j], q0, q1, dw, db);
-        by[j].x += (float)db;
-        by[j].y += (float)dw;
+        by[j].x += db;
+        by[j].y += dw;
         s[j].a = ::fma(q0, e.s0, s[j].a);
         s[j].b = ::fma(q1, e.s1, s[j].b);
         const double t0 = q0 * e.n0, t1 = q1 * e.n1;
@@ -444,7 +445,7 @@ __device__ __forceinline__ void write_back(const Raw<float, V>& lv, const Raw<fl
 
 // Per-channel sums of a CTA's threads, added up along the rows and written to `to`; red is free before and after.
 template <int V>
-__device__ __forceinline__ void put_channels(float2* red, const NormPlan& p, const NormBlock& b, int rt, int cv, const float2 (&by)[V], float2* to) {
+__device__ __forceinline__ void put_channels(double2* red, const NormPlan& p, const NormBlock& b, int rt, int cv, const double2 (&by)[V], float2* to) {
     const int width = p.tx * V;
     __syncthreads();
     if (rt < p.rt) {
@@ -479,12 +480,12 @@ bound_back_kept_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
     const size_t tensor = (size_t)p.rows * pitch;
     float* own = data + c;                                      // lower, upper and their gradients, one behind the other
     float w[V], o[V];
-    float2 by[V];
+    double2 by[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         w[j] = in ? load_param(gamma, b.c0 + c + j) : 1.f;
         o[j] = in ? load_param(beta, b.c0 + c + j) : 0.f;
-        by[j] = make_float2(0.f, 0.f);
+        by[j] = make_double2(0.0, 0.0);
     }
     for (int n = chunk * p.per_cta; n < n1; ++n) {
         const size_t at = ((size_t)n * d.L) * d.C + b.c0 + c;
@@ -521,7 +522,7 @@ bound_back_kept_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
             }
         __syncthreads();
     }
-    put_channels<V>(reinterpret_cast<float2*>(red), p, b, rt, cv, by, by_channel + (size_t)chunk * d.C + b.c0);
+    put_channels<V>(reinterpret_cast<double2*>(red), p, b, rt, cv, by, by_channel + (size_t)chunk * d.C + b.c0);
 }
 
 template <int V>
@@ -539,9 +540,9 @@ bound_back_sums_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
     const int rt = p.by_tx(threadIdx.x), cv = threadIdx.x - rt * p.tx, c = cv * V;
     const bool in = rt < p.rt && cv < b.nvec;
     Sum4 s[V];
-    float2 by[V];
+    double2 by[V];
 #pragma unroll
-    for (int j = 0; j < V; ++j) { s[j] = Sum4{0.0, 0.0, 0.0, 0.0}; by[j] = make_float2(0.f, 0.f); }
+    for (int j = 0; j < V; ++j) { s[j] = Sum4{0.0, 0.0, 0.0, 0.0}; by[j] = make_double2(0.0, 0.0); }
     if (in) {
         float w[V], o[V];
         load_params<V>(gamma, b.c0 + c, w);
@@ -553,7 +554,7 @@ bound_back_sums_kernel(In4 in4, Param gamma, Param beta, const Sum4* __restrict_
                         load_raw<float, V>(in4.g_u + i), box, w, o, d, p, c, act, s, by);
         }
     }
-    put_channels<V>(reinterpret_cast<float2*>(red), p, b, rt, cv, by, by_channel + ((size_t)n * p.splits + split) * d.C + b.c0);
+    put_channels<V>(reinterpret_cast<double2*>(red), p, b, rt, cv, by, by_channel + ((size_t)n * p.splits + split) * d.C + b.c0);
     if (in) put_sums<V>(red, p, rt, cv, s);
     __syncthreads();
     group_sums(red, d, p, b, [&](int g, const Sum4& q) { by_group[(((size_t)n * p.splits + split) * d.G + b.g0 + g) * p.pieces + b.piece] = q; });

@@ -157,3 +157,23 @@ def test_boxes_very_far_from_zero(cuda, lib, case):
     value = L.group_norm(lo, groups, eps=EPS)
     room = 28 * E * (1 + value.abs())                       # 16 of the value, 12 of the bound
     assert (got[0] - room <= value).all() and (value <= got[1] + room).all()
+
+
+@gpu
+@pytest.mark.parametrize("case", [(1, 1024, 32, 131072, 1024), (148 * 6 * 300, 64, 4, 2, 256)], ids=lambda c: "N{}_C{}_G{}_L{}".format(*c[:4]))
+def test_constant_gradients_of_boxes_over_long_columns(cuda, lib, case):
+    """As above, for the parameters of the bounds: 64-bit sums of a CTA's rows and samples, rounded once (E), then 64-bit sums, rounded once; the slope's
+    product with the gradient is exact here.  The weight's terms have z, which is that of the formulas, to 64 bits."""
+    N, C, groups, n, adds = case
+    c = (1 + 0.499 * 2.0 ** (math.log2(adds) - 24)) / 2
+    lo = stored(N, C, n, torch.float32, sum(case) % 1000)
+    up = lo + 0.01
+    w, b = torch.ones(C, device="cuda", requires_grad=True), torch.zeros(C, device="cuda", requires_grad=True)
+    ys = L.group_norm_bound(lo, up, groups, w, b, EPS)
+    g = torch.full_like(lo, c)
+    gw, gb = torch.autograd.grad(ys, (w, b), (g, g))
+    c = torch.tensor(c).double().item()
+    assert_within(gb, torch.full((C,), 2 * N * n * c, dtype=torch.float64, device="cuda"), 3 * E * 2 * N * n * c, "grad_bias")
+    z = sum(y.detach().double() for y in ys)                   # fp32, off by less than 12 E (1 + |z|) each
+    size = sum((y.detach().double().abs() + 1).sum((0, 2)) for y in ys)
+    assert_within(gw, c * z.sum((0, 2)), c * 16 * E * size, "grad_weight")
