@@ -386,8 +386,9 @@ int linf_dropout_next(long long* state, long long* used, void* stream);
  *   h = (x - mean) / sqrt(var + eps),   u = gamma[c] h + beta[c],   y = dropout(activation(u))
  * gamma, beta: [C] of param_type (fp32 or the type of x), each may be NULL (1 and 0).  rate > 0 drops elements of y under rng as
  * linf_dropout does, numbered as they lie in memory.  mean, rstd [N, G] (fp32) are kept for the backward pass, or both NULL.
- * fp32 inside whatever the type; one rounding at the end.  Values further than 1.8e19 from each other, whose squares
- * are beyond fp32, are treated as infinite ones: h is 0 or NaN in their group.  The workspace (16-byte aligned; NULL where it is 0 bytes) has
+ * fp32 inside whatever the type (64 bits where CTAs join their sums); one rounding at the end.  Values beyond 1e37 in size, or further than 1e15
+ * from each other, whose sums of squares may be beyond fp32, may be treated as infinite ones: h is 0 or NaN in their group.
+ * The workspace (16-byte aligned; NULL where it is 0 bytes) has
  * linf_group_norm_workspace_bytes(...) bytes.  N and L are 2^30 at most; N * L * C may exceed 2^31.
  */
 size_t linf_group_norm_workspace_bytes(int N, int C, int G, int L, int type, int backward);

@@ -88,7 +88,7 @@ dense_norm_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, 
             }
         }
         dense_load<T, V, K>(x + row + (size_t)p.subs * d.C, s.in && n + p.subs < s.n1, s.t, p.tpr, vecs, v);
-        const float mu = slot_sum(a, 0.f, p.tpr, part[0]).x * inv;
+        const float mu = slot_sum(a * inv, 0.f, p.tpr, part[0]).x;       // means of a thread's values: neither sum leaves fp32 first
         const Lanes<V> shift = filled<V>(-mu);
         float q = 0.f;
         a = 0.f;
@@ -102,8 +102,8 @@ dense_norm_kernel(const T* __restrict__ x, Param gamma, Param beta, NormDims d, 
                 for (int j = 0; j < V; ++j) { a += e[j]; q = fmaf(e[j], e[j], q); }
             }
         // the values about mu: what the rounding of mu left of their mean is taken off as well
-        const float2 m = slot_sum(a, q, p.tpr, part[1]);
-        const float rest = m.x * inv, r = 1.f / sqrtf(fmaxf(fmaf(m.y, inv, -rest * rest), 0.f) + (m.y != m.y ? m.y : (float)eps));
+        const float2 m = slot_sum(a * inv, q * inv, p.tpr, part[1]);
+        const float rest = m.x, r = 1.f / sqrtf(fmaxf(fmaf(-rest, rest, m.y), 0.f) + (m.y != m.y ? m.y : (float)eps));
         if (!in) continue;
         if (s.t == 0 && mean != nullptr) {
             mean[(size_t)n * d.G + s.g] = mu + rest;

@@ -177,3 +177,25 @@ def test_constant_gradients_of_boxes_over_long_columns(cuda, lib, case):
     z = sum(y.detach().double() for y in ys)                   # fp32, off by less than 12 E (1 + |z|) each
     size = sum((y.detach().double().abs() + 1).sum((0, 2)) for y in ys)
     assert_within(gw, c * z.sum((0, 2)), c * 16 * E * size, "grad_weight")
+
+
+@gpu
+@pytest.mark.parametrize("case", FAR + [(2, 8192, 1, 1), (1, 2048, 1, 4096)], ids=lambda c: "N{}_C{}_G{}_L{}".format(*c))
+def test_values_as_far_apart_as_the_header_allows(cuda, lib, case):
+    """Values 10^15 from each other (their squares by the thousand are far beyond what one square would say), and equal ones of 10^37.
+
+    As for far values: 16 E (1 + |h|); the gradient is 1 / deviation times terms of order 1 that are off by 16 E each, and by 36 E in their means."""
+    N, C, groups, n = case
+    x = stored(N, C, n, torch.float32, sum(case), spread=1.0, level=0.0).clamp_(-4, 4).mul_(1.2e14)
+    x = (x if n > 1 else x.reshape(N, C)).requires_grad_()
+    h, mean, r = parts(x.reshape(N, C, n), groups)
+    y = L.group_norm(x, groups, eps=EPS)
+    assert_within(y.reshape(h.shape), h, 16 * E * (1 + h.abs()), "values")
+    g = torch.randn(y.shape, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    gx, = torch.autograd.grad(y, x, g)
+    g = g.double().reshape(h.shape)
+    both = lambda t: t.mean((2, 3), keepdim=True)  # noqa: E731
+    want = r * (g - both(g) - h * both(g * h))
+    most = r * (16 * E * (g.abs() + (1 + h.abs()) * both((1 + h.abs()) * g.abs())) + 36 * E * (both(g.abs()) + h.abs() * both((g * h).abs())))
+    assert_within(gx.reshape(h.shape), want, most, "grad_x")
+    assert not L.group_norm(torch.full_like(x, 1e37), groups).any()
