@@ -742,13 +742,13 @@ int forward_as(const T* x, const NormGiven& given, const NormDims& d, const Norm
                float* rstd, void* ws, cudaStream_t st) {
     if (p.kept) {
         const KeptSpace sp = kept_space(p, sizeof(T), 1, sizeof(Part), SAME, sizeof(Stat), false);
-        return launch_kept(norm_kept_kernel<T, V, SAME>, p, sp.bytes, st, x, given.gamma, given.beta, d, p, sp, eps, act, drop, y, mean, rstd);
+        return launch_kept<norm_kept_kernel<T, V, SAME>>(p, sp.bytes, st, x, given.gamma, given.beta, d, p, sp, eps, act, drop, y, mean, rstd);
     }
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     double2* part = static_cast<double2*>(ws);
     const size_t ring = norm_ring_bytes<T, V, 1, kRing>();
     const size_t one = ring + sizeof(Part) * p.rt * p.tx * (SAME ? 1 : V), two = ring + sizeof(Stat) * p.groups;
-    if (!allow_shared(norm_sums_kernel<T, V, SAME>, one) || !allow_shared(norm_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
+    if (!allow_shared<norm_sums_kernel<T, V, SAME>>(one) || !allow_shared<norm_apply_kernel<T, V>>(two)) return LINF_ERR_LAUNCH;
     norm_sums_kernel<T, V, SAME><<<grid, kNormThreads, one, st>>>(x, d, p, part);
     if (launch_status()) return LINF_ERR_LAUNCH;
     return launch_behind(norm_apply_kernel<T, V>, grid, kNormThreads, two, st, x, given.gamma, given.beta, part, d, p, eps, act, drop, y, mean, rstd);
@@ -768,14 +768,14 @@ int backward(const T* dy, const T* x, const NormGiven& given, int ptype, const f
     float2* by_channel = reinterpret_cast<float2*>(static_cast<char*>(ws) + parts_bytes(d, p));
     if (p.kept) {
         const KeptSpace sp = kept_space(p, sizeof(T), 2, sizeof(float2), false, sizeof(float2), drop.on && sizeof(T) == 2);
-        const int rc = launch_kept(norm_back_kept_kernel<T, V>, p, sp.bytes, st, dy, x, given.gamma, given.beta, mean, rstd, d, p, sp, act, drop,
+        const int rc = launch_kept<norm_back_kept_kernel<T, V>>(p, sp.bytes, st, dy, x, given.gamma, given.beta, mean, rstd, d, p, sp, act, drop,
                                    dx, by_channel);
         if (rc) return rc;
     } else {
         const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
         const size_t ring = norm_ring_bytes<T, V, 2, kBackRing>();
         const size_t one = ring + sizeof(double2) * p.rt * p.tx * V, two = ring + sizeof(float2) * p.groups;
-        if (!allow_shared(norm_back_sums_kernel<T, V>, one) || !allow_shared(norm_back_apply_kernel<T, V>, two)) return LINF_ERR_LAUNCH;
+        if (!allow_shared<norm_back_sums_kernel<T, V>>(one) || !allow_shared<norm_back_apply_kernel<T, V>>(two)) return LINF_ERR_LAUNCH;
         norm_back_sums_kernel<T, V><<<grid, kNormThreads, one, st>>>(dy, x, given.gamma, given.beta, mean, rstd, d, p, act, drop, by_channel, by_group);
         if (launch_status()) return LINF_ERR_LAUNCH;
         if (dx != nullptr) {

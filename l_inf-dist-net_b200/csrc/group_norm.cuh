@@ -384,9 +384,23 @@ struct NormStream {
     }
 };
 
-template <typename F>
-bool allow_shared(F kernel, size_t bytes) {
-    return bytes <= 48 * 1024 || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) == cudaSuccess;
+// Lets a kernel have more than 48 KB of dynamic shared memory, once for each device and to the device's limit: the limit is the kernel's on that
+// device, not the call's, and one that followed each call's size would fall under that of another host thread's launch.
+template <auto kernel>
+bool allow_shared(size_t bytes) {
+    static std::atomic<bool> known[kMaxDevices];
+    if (bytes <= 48 * 1024) return true;
+    int dev = -1, most = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess) {
+        if (dev < kMaxDevices && known[dev].load(std::memory_order_relaxed)) return true;
+        if (cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev) == cudaSuccess &&
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) == cudaSuccess) {
+            if (dev < kMaxDevices) known[dev].store(true, std::memory_order_relaxed);
+            return true;
+        }
+    }
+    cudaGetLastError();
+    return false;
 }
 
 // ---- launches that begin before the kernel in front has ended ---------------------------------------------------------
@@ -416,9 +430,9 @@ int launch_behind(void (*kernel)(A...), dim3 grid, int threads, size_t shared, c
 }
 
 // A kept call.
-template <typename... A, typename... B>
-int launch_kept(void (*kernel)(A...), const NormPlan& p, size_t shared, cudaStream_t st, B... args) {
-    if (!allow_shared(kernel, shared)) return LINF_ERR_LAUNCH;
+template <auto kernel, typename... B>
+int launch_kept(const NormPlan& p, size_t shared, cudaStream_t st, B... args) {
+    if (!allow_shared<kernel>(shared)) return LINF_ERR_LAUNCH;
     kernel<<<(unsigned)(p.chunks * p.blocks), p.threads, shared, st>>>(args...);
     return launch_status();
 }

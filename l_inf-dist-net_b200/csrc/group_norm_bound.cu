@@ -607,12 +607,12 @@ template <int V, bool SAME>
 int forward_as(const float* lower, const float* upper, const NormGiven& given, const NormDims& d, const NormPlan& p, double eps, int act, float* out_l,
                float* out_u, Sum4* sums, void* ws, cudaStream_t st) {
     if (p.kept)
-        return launch_kept(bound_kept_kernel<V, SAME>, p, bound_space<V>(p, 2).bytes, st, lower, upper, given.gamma, given.beta, d, p, eps, act, out_l,
+        return launch_kept<bound_kept_kernel<V, SAME>>(p, bound_space<V>(p, 2).bytes, st, lower, upper, given.gamma, given.beta, d, p, eps, act, out_l,
                            out_u, sums);
     const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
     Sum4* part = static_cast<Sum4*>(ws);
     const size_t ring = norm_ring_bytes<float, V, 2, kBoundRing>(), one = ring + bound_space<V>(p, 0).box, two = ring + sizeof(Ends32) * p.groups;
-    if (!allow_shared(bound_sums_kernel<V, SAME>, one) || !allow_shared(bound_apply_kernel<V>, two)) return LINF_ERR_LAUNCH;
+    if (!allow_shared<bound_sums_kernel<V, SAME>>(one) || !allow_shared<bound_apply_kernel<V>>(two)) return LINF_ERR_LAUNCH;
     bound_sums_kernel<V, SAME><<<grid, kNormThreads, one, st>>>(lower, upper, d, p, part);
     if (launch_status()) return LINF_ERR_LAUNCH;
     return launch_behind(bound_apply_kernel<V>, grid, kNormThreads, two, st, lower, upper, given.gamma, given.beta, part, d, p, eps, act, out_l, out_u,
@@ -632,13 +632,13 @@ int backward(const In4& in4, const NormGiven& given, const Sum4* sums, const Nor
     Sum4* by_group = static_cast<Sum4*>(ws);
     float2* by_channel = reinterpret_cast<float2*>(static_cast<char*>(ws) + parts_bytes(d, p));
     if (p.kept) {
-        const int rc = launch_kept(bound_back_kept_kernel<V>, p, bound_space<V>(p, 4).bytes, st, in4, given.gamma, given.beta, sums, d, p, eps,
+        const int rc = launch_kept<bound_back_kept_kernel<V>>(p, bound_space<V>(p, 4).bytes, st, in4, given.gamma, given.beta, sums, d, p, eps,
                                    act, d_l, d_u, by_channel);
         if (rc) return rc;
     } else {
         const dim3 grid((unsigned)(p.blocks * d.N), p.splits);
         const size_t shared = bound_space<V>(p, 0).bytes;
-        if (!allow_shared(bound_back_sums_kernel<V>, shared) || !allow_shared(bound_back_apply_kernel<V>, shared)) return LINF_ERR_LAUNCH;
+        if (!allow_shared<bound_back_sums_kernel<V>>(shared) || !allow_shared<bound_back_apply_kernel<V>>(shared)) return LINF_ERR_LAUNCH;
         bound_back_sums_kernel<V><<<grid, kNormThreads, shared, st>>>(in4, given.gamma, given.beta, sums, d, p, eps, act, by_channel, by_group);
         if (launch_status()) return LINF_ERR_LAUNCH;
         if (d_l != nullptr) {

@@ -1,0 +1,38 @@
+"""Group norm and dropout called in ways of their own: from several threads at once, traced, under transforms and checkpoints, by replicas."""
+import threading
+
+import pytest
+import torch
+
+import linfdist_b200 as L
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+def test_two_threads_with_two_sizes(cuda, lib):
+    """The same kernel with 51 and 64 KB of shared memory for each CTA from two threads at once: no call sees the other's limit.  The library's
+    own entry point, call after call, so that the threads are inside it at the same time."""
+    wrong = []
+    begin = threading.Barrier(2)
+    data = [torch.randn(8, n, 16, device="cuda") for n in (1000, 800)]
+    want = [L.group_norm(x.movedim(-1, 1), 1).movedim(1, -1) for x in data]
+    assert all(lib.linf_group_norm_workspace_bytes(8, 16, 1, x.size(1), 0, 0) == 0 for x in data)        # kept: one launch
+    torch.cuda.synchronize()
+
+    def work(k):
+        x, y, n = data[k], torch.empty_like(data[k]), data[k].size(1)
+        stream = torch.cuda.Stream()
+        args = (x.data_ptr(), None, None, 8, 16, 1, n, 0, 0, 1e-5, 0, 0.0, None, y.data_ptr(), None, None, None, 0, stream.cuda_stream)
+        begin.wait()
+        codes = [lib.linf_group_norm_forward(*args) for _ in range(6000)]
+        stream.synchronize()
+        if any(codes) or not torch.equal(y, want[k]):
+            wrong.append(f"thread {k}: {sum(c != 0 for c in codes)} calls refused")
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
