@@ -811,7 +811,7 @@ bool norm_given(const void* gamma, const void* beta, int ptype, NormGiven* g) {
 }
 
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st) {
-    return launch_behind(norm_params_kernel, dim3((C + 7) / 8), kParamThreads, 0, st, by_channel, count, C, dgamma, dbeta, ptype);
+    return launch_behind(norm_params_kernel, dim3(norm_param_ctas(C)), kParamThreads, 0, st, by_channel, count, C, dgamma, dbeta, ptype);
 }
 
 size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back) {

@@ -224,7 +224,8 @@ int dense_norm_forward(const void* x, const NormGiven& given, const NormDims& d,
 int dense_norm_backward(const void* dy, const void* x, const NormGiven& given, const float* mean, const float* rstd, const NormDims& d, const DensePlan& p,
                         int type, int act, const Drop& drop, void* dx, float2* by_channel, cudaStream_t st);
 
-// dgamma and dbeta from `count` rows of per-channel sums (du, du h); either may be null (group_norm.cu)
+// dgamma and dbeta from `count` rows of per-channel sums (du, du h); either may be null (group_norm.cu).  A CTA has 8 channels.
+inline unsigned norm_param_ctas(int C) { return (unsigned)norm_ceil(C, 8); }
 int norm_params(const float2* by_channel, long long count, int C, void* dgamma, void* dbeta, int ptype, cudaStream_t st);
 
 // gamma and beta, or what stands for them where they are null, and a generator state that stands for one that is not needed, on the

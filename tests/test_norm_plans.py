@@ -20,6 +20,7 @@ int main(int argc, char** argv) {
         if (!make_drop(atof(argv[2]), atoi(argv[3]) ? rng : nullptr, idle, &d)) return printf("refused"), 0;
         printf("%d %s", d.on, d.rng == rng ? "rng" : d.rng == idle ? "idle" : "null");
     }
+    if (!strcmp(argv[1], "params")) printf("%u", norm_param_ctas(atoi(argv[2])));
     return 0;
 }
 """
@@ -43,3 +44,9 @@ def ask(tmp_path_factory):
 def test_no_kernel_holds_a_null_generator_state(ask, rate, given, want):
     """Where nothing is dropped a valid address stands for the state, so that a load moved in front of its condition reads nothing it must not."""
     assert ask("drop", rate, given) == want
+
+
+@pytest.mark.parametrize("channels", [1, 8, 9, 2 ** 31 - 8, 2 ** 31 - 7, 2 ** 31 - 1])
+def test_ctas_of_the_parameters_gradients(ask, channels):
+    """All channel counts that a call may have, the last seven below 2^31 among them."""
+    assert ask("params", channels) == [str(-(-channels // 8))]
