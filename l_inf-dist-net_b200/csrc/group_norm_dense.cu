@@ -210,7 +210,7 @@ bool dense_plan(const NormDims& d, int elem_bytes, bool aligned, int ctas, Dense
     }
     const int vecs = d.Cg / p->V, keep = p->V == 8 ? 2 : 4;
     p->tpr = 1;
-    while (p->tpr * keep < vecs) p->tpr *= 2;
+    while (p->tpr <= kDenseMost && p->tpr * keep < vecs) p->tpr *= 2;
     if (p->tpr > kDenseMost) return false;
     p->threads = p->tpr > kNormThreads ? p->tpr : kNormThreads;
     const int slots = p->threads / p->tpr;

@@ -50,3 +50,11 @@ def test_no_kernel_holds_a_null_generator_state(ask, rate, given, want):
 def test_ctas_of_the_parameters_gradients(ask, channels):
     """All channel counts that a call may have, the last seven below 2^31 among them."""
     assert ask("params", channels) == [str(-(-channels // 8))]
+
+
+@pytest.mark.parametrize("call", ["group_norm_workspace_bytes(1, 2**30 + 1, 1, 1, 0, 0)", "group_norm_workspace_bytes(1, 2**31 - 1, 1, 1, 1, 1)",
+                                  "group_norm_workspace_bytes(1, 2**31 - 2, 1, 1, 2, 1)", "group_norm_bound_workspace_bytes(1, 2**31 - 1, 1, 1, 1)"])
+def test_rows_of_a_thousand_million_channels_are_planned(lib, call):
+    """In a process of its own, which ends in time."""
+    code = f"import linfdist_b200 as L; assert L._lib.load().linf_{call} >= 0"
+    subprocess.run(["python", "-c", code], cwd=os.path.dirname(os.path.dirname(CSRC)), timeout=60, check=True)
