@@ -10,6 +10,7 @@ import operator
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dropout import DropoutTripleF, _Masks, _TYPES, _floating, _generator_state, _once, _rate, dropout_next
@@ -192,6 +193,10 @@ def _make_call(x, name, groups, weight, bias, eps, activation):
 
 
 def _wants_grad(*tensors):
+    """Whether the call has to go through its autograd function: for a backward pass, or because a tensor carries a forward-mode
+    tangent (which the function refuses; the launch alone would lose it)."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        return True
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 

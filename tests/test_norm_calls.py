@@ -36,3 +36,36 @@ def test_two_threads_with_two_sizes(cuda, lib):
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_a_forward_mode_tangent_counts_as_a_gradient():
+    """What a call without gradients would lose."""
+    import torch.autograd.forward_ad as fw
+    wants = L.group_norm.__globals__["_wants_grad"]
+    x, w = torch.randn(2, 8), torch.ones(8)
+    assert not wants(x, w, None) and wants(x, w.clone().requires_grad_())
+    with fw.dual_level():
+        assert not wants(x, w) and wants(fw.make_dual(x, x), w) and wants(x, None, fw.make_dual(w, w))
+        with torch.no_grad():
+            assert wants(fw.make_dual(x, x), w)
+    seen = []
+    torch.func.jvp(lambda t: (seen.append(wants(t)), t)[1], (x,), (x,))
+    assert seen == [True]
+
+
+@gpu
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(cuda, lib, which):
+    """A tangent of the input, the weight or the bias: an error and not a result without one."""
+    import torch.autograd.forward_ad as fw
+    with fw.dual_level():
+        a = [torch.randn(2, 8, device="cuda"), torch.ones(8, device="cuda"), torch.zeros(8, device="cuda")]
+        a[which] = fw.make_dual(a[which], torch.ones_like(a[which]))
+        for call in (lambda: L.group_norm(a[0], 2, a[1], a[2]), lambda: L.group_norm_bound(a[0], a[0], 2, a[1], a[2])):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+    x = torch.randn(2, 8, device="cuda")
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: L.group_norm(t, 2), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: L.group_norm(t, 2))(x.view(2, 1, 8))
