@@ -23,6 +23,12 @@ def _once(backward):
     return run
 
 
+def _not_traced(name):
+    """torch.jit.trace sees the allocation of a result and not the launch that fills it."""
+    if torch.jit.is_tracing():
+        raise RuntimeError(f"{name} cannot be traced by torch.jit")
+
+
 def _floating(t, name):
     if t.dtype not in _TYPES:
         raise RuntimeError(f"{name} must have dtype torch.float32, torch.float16 or torch.bfloat16")
@@ -108,6 +114,7 @@ class DropoutTripleF(torch.autograd.Function):
 def dropout_next(state):
     """{seed, offset} to draw one mask with, as a tensor of its own; the offset of `state` rises by 1.  Runs on the device, so a
     captured graph draws another mask each time it is replayed, and calls on several streams never get the same offset."""
+    _not_traced("dropout_next")
     _generator_state(state, state.device)
     if not state.is_cuda:
         raise RuntimeError("rng must be a CUDA tensor")

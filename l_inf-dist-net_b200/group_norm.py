@@ -13,7 +13,7 @@ import torch.nn as nn
 from torch.autograd import forward_ad
 
 from . import _lib
-from .dropout import DropoutTripleF, _Masks, _TYPES, _floating, _generator_state, _once, _rate, dropout_next
+from .dropout import DropoutTripleF, _Masks, _TYPES, _floating, _generator_state, _not_traced, _once, _rate, dropout_next
 from .norm_dist import _on, _scratch, _stream, skips_values
 
 ACTIVATIONS = {"identity": 0, "relu": 1, "tanh": 2, "silu": 3}        # LINF_ACT_*
@@ -207,6 +207,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation="identity
     activation: "identity", "relu", "tanh" or "silu".  rate > 0 drops elements of the result under rng {seed, offset} in the same pass:
     what `dropout(y, rate, rng)` gives.  Computed in fp32 and rounded once.  Channels-last memory is taken as it is, any
     other layout is copied to it; the result has its channels last in memory."""
+    _not_traced("group_norm")
     rate = _rate(rate)
     if rate > 0:
         if rng is None:
@@ -226,6 +227,7 @@ def group_norm_bound(lower, upper, groups, weight=None, bias=None, eps=1e-5, act
     The exact range of x_i - mean(x) over the box is divided by a range of the deviation that the triangle inequality gives, so the
     bounds hold for the box as a whole and collapse to the value where lower = upper; nothing normalised exceeds sqrt(M - 1) in a
     group of M.  The sums are 64-bit, the bounds fp32, rounded to nearest (as the bounds of the other layers are)."""
+    _not_traced("group_norm_bound")
     if upper.shape != lower.shape or upper.dtype != lower.dtype or upper.device != lower.device:
         raise RuntimeError("upper must have the shape, dtype and device of lower")
     if lower.dtype != torch.float32:

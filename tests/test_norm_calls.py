@@ -69,3 +69,12 @@ def test_forward_mode_derivatives_are_refused(cuda, lib, which):
         torch.func.jvp(lambda t: L.group_norm(t, 2), (x,), (x,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda t: L.group_norm(t, 2))(x.view(2, 1, 8))
+
+
+def test_tracing_is_refused():
+    """A traced call would give the memory of its result and nothing in it."""
+    x, rng = torch.randn(2, 8), torch.zeros(2, dtype=torch.int64)
+    for call in (lambda t: L.group_norm(t, 2), lambda t: L.group_norm_bound(t, t, 2)[0], lambda t: L.BoundGroupNorm(2, 8)(t)[0],
+                 lambda t: t * L.dropout_next(rng)[0]):
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(call, x)
