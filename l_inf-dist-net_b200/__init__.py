@@ -12,7 +12,7 @@ from .norm_dist import (DistF, MeanNorm, NormDist, NormDistConv, get_p_norm, inf
                         inf_dist_post, set_fused_epilogue, get_fused_epilogue)
 from .bound_module import (BoundFinalIdentity, BoundFinalLinear, BoundLinear, BoundMeanNorm,
                            BoundReLU, BoundTanh, Predictor)
-from .dropout import BoundDropout, dropout, dropout_next
+from .dropout import BoundDropout, checkpoint_masks, dropout, dropout_next
 from .group_norm import BoundGroupNorm, group_norm, group_norm_bound
 from .nets import MLP, MLPFeature, Model, get_eps, set_eps
 from .adamw import AdamW
@@ -24,6 +24,6 @@ __all__ = [
     "inf_dist_post", "set_fused_epilogue", "get_fused_epilogue",
     "BoundReLU", "BoundTanh", "BoundLinear", "BoundFinalLinear", "BoundMeanNorm",
     "BoundFinalIdentity", "Predictor", "MLP", "MLPFeature", "Model", "set_eps", "get_eps",
-    "group_norm", "group_norm_bound", "BoundGroupNorm", "dropout", "dropout_next", "BoundDropout",
+    "group_norm", "group_norm_bound", "BoundGroupNorm", "dropout", "dropout_next", "checkpoint_masks", "BoundDropout",
     "AdamW", "certify", "certified_accuracy", "AttackPGD",
 ]

@@ -4,6 +4,8 @@ again (csrc/dropout.cu; the generator is Philox4x32 with 7 rounds, 16 bits for e
 Beside the elementwise maps of the heads (BoundReLU, BoundTanh): `BoundDropout` maps a triple (value, lower, upper) under ONE
 mask, so that lower <= value <= upper still holds behind it.  zbh2047/L_inf-dist-net has no counterpart.
 """
+import threading
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
@@ -111,11 +113,40 @@ class DropoutTripleF(torch.autograd.Function):
         return (None, None, *_launch(ctx.rate, rng, *given))
 
 
-def dropout_next(state):
-    """{seed, offset} to draw one mask with, as a tensor of its own; the offset of `state` rises by 1.  Runs on the device, so a
-    captured graph draws another mask each time it is replayed, and calls on several streams never get the same offset."""
-    _not_traced("dropout_next")
-    _generator_state(state, state.device)
+_masks_of = threading.local()          # .stack: the blocks of `checkpoint_masks` that this thread is in, the innermost last
+
+
+class _Drawn:
+    """A block of `checkpoint_masks`: where the pairs that are drawn in it are kept, or, `again`, from where they come once more."""
+
+    def __init__(self, pairs, again):
+        self.pairs, self.again, self.at = pairs, again, 0
+
+    def __enter__(self):
+        self.at = 0
+        if not hasattr(_masks_of, "stack"):
+            _masks_of.stack = []
+        _masks_of.stack.append(self)
+        return self
+
+    def __exit__(self, *exc):
+        _masks_of.stack.pop()
+
+    def take(self, state):
+        if self.at == len(self.pairs) or self.pairs[self.at][0] is not state:
+            raise RuntimeError("the checkpointed function draws other masks when it is run again than it did at first")
+        self.at += 1
+        return self.pairs[self.at - 1][1]
+
+
+def checkpoint_masks():
+    """The `context_fn` with which `torch.utils.checkpoint.checkpoint(..., use_reentrant=False)` runs a function that drops elements: the second run
+    gets the pairs of the first, and with them its masks.  Without it a pass that is run again is refused, for it would draw others."""
+    pairs = []
+    return _Drawn(pairs, False), _Drawn(pairs, True)
+
+
+def _draw(state):
     if not state.is_cuda:
         raise RuntimeError("rng must be a CUDA tensor")
     used = torch.empty_like(state)
@@ -123,6 +154,29 @@ def dropout_next(state):
         rc = _lib.load().linf_dropout_next(state.data_ptr(), used.data_ptr(), _stream())
     _lib.check(rc, "dropout_next")
     torch.autograd.graph.increment_version(state)       # a backward pass that was to read `state` itself is refused by autograd
+    return used
+
+
+def dropout_next(state):
+    """{seed, offset} to draw one mask with, as a tensor of its own; the offset of `state` rises by 1.  Runs on the device, so a
+    captured graph draws another mask each time it is replayed, and calls on several streams never get the same offset.
+
+    Within a backward pass (a checkpointed function that is run again) it is refused, or gives what it gave at first: `checkpoint_masks`."""
+    _not_traced("dropout_next")
+    _generator_state(state, state.device)
+    used, keep = None, []
+    for block in reversed(getattr(_masks_of, "stack", ())):
+        if block.again:
+            used = block.take(state)
+            break
+        keep.append(block)
+    if used is None:
+        if torch._C._current_graph_task_id() != -1:
+            raise RuntimeError("a mask is drawn within a backward pass: a checkpointed function that drops elements needs use_reentrant=False and "
+                               "context_fn=checkpoint_masks")
+        used = _draw(state)
+    for block in keep:
+        block.pairs.append((state, used))
     return used
 
 

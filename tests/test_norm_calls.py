@@ -1,8 +1,10 @@
 """Group norm and dropout called in ways of their own: from several threads at once, traced, under transforms and checkpoints, by replicas."""
+import sys
 import threading
 
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import linfdist_b200 as L
 
@@ -78,3 +80,90 @@ def test_tracing_is_refused():
                  lambda t: t * L.dropout_next(rng)[0]):
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(call, x)
+
+
+class _ByHand(torch.autograd.Function):
+    """Dropout on the CPU: elements whose number has the parity of the offset are kept."""
+
+    @staticmethod
+    def forward(ctx, x, rate, used):
+        ctx.keep = (torch.arange(x.numel()).view(x.shape) + int(used[1])) % 2 == 0
+        return x * ctx.keep
+
+    @staticmethod
+    def backward(ctx, g):
+        return g * ctx.keep, None, None
+
+
+@pytest.fixture
+def by_hand(monkeypatch):
+    """The modules of this package with the library's two calls done on the CPU."""
+    module = sys.modules[L.BoundDropout.__module__]
+
+    def draw(state):
+        used = state.clone()
+        state[1] += 1
+        return used
+    monkeypatch.setattr(module, "_draw", draw)
+    monkeypatch.setattr(module, "dropout", _ByHand.apply)
+
+
+@pytest.mark.parametrize("nested", [False, True])
+def test_checkpoints_get_the_masks_of_the_first_run(by_hand, nested):
+    """Value and gradient have the same mask, twice in a row and with checkpoints of several calls; the offset counts the first runs alone."""
+    drop, other = L.BoundDropout(0.5, seed=1).train(), L.BoundDropout(0.5, seed=2).train()
+    keep = dict(use_reentrant=False, context_fn=L.checkpoint_masks)
+
+    def block(t):
+        t = checkpoint(lambda s: drop(s * 2)[0], t, **keep) if nested else drop(t * 2)[0]
+        return other(drop(torch.cat([t, t]).exp())[0])[0]
+
+    x = torch.rand(12, requires_grad=True)
+    ys = [checkpoint(block, x, **keep) for _ in range(3)]                     # all before the first backward pass
+    assert drop.rng[1] == 6 and other.rng[1] == 3
+    got = [torch.autograd.grad(y.sum(), x, retain_graph=True)[0] for y in ys]
+    again = [torch.autograd.grad(y.sum(), x)[0] for y in reversed(ys)]
+    assert drop.rng[1] == 6 and other.rng[1] == 3
+    drop.rng[1], other.rng[1] = 0, 0
+    for y, g, h in zip(ys, got, reversed(again)):
+        want = block(x) if not nested else None
+        if want is not None:
+            assert torch.equal(y, want) and torch.equal(g, torch.autograd.grad(want.sum(), x)[0])
+        assert torch.equal(g, h) and ((g != 0) <= (y.view(2, 12) != 0).any(0)).all()
+
+
+def test_checkpoints_without_the_masks_are_refused(by_hand):
+    drop = L.BoundDropout(0.5, seed=1).train()
+    x = torch.rand(12, requires_grad=True)
+    for kw in (dict(use_reentrant=False), dict(use_reentrant=True)):
+        y = checkpoint(lambda t: drop(t * 2)[0].exp(), x, **kw)
+        with pytest.raises(RuntimeError, match="checkpoint_masks"):
+            y.sum().backward()
+    count = [0]
+
+    def changes(t):
+        count[0] += 1
+        return drop(drop(t)[0] if count[0] > 1 else t)[0].exp()
+    y = checkpoint(changes, x, use_reentrant=False, context_fn=L.checkpoint_masks)
+    with pytest.raises(RuntimeError, match="other masks|different number"):
+        y.sum().backward()
+    assert not sys.modules[L.BoundDropout.__module__]._masks_of.stack
+
+
+@gpu
+def test_checkpoint_of_norm_and_dropout(cuda, lib):
+    """The modules themselves: values and gradients of a checkpointed block are those of the block."""
+    norm = L.BoundGroupNorm(4, 32, activation="tanh", dropout=0.25, seed=5).cuda().train()
+    drop = L.BoundDropout(0.5, seed=6).cuda().train()
+    x = torch.randn(20, 32, device="cuda", requires_grad=True)
+
+    def block(t):
+        return [s.sin() for s in drop(*norm(t, t - 0.1, t + 0.1))]
+
+    results = []
+    for run in (block, lambda t: checkpoint(block, t, use_reentrant=False, context_fn=L.checkpoint_masks)):
+        norm.rng[1] = drop.rng[1] = 0
+        ys = run(x)
+        results.append([*ys, *torch.autograd.grad(sum(k * y.sum() for k, y in enumerate(ys, 1)), [x, norm.weight, norm.bias])])
+        assert norm.rng[1] == 1 and drop.rng[1] == 1
+    assert all(torch.equal(a, e) for a, e in zip(*results))
