@@ -380,6 +380,8 @@ int linf_dropout(const void* x, const void* lower, const void* upper, long long 
 
 /* used = {seed, offset} of `state`, whose offset then rises by 1 (atomically): the pair to draw one mask with. */
 int linf_dropout_next(long long* state, long long* used, void* stream);
+/* The same for one of several replicas that hold equal states: used = {seed + replica * 0x9E3779B97F4A7C15 (modulo 2^64), offset}. */
+int linf_dropout_next_replica(long long* state, long long replica, long long* used, void* stream);
 
 /*
  * Group norm of x [N, L, C], channels last: C/G neighbouring channels over all L positions of a sample form a group,

@@ -52,6 +52,7 @@ _PROTOS = {
     "linf_norm_dist_backward": [_F, _F, _F, _F, _INT, _INT, _INT, _INT, _INT, _F, _F, ctypes.c_float, _F, ctypes.c_size_t, _F],
     "linf_dropout": [_F, _F, _F, ctypes.c_longlong, _INT, ctypes.c_double, _F, _F, _F, _F, _F],
     "linf_dropout_next": [_F, _F, _F],
+    "linf_dropout_next_replica": [_F, ctypes.c_longlong, _F, _F],
     "linf_group_norm_workspace_bytes": [_INT, _INT, _INT, _INT, _INT, _INT],
     "linf_group_norm_forward": [_F, _F, _F, _INT, _INT, _INT, _INT, _INT, _INT, ctypes.c_double, _INT, ctypes.c_double, _F, _F, _F, _F, _F,
                                 ctypes.c_size_t, _F],

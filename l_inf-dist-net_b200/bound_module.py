@@ -119,16 +119,17 @@ class BoundFinalIdentity(nn.Module):
 
 class Predictor(nn.Module):
     """BoundLinear -> tanh -> BoundFinalLinear head used by the '++' nets.  groups: the hidden units go through a group norm of
-    that many groups before the tanh (one kernel for both); dropout: rate at which hidden units are dropped while training."""
+    that many groups before the tanh (one kernel for both); dropout: rate at which hidden units are dropped while training, under
+    masks from `seed` (BoundDropout)."""
 
-    def __init__(self, in_features, hidden, out_dim, groups=None, dropout=0.0):
+    def __init__(self, in_features, hidden, out_dim, groups=None, dropout=0.0, seed=None):
         super().__init__()
         self.fc1 = BoundLinear(in_features, hidden, bias=True)
         if groups is None:
             self.tanh = BoundTanh()
-            self.drop = BoundDropout(dropout) if dropout != 0 else None
+            self.drop = BoundDropout(dropout, seed) if dropout != 0 else None
         else:
-            self.norm = BoundGroupNorm(groups, hidden, activation="tanh", dropout=dropout)
+            self.norm = BoundGroupNorm(groups, hidden, activation="tanh", dropout=dropout, seed=seed)
         self.groups = groups
         self.fc2 = BoundFinalLinear(hidden, out_dim)
 

@@ -386,7 +386,12 @@ int linf_fold_rows(const float* rows, int B, int C, int H, int W, int kernel_siz
 
 int linf_dropout_next(long long* state, long long* used, void* stream) {
     if (!state || !used) return LINF_ERR_NULL;
-    return dropout_next(state, used, as_stream(stream));
+    return dropout_next(state, 0, used, as_stream(stream));
+}
+
+int linf_dropout_next_replica(long long* state, long long replica, long long* used, void* stream) {
+    if (!state || !used) return LINF_ERR_NULL;
+    return dropout_next(state, replica, used, as_stream(stream));
 }
 
 int linf_dropout(const void* x, const void* lower, const void* upper, long long n, int type, double rate, const long long* rng,

@@ -195,7 +195,7 @@ int unfold_rows(const float* x, int B, int C, int H, int W, int k, int dil, int 
 int fold_rows(const float* rows, int B, int C, int H, int W, int k, int dil, int pad, int stride, float* gx, cudaStream_t st);
 // dropout with a mask computed from (seed, offset, element number) (dropout.cu)
 int dropout(const void* const* in, void* const* out, int tensors, long long n, int type, double rate, const long long* rng, cudaStream_t st);
-int dropout_next(long long* state, long long* used, cudaStream_t st);
+int dropout_next(long long* state, long long replica, long long* used, cudaStream_t st);
 // group norm, channels last, with activation and dropout (group_norm.cu), and over a box (group_norm_bound.cu)
 size_t group_norm_workspace(int N, int C, int G, int L, int type, bool back);
 int group_norm_forward(const void* x, const void* gamma, const void* beta, int N, int C, int G, int L, int type, int ptype, double eps, int act,

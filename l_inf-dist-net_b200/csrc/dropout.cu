@@ -71,8 +71,9 @@ dropout_kernel(Tensors t, long long n, Drop d) {
     }
 }
 
-__global__ void dropout_next_kernel(long long* state, long long* used) {
-    used[0] = state[0];
+__global__ void dropout_next_kernel(long long* state, unsigned long long replica, long long* used) {
+    // an odd multiple of the replica's number: seeds of their own for 2^64 replicas, and that of the state for replica 0
+    used[0] = (long long)((unsigned long long)state[0] + replica * 0x9E3779B97F4A7C15ull);
     used[1] = (long long)atomicAdd(reinterpret_cast<unsigned long long*>(state + 1), 1ull);
 }
 
@@ -110,8 +111,8 @@ int dropout(const void* const* in, void* const* out, int tensors, long long n, i
     return launch<__nv_bfloat16>(t, tensors, n, d, st);
 }
 
-int dropout_next(long long* state, long long* used, cudaStream_t st) {
-    dropout_next_kernel<<<1, 1, 0, st>>>(state, used);
+int dropout_next(long long* state, long long replica, long long* used, cudaStream_t st) {
+    dropout_next_kernel<<<1, 1, 0, st>>>(state, (unsigned long long)replica, used);
     return launch_status();
 }
 

@@ -146,20 +146,21 @@ def checkpoint_masks():
     return _Drawn(pairs, False), _Drawn(pairs, True)
 
 
-def _draw(state):
+def _draw(state, replica):
     if not state.is_cuda:
         raise RuntimeError("rng must be a CUDA tensor")
     used = torch.empty_like(state)
     with _on(state.device):
-        rc = _lib.load().linf_dropout_next(state.data_ptr(), used.data_ptr(), _stream())
+        rc = _lib.load().linf_dropout_next_replica(state.data_ptr(), replica, used.data_ptr(), _stream())
     _lib.check(rc, "dropout_next")
     torch.autograd.graph.increment_version(state)       # a backward pass that was to read `state` itself is refused by autograd
     return used
 
 
-def dropout_next(state):
+def dropout_next(state, replica=0):
     """{seed, offset} to draw one mask with, as a tensor of its own; the offset of `state` rises by 1.  Runs on the device, so a
     captured graph draws another mask each time it is replayed, and calls on several streams never get the same offset.
+    replica: its number among those that hold equal states, each of which gets a seed of its own.
 
     Within a backward pass (a checkpointed function that is run again) it is refused, or gives what it gave at first: `checkpoint_masks`."""
     _not_traced("dropout_next")
@@ -174,7 +175,7 @@ def dropout_next(state):
         if torch._C._current_graph_task_id() != -1:
             raise RuntimeError("a mask is drawn within a backward pass: a checkpointed function that drops elements needs use_reentrant=False and "
                                "context_fn=checkpoint_masks")
-        used = _draw(state)
+        used = _draw(state, replica)
     for block in keep:
         block.pairs.append((state, used))
     return used
@@ -203,7 +204,11 @@ def dropout(x, rate, rng, lower=None, upper=None):
 
 
 class _Masks(nn.Module):
-    """Keeps the generator state of a module that drops elements: a buffer `rng` of {seed, offset}."""
+    """Keeps the generator state of a module that drops elements: a buffer `rng` of {seed, offset}.  `replica`: the module's number among
+    the replicas of a data-parallel job (the step classes of train_step.py set it; with another wrapper, the program does).  It is no part of the
+    state, which the ranks load, or broadcast to each other, as it is."""
+
+    replica = 0
 
     def _make_masks(self, rate, seed):
         self.rate = _rate(rate)
@@ -214,7 +219,7 @@ class _Masks(nn.Module):
 
 class BoundDropout(_Masks):
     """Dropout of a triple (value, lower, upper) while training; nothing in eval mode.  Every forward pass draws a mask of its own.
-    seed: by default a number from torch's CPU generator.  Replicas of a data-parallel job need seeds of their own."""
+    seed: by default a number from torch's CPU generator.  Replicas of a data-parallel job may have equal ones (`replica`)."""
 
     def __init__(self, rate, seed=None):
         super().__init__()
@@ -225,7 +230,7 @@ class BoundDropout(_Masks):
             lower = upper = None
         if not self.training or self.rate == 0:
             return x, lower, upper
-        used = dropout_next(self.rng)
+        used = dropout_next(self.rng, self.replica)
         if lower is None:
             return dropout(x, self.rate, used), None, None
         return dropout(x, self.rate, used, lower, upper)

@@ -259,7 +259,7 @@ class BoundGroupNorm(_Masks):
             raise RuntimeError(f"the input must have {self.channels} channels")
         args = (self.groups, self.weight, self.bias, self.eps, self.activation)
         rate = self.rate if self.training else 0.0
-        used = dropout_next(self.rng) if rate > 0 else None
+        used = dropout_next(self.rng, self.replica) if rate > 0 else None
         if lower is None or upper is None:
             return group_norm(x, *args, rate, used), None, None
         lo, up = group_norm_bound(lower, upper, *args)

@@ -11,6 +11,7 @@ import torch.nn as nn
 from . import _lib
 from .adamw import AdamW
 from .bound_module import BoundFinalIdentity, Predictor
+from .dropout import _Masks
 from .nets import MLP, MLPFeature, Model
 from .norm_dist import NormDistConv, get_p_norm, set_p_norm
 
@@ -89,6 +90,7 @@ class DataParallelStep:
       * parameters are broadcast from rank 0 once; the MeanNorm running means (views of one flat tensor)
         are broadcast from rank 0 right after the forward that updated them and waited for at the start of
         the next step: the same values at the start of every step as DDP's broadcast_buffers gives;
+      * modules that drop elements get the rank as their `replica`, so that every rank draws masks of its own;
       * when autograd has accumulated the gradient of a parameter, its all-reduce (average) is
         issued asynchronously and, on a side stream that waits for exactly that all-reduce, the
         optimiser updates that parameter; the next forward waits, layer by layer, only for the
@@ -129,6 +131,9 @@ class DataParallelStep:
         if self.world > 1:
             for p in net.parameters():
                 self.dist.broadcast(p.data, src=0)
+            for m in net.modules():
+                if isinstance(m, _Masks):
+                    m.replica = self.dist.get_rank()        # masks of its own, from states that the ranks have in common
         # the MeanNorm running means of all layers as views of ONE tensor: one broadcast per step
         self.buffers, self.flat_buffers, self.buffer_work = [], None, None
         if self.world > 1:

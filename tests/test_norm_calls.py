@@ -1,4 +1,5 @@
 """Group norm and dropout called in ways of their own: from several threads at once, traced, under transforms and checkpoints, by replicas."""
+import os
 import sys
 import threading
 
@@ -100,8 +101,9 @@ def by_hand(monkeypatch):
     """The modules of this package with the library's two calls done on the CPU."""
     module = sys.modules[L.BoundDropout.__module__]
 
-    def draw(state):
+    def draw(state, replica):
         used = state.clone()
+        used[0] += replica
         state[1] += 1
         return used
     monkeypatch.setattr(module, "_draw", draw)
@@ -167,3 +169,64 @@ def test_checkpoint_of_norm_and_dropout(cuda, lib):
         results.append([*ys, *torch.autograd.grad(sum(k * y.sum() for k, y in enumerate(ys, 1)), [x, norm.weight, norm.bias])])
         assert norm.rng[1] == 1 and drop.rng[1] == 1
     assert all(torch.equal(a, e) for a, e in zip(*results))
+
+
+def _replica(rank, world, port, out):
+    import torch.distributed as dist
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    from linfdist_b200.train_step import DataParallelStep
+    seen = []
+    for groups in (None, 4):
+        torch.manual_seed(7)                                  # the same net on every rank
+        net = torch.nn.Sequential(L.Predictor(8, 16, 3, groups=groups, dropout=0.25))
+        step = DataParallelStep(net, L.AdamW(net, lr=0.1))
+        module = net[0].drop if groups is None else net[0].norm
+        net.load_state_dict(net.state_dict())
+        seen.append((module.replica, module.rng.tolist()))
+        step.close()
+    all_seen = [None] * world
+    dist.all_gather_object(all_seen, seen)
+    if rank == 0:
+        out.put(all_seen)
+    dist.destroy_process_group()
+
+
+def test_replicas_are_numbered():
+    """Two CPU ranks with the same net: equal states, which may be loaded and broadcast, and a number of its own for each rank."""
+    import torch.multiprocessing as mp
+    ctx = mp.get_context("spawn")
+    out = ctx.Queue()
+    port = 29950 + os.getpid() % 400
+    ranks = [ctx.Process(target=_replica, args=(r, 2, port, out)) for r in range(2)]
+    for p in ranks:
+        p.start()
+    seen = out.get(timeout=240)
+    for p in ranks:
+        p.join(timeout=60)
+        assert p.exitcode == 0
+    for a, b in zip(*seen):
+        assert (a[0], b[0]) == (0, 1) and a[1] == b[1]
+
+
+def test_seeds_of_the_head():
+    for groups in (None, 4):
+        heads = [L.Predictor(8, 16, 3, groups=groups, dropout=0.25, seed=s) for s in (3, 4)]
+        assert [(h.norm if groups else h.drop).rng.tolist() for h in heads] == [[3, 0], [4, 0]]
+
+
+@gpu
+def test_masks_of_replicas(cuda, lib):
+    """Equal states, a seed of its own for each replica; that of replica 0 as it is; the modules' masks differ."""
+    rng = [torch.tensor([-5, 40], dtype=torch.int64, device="cuda") for _ in range(3)]
+    used = [L.dropout_next(s, replica=k).tolist() for k, s in enumerate(rng)]
+    want = [(-5 + k * 0x9E3779B97F4A7C15 + 2 ** 63) % 2 ** 64 - 2 ** 63 for k in range(3)]
+    assert used == [[w, 40] for w in want] and all(s.tolist() == [-5, 41] for s in rng)
+    x = torch.ones(4, 64, device="cuda")
+    for make in (lambda: L.BoundDropout(0.5, seed=1), lambda: L.BoundGroupNorm(4, 64, dropout=0.5, seed=1)):
+        masks = []
+        for k in (0, 1, 0):
+            m = make().cuda().train()
+            m.replica = k
+            masks.append(m(x + torch.arange(64, device="cuda"))[0] != 0)
+        assert torch.equal(masks[0], masks[2]) and not torch.equal(masks[0], masks[1])
