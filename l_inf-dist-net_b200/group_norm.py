@@ -39,6 +39,8 @@ def _work_space(query, device, *key):
     """Scratch of a call (from the current stream's pool), or None where it needs none; what a call needs is asked once."""
     need = _workspace_bytes.get((query, device.index, key))
     if need is None:
+        if len(_workspace_bytes) >= 4096:
+            _workspace_bytes.clear()
         need = _workspace_bytes[query, device.index, key] = getattr(_lib.load(), query)(*key)
     return _scratch(device, need) if need else None, need
 

@@ -230,3 +230,13 @@ def test_masks_of_replicas(cuda, lib):
             m.replica = k
             masks.append(m(x + torch.arange(64, device="cuda"))[0] != 0)
         assert torch.equal(masks[0], masks[2]) and not torch.equal(masks[0], masks[1])
+
+
+def test_what_is_kept_of_sizes_has_an_end(lib, monkeypatch):
+    """One entry for each size, up to some thousand."""
+    G = sys.modules[L.BoundGroupNorm.__module__]
+    monkeypatch.setattr(G, "_scratch", lambda device, need: need)
+    device = torch.device("cuda:0")
+    for n in range(1, 9001):
+        assert G._work_space("linf_group_norm_workspace_bytes", device, n, 8, 2, 1, 0, 1)[1] > 0
+    assert len(G._workspace_bytes) <= 4096
