@@ -133,6 +133,12 @@ class Predictor(nn.Module):
         self.groups = groups
         self.fc2 = BoundFinalLinear(hidden, out_dim)
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for name in ("groups", "drop"):                 # a net that was saved whole before there were norms and dropout
+            if not hasattr(self, name):
+                setattr(self, name, None)
+
     def forward(self, x, lower=None, upper=None, targets=None):
         triple = self.fc1(x, lower, upper)
         if self.groups is not None:

@@ -420,6 +420,7 @@ class NormDistConv(nn.Module):
     optional bias [CO], optional normalize.running_mean [CO]."""
 
     tag_counter = 0
+    channels_last = False                   # also of a layer that was saved whole before there was the choice
 
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1, group=1, p=0,
                  bias=True, mean_normalize=False, identity_init=True, channels_last=False):

@@ -1,5 +1,6 @@
 """Group norm and dropout called in ways of their own: from several threads at once, traced, under transforms and checkpoints, by replicas."""
 import os
+import pickle
 import sys
 import threading
 
@@ -240,3 +241,19 @@ def test_what_is_kept_of_sizes_has_an_end(lib, monkeypatch):
     for n in range(1, 9001):
         assert G._work_space("linf_group_norm_workspace_bytes", device, n, 8, 2, 1, 0, 1)[1] > 0
     assert len(G._workspace_bytes) <= 4096
+
+
+def test_nets_saved_whole_before_there_were_norms():
+    """A pickled head and a pickled convolution without the newer attributes are what they were."""
+    head, conv = L.Predictor(8, 16, 3), L.NormDistConv(4, 32, 3)
+    for m, names in ((head, ("groups", "drop")), (conv, ("channels_last",))):
+        for name in names:
+            del m.__dict__[name]
+    head, conv = pickle.loads(pickle.dumps(head)), pickle.loads(pickle.dumps(conv))
+    assert conv.channels_last is False
+    x, t = torch.randn(5, 8), torch.arange(5) % 3
+    y, worst = head(x, x - 0.1, x + 0.1, targets=t)
+    triple = head.tanh(*head.fc1(x, x - 0.1, x + 0.1))
+    assert all(torch.equal(a, e) for a, e in zip((y, worst), head.fc2(*triple, targets=t)))
+    new = pickle.loads(pickle.dumps(L.Predictor(8, 16, 3, dropout=0.5)))
+    assert new.drop.rate == 0.5 and new.groups is None
