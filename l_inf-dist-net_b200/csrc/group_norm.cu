@@ -174,7 +174,7 @@ template <int V, bool SAME> __device__ __forceinline__ Part* moments_at(Part* re
 }
 
 // Mean and variance of each group of the block over the CTA's rows from what the threads put into red; done(g, mean, variance) in one lane.
-// Parts of weights w_i join as mean = sum w_i mean_i, variance = sum w_i (variance_i + mean_i^2) - mean^2, about one part's shift.
+// Parts of weights w_i join as mean = sum w_i mean_i, variance = sum w_i (variance_i + mean_i^2) - mean^2, about one part's mean.
 template <int V, bool SAME, typename Done>
 __device__ __forceinline__ void join_moments(Part* red, const NormDims& d, const NormPlan& p, const NormBlock& b, const NormRows& share, Done done) {
     const int width = SAME ? p.tx : p.tx * V, lane = threadIdx.x & 31;
@@ -183,7 +183,7 @@ __device__ __forceinline__ void join_moments(Part* red, const NormDims& d, const
     if (p.rt > 1) {
         // columns along the rows
         by_columns(width, p.rt, [&](int c, int first, int step, auto join) {
-            const float k0 = c < width ? red[c].shift : 0.f, inv = 1.f / (float)share.all;
+            const float k0 = c < width ? red[c].shift + red[c].mean : 0.f, inv = 1.f / (float)share.all;
             float s = 0.f, q = 0.f;
             for (int r = first; r < p.rt; r += step) {
                 const Part v = red[r * width + c];
@@ -203,7 +203,7 @@ __device__ __forceinline__ void join_moments(Part* red, const NormDims& d, const
         const int g = g0 + lane / wide;
         float s = 0.f, q = 0.f, k0 = 0.f;
         if (g < b.ng) {
-            k0 = red[g * per].shift;
+            k0 = red[g * per].shift + red[g * per].mean;
             for (int c = lane & (wide - 1); c < per; c += wide) {
                 const Part v = red[g * per + c];
                 const float e = (v.shift - k0) + v.mean;
