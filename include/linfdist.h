@@ -407,8 +407,9 @@ int linf_group_norm_backward(const void* grad_output, const void* x, const void*
  * Bounds of a group norm with its activation over the box lower <= x <= upper, fp32, same layout: for every x in the box
  * output_lower <= activation(u) <= output_upper up to the rounding of the results.  The exact range of x_i - mean(x) is divided by
  * the range of the deviation, [max(0, std(c) - rho), std(c) + rho] with c the box's centre and rho the root mean square of
- * its radii.  sums [N, G, 4] (64 bits) is kept for the backward pass, or NULL.  Sums, and the whole backward pass, are computed in 64
- * bits; the bounds themselves in fp32, off by no more than a few roundings of their own terms.
+ * its radii.  sums [N, G, 4] (64 bits) is kept for the backward pass, or NULL.  Sums, and the backward pass
+ * but for the activation's slope and its product with a gradient, are computed in 64 bits; the bounds themselves in fp32, off by no more
+ * than a few roundings of their own terms, over all of fp32.
  */
 size_t linf_group_norm_bound_workspace_bytes(int N, int C, int G, int L, int backward);
 int linf_group_norm_bound_forward(const float* lower, const float* upper, const float* gamma, const float* beta, int N, int C, int G,

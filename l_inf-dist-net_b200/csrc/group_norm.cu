@@ -4,10 +4,11 @@
 //   dbeta = sum du, dgamma = sum du h (over samples and positions),
 //   dx = (gamma du - mean(gamma du) - h mean(gamma du h)) / sqrt(var + eps)
 //
-// What bounds it: kept and dense slabs the latency of load, reduction and store; two passes the instructions (a bf16 value with silu takes 12 to
-// 15, with dropout 25; 2.0 to 2.4 a clock are issued) before HBM, which sees x once or twice.  Measured on one B200, us: 32 x 320 x 64 x 64 bf16,
-// 32 groups, silu: 58 (sums 23, results 38 with what is left in L2; 26 if x and y crossed HBM once); 16 x 128 x 160 x 160 bf16, silu and dropout:
-// forward 83, backward 133; 64 x 128 x 16 x 16 fp32, tanh, kept: forward 11, backward 18.  Clusters of up to 8 CTAs that held larger slabs in
+// What bounds it: kept and dense slabs the latency of load, reduction and store; two passes latency as well, at 14 to 28 warps on an SM: a bf16
+// value with silu takes 12 to 15 instructions, with dropout 25, and 1.1 to 2.1 of 4 a clock are issued, while HBM, which sees x once or
+// twice, is at 31 to 51 % of its peak.  Measured on one B200, us: 32 x 320 x 64 x 64 bf16, 32 groups, silu: 57 (sums 21, results 40 one by one and
+// from HBM; 26 if x and y crossed HBM once); 16 x 128 x 160 x 160 bf16, silu and dropout: forward 83, backward 134; 64 x 128 x 16 x 16 fp32,
+// tanh, kept: forward 10, backward 19.  Clusters of up to 8 CTAs that held larger slabs in
 // their shared memory read x once, but loaded, reduced and stored in turn: 65 for the first, and 528 instead of 216 for the second, whose rows
 // they had to cut into pieces of 32 bytes.
 //

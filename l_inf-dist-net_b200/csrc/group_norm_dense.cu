@@ -4,7 +4,7 @@
 // slot keeps its group and goes through a range of samples, so that gamma and beta are read once and, in the backward pass, the
 // sums for their gradients stay in registers; the next sample's loads are on their way while one is reduced.  Bound by the
 // instructions and the latency of the reductions.  Measured on one B200, us, forward / forward and backward: 512 x 5120 fp32, 32 groups, tanh 12.5 /
-// -; 2048 x 5120 bf16, 32 groups, tanh 30 / 80; 2048 x 5120 fp32, one group, no activation 40 / 97.  (The kernels for maps, whose CTA begins
+// -; 2048 x 5120 bf16, 32 groups, tanh 30 / 82; 2048 x 5120 fp32, one group, no activation 40 / 97.  (The kernels for maps, whose CTA begins
 // anew for each sample, took 18.6 / -, 58 / 172 and 99 / 345.)
 #include "group_norm.cuh"
 
